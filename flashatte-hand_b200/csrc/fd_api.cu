@@ -381,6 +381,27 @@ bool is_short_launch(int64_t block_table_stride, int64_t page_block_size, int64_
   return bound <= simt_max_tokens();
 }
 
+int device_sms(int dev) { return ::device_sms(dev); }
+unsigned long long wait_timeout_ns() { return timeout_ns(); }
+bool pdl_enabled() { return ::pdl_enabled(); }
+int env_int(const char* name, int dflt, int lo, int hi) { return ::env_int(name, dflt, lo, hi); }
+void* library_workspace(int dev, size_t bytes, cudaStream_t stream, const char** why) {
+  return internal_workspace(dev, bytes, stream, why);
+}
+int64_t seqs_per_launch(int64_t per_seq_cost, int64_t aligned_cost, int64_t hkv, int grid) {
+  return ::seqs_per_launch(per_seq_cost, aligned_cost, hkv, grid);
+}
+bool tensor_maps_available() { return encode_fn() != nullptr; }
+CUresult encode_tensor_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* base,
+                           const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                           CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
+  const cuuint32_t estride[5] = {1, 1, 1, 1, 1};
+  return encode_fn()(m, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides,
+                     box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+int report_ok() { return set_ok(); }
+
 bool uses_tensor_core_path(const void* q, const void* k_cache, const void* v_cache,
                            int64_t headdim, int64_t qrows, int64_t page_block_size) {
   return headdim == kHeadDim && qrows <= kMaxGroup && pick_chunk(page_block_size) > 0 &&
@@ -414,6 +435,7 @@ const char* fd_error_string(int code) {
     case FD_ERR_CUDA: return "CUDA error";
     case FD_ERR_DEVICE_TIMEOUT: return "in-kernel wait timed out";
     case FD_ERR_BAD_PAGE: return "page id outside the KV pool";
+    case FD_ERR_NO_PAGES: return "not enough pages or slots for the step";
     default: return "unknown error";
   }
 }
@@ -1222,6 +1244,10 @@ int fd_device_status(void) {
     return set_error(FD_ERR_BAD_PAGE,
                      "a block_table entry inside a sequence's length was outside [0, num_blocks) "
                      "(those rows were read as zeros)");
+  if (word == FD_ERR_NO_PAGES)
+    return set_error(FD_ERR_NO_PAGES,
+                     "a step's new tokens did not all get slots: the pool ran out of pages, or a "
+                     "block table row or the slot map is too short");
   if (word == FD_ERR_DEVICE_TIMEOUT)
     return set_error(FD_ERR_DEVICE_TIMEOUT, "a bounded in-kernel wait ran out");
   return set_error(word, "device reported status %d", word);

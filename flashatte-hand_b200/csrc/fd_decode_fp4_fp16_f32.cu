@@ -1,0 +1,11 @@
+// fd_decode_fp4_fp16_f32.cu - fp16-query instantiations of the 4-bit-cache decode kernel, fp32 output.
+#include "fd_decode_fp4.cuh"
+
+namespace fd {
+
+cudaError_t launch_fp4_fp16_f32(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid,
+                          cudaStream_t stream) {
+  return launch_fp4<__half, float>(m, p, head_dim, grid, stream);
+}
+
+}  // namespace fd

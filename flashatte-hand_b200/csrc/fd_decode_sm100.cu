@@ -9,7 +9,7 @@ namespace fd {
 size_t sm100_smem_bytes() { return static_cast<size_t>(Geo<false>::kSmemBytes); }
 
 WorkspaceLayout workspace_layout(int64_t batch_per_launch, int64_t num_heads_k, int64_t qrows,
-                                 int grid_max) {
+                                 int grid_max, int head_dim) {
   auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
   const size_t pairs = static_cast<size_t>(batch_per_launch * num_heads_k);
   const size_t slots = pairs + static_cast<size_t>(grid_max);
@@ -19,7 +19,7 @@ WorkspaceLayout workspace_layout(int64_t batch_per_launch, int64_t num_heads_k, 
   w.tickets_off = 128; // one 64-bit arrival counter per (sequence, KV head) pair
   w.lse_off = up(w.tickets_off + pairs * 8);
   w.o_off = w.lse_off + up(slots * qrows * 4);
-  w.total = w.o_off + up(slots * qrows * kHeadDim * 4);
+  w.total = w.o_off + up(slots * qrows * head_dim * 4);
   return w;
 }
 

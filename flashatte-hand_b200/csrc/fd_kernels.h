@@ -98,6 +98,92 @@ cudaError_t launch_append_kv(const AppendParams& p, cudaStream_t stream);
 // 16-bit new rows (src_dtype 0 bf16, 1 fp16) into an e4m3 cache: x / scale[h], head_dim % 8 == 0.
 cudaError_t launch_append_kv_e4m3(const AppendParams& p, int src_dtype, cudaStream_t stream);
 
+// Packed rows to (append) or from (gather) cache slots.
+struct SlotParams {
+  const void* k; const void* v;          // append: [rows, Hkv, D] 16-bit, token strides below
+  int64_t k_stride, v_stride;            // elements from one row to the next
+  void* k_cache; void* v_cache;          // [num_blocks, page, Hkv, D] (4-bit: D / 2 bytes a row)
+  uint8_t* k_block; uint8_t* v_block;    // 4-bit: e4m3 block scales [num_blocks, Hkv, page, D / 16]
+  const float* k_scale; const float* v_scale;  // e4m3 and 4-bit: [Hkv]
+  void* k_out; void* v_out;              // gather: [rows, Hkv, D]
+  const int64_t* slot_map;               // [rows]; nullptr: dense rows placed by the table below
+  const int32_t* seqlens; const int32_t* block_table;
+  int64_t bt_stride, num_blocks, rows;
+  int seqlen_new, num_heads_k, head_dim, page;
+  int rows_per_cta;                      // set by the launcher
+  int* err;
+};
+cudaError_t launch_append_slots(const SlotParams& p, int src_dtype, int cache_dtype, cudaStream_t stream);
+// 16-bit caches whose rows the 16-byte path cannot take.
+cudaError_t launch_append_slots_narrow(const SlotParams& p, cudaStream_t stream);
+cudaError_t launch_gather_slots(const SlotParams& p, int cache_dtype, int out_dtype, cudaStream_t stream);
+
+// Block tables and slot maps (fd_pages.cu).
+constexpr int kMaxPagedRequests = 8192;
+struct AssignPagesParams {
+  int32_t* block_table;          // [B, bt_stride]
+  const int32_t* seqlens;        // [B] stored tokens
+  const int32_t* new_lens;       // [B] tokens of this step
+  const int32_t* free_pages;     // [num_blocks] stack of free page ids
+  int32_t* free_count;           // [0] entries of the stack, [1] arrivals (0 between calls)
+  int32_t* seqlens_out;          // [B], may be seqlens
+  int32_t* cu_new;               // [B + 1]
+  int64_t* slot_map;             // [num_slots]
+  int64_t bt_stride, num_blocks, num_slots;
+  int batch, page;
+  int* err;
+};
+struct ReleasePagesParams {
+  int32_t* block_table;
+  const int32_t* seqlens;
+  const int32_t* keep_lens;
+  int32_t* free_pages;
+  int32_t* free_count;
+  int64_t bt_stride, num_blocks;
+  int batch, page;
+  int* err;
+};
+cudaError_t launch_assign_pages(const AssignPagesParams& p, int sms, cudaStream_t stream);
+cudaError_t launch_release_pages(const ReleasePagesParams& p, cudaStream_t stream);
+
+// Decode over a 4-bit block-scaled cache (fd_decode_fp4.cuh).
+struct Fp4DecodeParams {
+  const void* q;                 // [B, seqlen_q, Hq, D]
+  void* out;                     // [B, seqlen_q, Hq, D]
+  float* lse;                    // [B, Hq, seqlen_q], nullable
+  const float* k_scale;          // [Hkv]
+  const float* v_scale;
+  const int32_t* seqlens;
+  const int32_t* block_table;
+  int64_t bt_stride, num_blocks;
+  int batch, num_heads, num_heads_k, group, page, chunk;
+  int seqlen_q, causal, qrows;   // qrows = seqlen_q * group
+  int row_tiles, rows;           // query rows are taken `rows` at a time, in row_tiles passes
+  int len_add;
+  float scale_log2;
+  float* part_o;                 // [slots, rows, D] normalised partial O
+  float* part_lse;               // [slots, rows] log2-domain partial LSE
+  unsigned long long* tickets;   // arrival counters, as DecodeParams::tickets
+  unsigned long long* epoch_word;
+  int* err;
+  unsigned long long timeout_ns;
+  int cost_tile, cost_seg, cost_floor;
+  int pdl;
+};
+struct Fp4TensorMaps {
+  CUtensorMap k, v, k_block, v_block;
+};
+// Query rows of one pass for this head dim (8 or 16).
+int fp4_rows(int head_dim, int64_t qrows);
+// Most CTAs a launch uses on a device of `sms` SMs.
+int fp4_max_grid(int head_dim, int rows, int sms);
+cudaError_t launch_fp4_bf16(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream);
+cudaError_t launch_fp4_bf16_f32(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream);
+cudaError_t launch_fp4_fp16(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream);
+cudaError_t launch_fp4_fp16_f32(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream);
+cudaError_t launch_decode_fp4(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim,
+                              int q_dtype, bool out_fp32, int grid, cudaStream_t stream);
+
 // Workspace carve-up for the tensor-core kernel: [epoch_off, lse_off) must
 // be zero before the workspace's first use (the kernel keeps it consistent
 // afterwards); the partials after it need no initial value.
@@ -105,7 +191,7 @@ struct WorkspaceLayout {
   size_t epoch_off, done_off, tickets_off, lse_off, o_off, total;
 };
 WorkspaceLayout workspace_layout(int64_t batch_per_launch, int64_t num_heads_k, int64_t qrows,
-                                 int grid_max);
+                                 int grid_max, int head_dim = kHeadDim);
 
 // TMA descriptors of one launch: q [B, sq, Hq, 128] (box 64 x group x sq), K and
 // V caches [num_blocks, page, Hkv, 128] with `chunk`-token boxes for full
@@ -150,9 +236,10 @@ cudaError_t launch_bounded_wait_probe(unsigned long long budget_ns, int* status,
 
 size_t sm100_smem_bytes();
 
-// Device status word codes (match FD_ERR_DEVICE_TIMEOUT / FD_ERR_BAD_PAGE).
+// Device status word codes (match FD_ERR_DEVICE_TIMEOUT / FD_ERR_BAD_PAGE / FD_ERR_NO_PAGES).
 constexpr int kStatusTimeout = 5;
 constexpr int kStatusBadPage = 6;
+constexpr int kStatusNoPages = 7;
 
 // Address of the current device's status word (a __device__ int inside this
 // library, looked up once per device); nullptr if the lookup failed.
@@ -168,6 +255,22 @@ bool is_short_launch(int64_t block_table_stride, int64_t page_block_size, int64_
 // uses split scratch) rather than the CUDA-core kernel, which needs none.
 bool uses_tensor_core_path(const void* q, const void* k_cache, const void* v_cache,
                            int64_t headdim, int64_t qrows, int64_t page_block_size);
+
+// What the entry points outside fd_api.cu share with it.
+int device_sms(int dev);
+unsigned long long wait_timeout_ns();
+bool pdl_enabled();
+int env_int(const char* name, int dflt, int lo, int hi);
+// Library-owned workspace of (current device `dev`, `stream`); nullptr and *why on failure.
+void* library_workspace(int dev, size_t bytes, cudaStream_t stream, const char** why);
+// Sequences a launch of `grid` CTAs may take (see fd_api.cu); 0: not even one fits.
+int64_t seqs_per_launch(int64_t per_seq_cost, int64_t aligned_cost, int64_t hkv, int grid);
+// cuTensorMapEncodeTiled with interleave and out-of-bounds fill none.
+bool tensor_maps_available();
+CUresult encode_tensor_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* base,
+                           const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                           CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion);
+int report_ok();
 
 // Record `code` and a printf-style message as this thread's last error (what
 // fd_last_error / fd_last_error_message report) and return `code`.

@@ -19,10 +19,12 @@ import math
 
 import torch
 
-from ._lib import (FD_DTYPE_BF16, FD_DTYPE_FP16, FD_DTYPE_FP32, FlashDecodeError, check,
-                   load_library)
+from ._lib import (FD_DTYPE_BF16, FD_DTYPE_E2M1, FD_DTYPE_E4M3, FD_DTYPE_FP16, FD_DTYPE_FP32,
+                   FlashDecodeError, check, load_library)
 
 _DTYPES = {torch.bfloat16: FD_DTYPE_BF16, torch.float16: FD_DTYPE_FP16}
+_CACHE_DTYPES = {torch.bfloat16: FD_DTYPE_BF16, torch.float16: FD_DTYPE_FP16,
+                 torch.float8_e4m3fn: FD_DTYPE_E4M3, torch.float4_e2m1fn_x2: FD_DTYPE_E2M1}
 _OUT_DTYPES = {torch.bfloat16: FD_DTYPE_BF16, torch.float16: FD_DTYPE_FP16, torch.float32: FD_DTYPE_FP32}
 
 
@@ -94,7 +96,8 @@ def flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                  stream: torch.cuda.Stream | None = None, lse: torch.Tensor | None = None,
                  causal: bool = False, k: torch.Tensor | None = None,
                  v: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
-                 v_scale: torch.Tensor | None = None):
+                 v_scale: torch.Tensor | None = None, k_block_scale: torch.Tensor | None = None,
+                 v_block_scale: torch.Tensor | None = None):
     """Paged decode attention for seqlen_q >= 1 query tokens per sequence.
 
     q [B, sq, Hq, D]; k_cache/v_cache [num_blocks, page, Hkv, D];
@@ -116,10 +119,17 @@ def flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     bf16 or fp16 and k / v, when given, are 16-bit rows quantised into the
     cache.  Head dim 128, seqlen_q * (Hq / Hkv) <= 16, pages of a multiple
     of 16 tokens.
+
+    4-bit cache: k_cache / v_cache of dtype torch.float4_e2m1fn_x2
+    [num_blocks, page, Hkv, D / 2] with block scales k_block_scale /
+    v_block_scale torch.float8_e4m3fn [num_blocks, Hkv, page, D / 16] (one
+    for 16 consecutive values) and k_scale / v_scale fp32 [Hkv]: the attended
+    key is e2m1 * block scale * k_scale[h].  Otherwise as the FP8 cache, with
+    head dim 64, 128 or 256 and any number of query rows.
     """
     call = _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale,
                     return_softmax_lse, out, out_dtype, max_seqlen_k, workspace, lse, causal, k, v,
-                    k_scale, v_scale)
+                    k_scale, v_scale, k_block_scale, v_block_scale)
     with _on_device(q.device):
         check(call.fn(*call.args, _stream_handle(stream, q.device)))
     return (call.out, call.lse) if call.return_lse else call.out
@@ -136,7 +146,8 @@ class _Call:
 
 
 def _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, return_softmax_lse,
-             out, out_dtype, max_seqlen_k, workspace, lse, causal, k, v, k_scale, v_scale) -> _Call:
+             out, out_dtype, max_seqlen_k, workspace, lse, causal, k, v, k_scale, v_scale,
+             k_block_scale=None, v_block_scale=None) -> _Call:
     """Check the arguments of flash_decode, allocate the outputs it was not
     given and bind the C entry point that serves them."""
     lib = load_library()
@@ -144,12 +155,15 @@ def _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, ret
     if q.dim() != 4:
         raise ValueError(f"q must be [B, seqlen_q, Hq, D], got {tuple(q.shape)}")
     kv8 = k_cache.dtype == torch.float8_e4m3fn
-    if q.dtype not in _DTYPES or v_cache.dtype != k_cache.dtype or (not kv8 and k_cache.dtype != q.dtype):
-        raise ValueError("q, k_cache, v_cache must share dtype bf16 or fp16 (or e4m3 caches)")
-    if kv8:
+    kv4 = k_cache.dtype == torch.float4_e2m1fn_x2
+    if q.dtype not in _DTYPES or v_cache.dtype != k_cache.dtype \
+            or not (kv8 or kv4 or k_cache.dtype == q.dtype):
+        raise ValueError("q, k_cache, v_cache must share dtype bf16 or fp16 (or e4m3 or e2m1 caches)")
+    if kv8 or kv4:
         _check_scales(k_scale, v_scale, k_cache.shape[2])
     elif k_scale is not None or v_scale is not None:
-        raise ValueError("k_scale / v_scale apply to float8_e4m3fn caches only")
+        raise ValueError("k_scale / v_scale apply to float8_e4m3fn and float4_e2m1fn_x2 caches only")
+    _check_block_scales(k_block_scale, v_block_scale, k_cache)
     if cache_seqlens.dtype != torch.int32 or block_table.dtype != torch.int32:
         raise ValueError("cache_seqlens and block_table must be int32")
     for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache),
@@ -158,7 +172,7 @@ def _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, ret
             raise ValueError(f"{name} must be contiguous")
     B, sq, Hq, D = q.shape
     num_blocks, page, Hkv, Dk = k_cache.shape
-    if tuple(v_cache.shape) != tuple(k_cache.shape) or Dk != D:
+    if tuple(v_cache.shape) != tuple(k_cache.shape) or (2 * Dk if kv4 else Dk) != D:
         raise ValueError("k_cache/v_cache shape mismatch")
     if block_table.dim() != 2 or block_table.shape[0] != B or cache_seqlens.shape != (B,):
         raise ValueError("block_table must be [B, max_blocks] and cache_seqlens [B]")
@@ -182,6 +196,15 @@ def _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, ret
         raise ValueError("k and v must be given together")
     causal_i = 1 if causal else 0
     max_len = int(max_seqlen_k or 0)
+    if kv4:
+        if k is not None:
+            _check_new_kv(k, v, k_cache, B, q.dtype)
+        args = (_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_block_scale), _ptr(v_block_scale),
+                _ptr(k_scale), _ptr(v_scale), _ptr(k), _ptr(v), 0 if k is None else k.shape[1],
+                _ptr(out), _ptr(lse), _ptr(cache_seqlens), _ptr(block_table),
+                int(block_table.shape[1]), B, sq, Hq, Hkv, D, page, num_blocks, _DTYPES[q.dtype],
+                _OUT_DTYPES[odt], scale, causal_i, max_len, ws_ptr, ws_bytes)
+        return _Call(lib.fd_decode_paged_fp4, args, out, lse, return_softmax_lse)
     if kv8:
         if k is not None:
             _check_new_kv(k, v, k_cache, B, q.dtype)
@@ -222,13 +245,13 @@ class DecodePlan:
     def __init__(self, q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale=None,
                  return_softmax_lse=False, out=None, out_dtype=None, max_seqlen_k=None,
                  workspace=None, lse=None, causal=False, k=None, v=None, k_scale=None,
-                 v_scale=None):
+                 v_scale=None, k_block_scale=None, v_block_scale=None):
         self._call = _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale,
                               return_softmax_lse, out, out_dtype, max_seqlen_k, workspace, lse,
-                              causal, k, v, k_scale, v_scale)
+                              causal, k, v, k_scale, v_scale, k_block_scale, v_block_scale)
         self._device = q.device
         self._keep = (q, k_cache, v_cache, cache_seqlens, block_table, workspace, k, v, k_scale,
-                      v_scale)
+                      v_scale, k_block_scale, v_block_scale)
 
     @property
     def out(self) -> torch.Tensor:
@@ -248,10 +271,30 @@ class DecodePlan:
 def _check_scales(k_scale, v_scale, Hkv: int) -> None:
     for name, sc in (("k_scale", k_scale), ("v_scale", v_scale)):
         if sc is None:
-            raise ValueError(f"{name} [Hkv] fp32 is required with a float8_e4m3fn cache")
+            raise ValueError(f"{name} [Hkv] fp32 is required with a float8_e4m3fn or "
+                             "float4_e2m1fn_x2 cache")
         _require_cuda(sc)
         if sc.dtype != torch.float32 or sc.shape != (Hkv,) or not sc.is_contiguous():
             raise ValueError(f"{name} must be a contiguous fp32 [{Hkv}] tensor")
+
+
+def _check_block_scales(k_block_scale, v_block_scale, k_cache: torch.Tensor) -> None:
+    """Block scales are given exactly with a 4-bit cache, in its shape."""
+    if k_cache.dtype != torch.float4_e2m1fn_x2:
+        if k_block_scale is not None or v_block_scale is not None:
+            raise ValueError("k_block_scale / v_block_scale apply to float4_e2m1fn_x2 caches only")
+        return
+    if k_cache.dim() != 4 or k_cache.shape[3] % 8 != 0:
+        raise ValueError("a float4_e2m1fn_x2 cache is [num_blocks, page, Hkv, D / 2] with D a "
+                         "multiple of 16")
+    num_blocks, page, Hkv, half = k_cache.shape
+    want = (num_blocks, Hkv, page, half // 8)
+    for name, sc in (("k_block_scale", k_block_scale), ("v_block_scale", v_block_scale)):
+        if sc is None:
+            raise ValueError(f"{name} is required with a float4_e2m1fn_x2 cache")
+        _require_cuda(sc)
+        if sc.dtype != torch.float8_e4m3fn or tuple(sc.shape) != want or not sc.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float8_e4m3fn {want} tensor")
 
 
 def _check_new_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, B: int,
@@ -259,7 +302,8 @@ def _check_new_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, B: in
     _require_cuda(k, v)
     if k.dim() != 4 or tuple(v.shape) != tuple(k.shape):
         raise ValueError("k and v must both be [B, seqlen_new, Hkv, D]")
-    if k.shape[0] != B or k.shape[2] != k_cache.shape[2] or k.shape[3] != k_cache.shape[3]:
+    D = k_cache.shape[3] * (2 if k_cache.dtype == torch.float4_e2m1fn_x2 else 1)
+    if k.shape[0] != B or k.shape[2] != k_cache.shape[2] or k.shape[3] != D:
         raise ValueError("k / v shape does not match the batch and cache heads")
     want = k_cache.dtype if new_dtype is None else new_dtype
     if k.dtype != want or v.dtype != want:
@@ -271,11 +315,13 @@ def _check_new_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, B: in
 def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
               cache_seqlens: torch.Tensor, block_table: torch.Tensor,
               stream: torch.cuda.Stream | None = None, k_scale: torch.Tensor | None = None,
-              v_scale: torch.Tensor | None = None) -> None:
+              v_scale: torch.Tensor | None = None, k_block_scale: torch.Tensor | None = None,
+              v_block_scale: torch.Tensor | None = None) -> None:
     """Write k / v [B, seqlen_new, Hkv, D] into the paged cache at positions
     cache_seqlens[b] + t (the cache update of flash_attn_with_kvcache).  For
     float8_e4m3fn caches k / v are 16-bit and stored as e4m3(x / scale[h])
-    with the fp32 [Hkv] k_scale / v_scale."""
+    with the fp32 [Hkv] k_scale / v_scale; float4_e2m1fn_x2 caches also take
+    the block scales to write (see flash_decode)."""
     lib = load_library()
     _require_cuda(k_cache, v_cache, cache_seqlens, block_table)
     if cache_seqlens.dtype != torch.int32 or block_table.dtype != torch.int32:
@@ -283,12 +329,29 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     if not (k_cache.is_contiguous() and v_cache.is_contiguous() and block_table.is_contiguous()):
         raise ValueError("caches and block_table must be contiguous")
     kv8 = k_cache.dtype == torch.float8_e4m3fn
-    if (k_cache.dtype not in _DTYPES and not kv8) or v_cache.dtype != k_cache.dtype \
+    if k_cache.dtype not in _CACHE_DTYPES or v_cache.dtype != k_cache.dtype \
             or tuple(v_cache.shape) != tuple(k_cache.shape):
-        raise ValueError("k_cache/v_cache must be bf16, fp16 or float8_e4m3fn with equal shapes")
+        raise ValueError("k_cache/v_cache must be bf16, fp16, float8_e4m3fn or float4_e2m1fn_x2 "
+                         "with equal shapes")
     B = block_table.shape[0]
     num_blocks, page, Hkv, D = k_cache.shape
+    _check_block_scales(k_block_scale, v_block_scale, k_cache)
     st = stream if stream is not None else torch.cuda.current_stream(k.device)
+    if k_cache.dtype == torch.float4_e2m1fn_x2:
+        _check_scales(k_scale, v_scale, Hkv)
+        if k.dtype not in _DTYPES:
+            raise ValueError("k / v must be bf16 or fp16")
+        _check_new_kv(k, v, k_cache, B, k.dtype)
+        if cache_seqlens.shape != (B,) or not cache_seqlens.is_contiguous():
+            raise ValueError("cache_seqlens must be a contiguous [B] tensor")
+        with torch.cuda.device(k.device):
+            status = lib.fd_append_kv_paged_fp4(
+                _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(k_block_scale),
+                _ptr(v_block_scale), _ptr(k_scale), _ptr(v_scale), _ptr(cache_seqlens),
+                _ptr(block_table), int(block_table.shape[1]), B, k.shape[1], Hkv, 2 * D, page,
+                num_blocks, _DTYPES[k.dtype], st.cuda_stream)
+        check(status)
+        return
     if kv8:
         _check_scales(k_scale, v_scale, Hkv)
         if k.dtype not in _DTYPES:
@@ -308,6 +371,181 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
             int(block_table.shape[1]), B, k.shape[1], Hkv, D, page, num_blocks, _DTYPES[k.dtype],
             st.cuda_stream)
     check(status)
+
+
+def _check_slot_cache(k_cache, v_cache, slot_map, k_scale, v_scale, k_block_scale, v_block_scale):
+    """Checks that append_kv_slots and gather_kv share; returns (T, page,
+    Hkv, D, num_blocks) of the call."""
+    _require_cuda(k_cache, v_cache, slot_map)
+    if k_cache.dtype not in _CACHE_DTYPES or v_cache.dtype != k_cache.dtype or k_cache.dim() != 4 \
+            or v_cache.shape != k_cache.shape:
+        raise ValueError("k_cache/v_cache must be bf16, fp16, float8_e4m3fn or float4_e2m1fn_x2 "
+                         "[num_blocks, page, Hkv, D] tensors with equal shapes")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("caches must be contiguous")
+    if slot_map.dtype != torch.int64 or slot_map.dim() != 1 or not slot_map.is_contiguous():
+        raise ValueError("slot_map must be a contiguous int64 [T] tensor")
+    num_blocks, page, Hkv, D = k_cache.shape
+    if k_cache.dtype in _DTYPES:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("k_scale / v_scale apply to float8_e4m3fn and float4_e2m1fn_x2 caches only")
+    else:
+        _check_scales(k_scale, v_scale, Hkv)
+    _check_block_scales(k_block_scale, v_block_scale, k_cache)
+    return (slot_map.shape[0], page, Hkv, 2 * D if k_cache.dtype == torch.float4_e2m1fn_x2 else D,
+            num_blocks)
+
+
+def append_kv_slots(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    slot_map: torch.Tensor, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None, k_block_scale: torch.Tensor | None = None,
+                    v_block_scale: torch.Tensor | None = None,
+                    stream: torch.cuda.Stream | None = None) -> None:
+    """Write packed rows k / v [T, Hkv, D] (bf16 or fp16) into the paged cache
+    at slot_map [T] int64: slot = page id * page + row in the page, as
+    assign_pages gives them; negative slots are skipped.  The rows may have
+    any stride from token to token (a slice of a fused projection); the cache
+    is of any kind flash_decode reads, and quantised ones take their scales.
+    The slots should be distinct."""
+    lib = load_library()
+    T, page, Hkv, D, num_blocks = _check_slot_cache(k_cache, v_cache, slot_map, k_scale, v_scale,
+                                                    k_block_scale, v_block_scale)
+    _require_cuda(k, v)
+    if k.dtype not in _DTYPES or v.dtype != k.dtype:
+        raise ValueError("k / v must be bf16 or fp16")
+    if k_cache.dtype in _DTYPES and k.dtype != k_cache.dtype:
+        raise ValueError(f"k / v must be {k_cache.dtype}")
+    for name, x in (("k", k), ("v", v)):
+        if tuple(x.shape) != (T, Hkv, D):
+            raise ValueError(f"{name} must be [T, Hkv, D] = {(T, Hkv, D)}, got {tuple(x.shape)}")
+        if T > 0 and ((D > 1 and x.stride(2) != 1) or (Hkv > 1 and x.stride(1) != D)
+                      or (T > 1 and x.stride(0) < Hkv * D)):
+            raise ValueError(f"the heads of a token of {name} must be contiguous")
+    row = Hkv * D
+    with _on_device(k_cache.device):
+        check(lib.fd_append_kv_slots(
+            _ptr(k), k.stride(0) if T > 1 else row, _ptr(v), v.stride(0) if T > 1 else row,
+            _ptr(k_cache), _ptr(v_cache), _ptr(k_block_scale), _ptr(v_block_scale), _ptr(k_scale),
+            _ptr(v_scale), _ptr(slot_map), T, Hkv, D, page, num_blocks, _DTYPES[k.dtype],
+            _CACHE_DTYPES[k_cache.dtype], _stream_handle(stream, k_cache.device)))
+
+
+def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_map: torch.Tensor,
+              k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+              k_block_scale: torch.Tensor | None = None, v_block_scale: torch.Tensor | None = None,
+              out_dtype: torch.dtype | None = None, k_out: torch.Tensor | None = None,
+              v_out: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None):
+    """The cache rows at slot_map [T] int64 as values: k, v [T, Hkv, D] of
+    out_dtype (default: the cache's type, bf16 for quantised caches), zeros at
+    negative slots.  The inverse of append_kv_slots."""
+    lib = load_library()
+    T, page, Hkv, D, num_blocks = _check_slot_cache(k_cache, v_cache, slot_map, k_scale, v_scale,
+                                                    k_block_scale, v_block_scale)
+    if out_dtype is None:
+        out_dtype = k_out.dtype if k_out is not None else \
+            k_cache.dtype if k_cache.dtype in _DTYPES else torch.bfloat16
+    if out_dtype not in _OUT_DTYPES:
+        raise ValueError("out_dtype must be bf16, fp16 or fp32")
+    outs = []
+    for name, x in (("k_out", k_out), ("v_out", v_out)):
+        if x is None:
+            x = torch.empty((T, Hkv, D), dtype=out_dtype, device=k_cache.device)
+        elif not x.is_cuda or x.dtype != out_dtype or tuple(x.shape) != (T, Hkv, D) \
+                or not x.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {out_dtype} {(T, Hkv, D)} CUDA tensor")
+        outs.append(x)
+    with _on_device(k_cache.device):
+        check(lib.fd_gather_kv_slots(
+            _ptr(k_cache), _ptr(v_cache), _ptr(k_block_scale), _ptr(v_block_scale), _ptr(k_scale),
+            _ptr(v_scale), _ptr(slot_map), T, _ptr(outs[0]), _ptr(outs[1]), Hkv, D, page, num_blocks,
+            _CACHE_DTYPES[k_cache.dtype], _OUT_DTYPES[out_dtype],
+            _stream_handle(stream, k_cache.device)))
+    return outs[0], outs[1]
+
+
+def _check_pool(block_table, lens: dict, free_pages, free_count) -> int:
+    """Checks that assign_pages and release_pages share; returns B."""
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [B, max_blocks]")
+    B = block_table.shape[0]
+    tensors = {"block_table": block_table, "free_pages": free_pages, "free_count": free_count, **lens}
+    for name, t in tensors.items():
+        if not t.is_cuda:
+            raise ValueError("flashdecode runs on CUDA tensors only (no CPU path)")
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor")
+    for name, t in lens.items():
+        if t.shape != (B,):
+            raise ValueError(f"{name} must be [B] = [{B}]")
+    if free_pages.dim() != 1 or free_count.shape != (2,):
+        raise ValueError("free_pages must be [num_blocks] and free_count [2]")
+    return B
+
+
+def assign_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, new_lens: torch.Tensor,
+                 free_pages: torch.Tensor, free_count: torch.Tensor, page_block_size: int,
+                 slot_map: torch.Tensor | None = None, num_slots: int | None = None,
+                 cu_new_lens: torch.Tensor | None = None, seqlens_out: torch.Tensor | None = None,
+                 stream: torch.cuda.Stream | None = None):
+    """Pages and cache slots for a step's new tokens, on the device.
+
+    Request b holds cache_seqlens[b] tokens in the pages of its block_table
+    row and gets new_lens[b] more.  Pages come off the top of the stack
+    free_pages [num_blocks] int32 (its size is the cache's number of pages),
+    of which free_count[0] entries are free, in the order of the requests, and
+    are entered in block_table; free_count [2] int32 starts as (free, 0) and
+    its second word belongs to the library.
+
+    Returns (slot_map, cu_new_lens, seqlens_out): the slot of each packed new
+    token (int64; give a slot_map buffer of fixed size, e.g. for a CUDA graph,
+    or num_slots = the step's tokens; -1 behind the last token), the prefix
+    sums of new_lens [B + 1], and the lengths afterwards (a buffer may be
+    given; cache_seqlens itself updates them in place).  A request that does
+    not fit gets nothing (slots -1, length unchanged) and device_status()
+    reports FD_ERR_NO_PAGES; requests are served in order.
+    """
+    lib = load_library()
+    B = _check_pool(block_table, {"cache_seqlens": cache_seqlens, "new_lens": new_lens}, free_pages,
+                    free_count)
+    dev = block_table.device
+    if slot_map is None:
+        if num_slots is None:
+            raise ValueError("give slot_map or num_slots")
+        slot_map = torch.empty((int(num_slots),), dtype=torch.int64, device=dev)
+    elif not slot_map.is_cuda or slot_map.dtype != torch.int64 or slot_map.dim() != 1 \
+            or not slot_map.is_contiguous():
+        raise ValueError("slot_map must be a contiguous int64 [num_slots] CUDA tensor")
+    if cu_new_lens is None:
+        cu_new_lens = torch.empty((B + 1,), dtype=torch.int32, device=dev)
+    if seqlens_out is None:
+        seqlens_out = torch.empty((B,), dtype=torch.int32, device=dev)
+    for name, t, n in (("cu_new_lens", cu_new_lens, B + 1), ("seqlens_out", seqlens_out, B)):
+        if not t.is_cuda or t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 [{n}] CUDA tensor")
+    with _on_device(dev):
+        check(lib.fd_assign_pages(
+            _ptr(block_table), block_table.shape[1], _ptr(cache_seqlens), _ptr(new_lens),
+            _ptr(free_pages), _ptr(free_count), B, int(page_block_size), free_pages.shape[0],
+            _ptr(seqlens_out), _ptr(cu_new_lens), _ptr(slot_map), slot_map.shape[0],
+            _stream_handle(stream, dev)))
+    return slot_map, cu_new_lens, seqlens_out
+
+
+def release_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, keep_lens: torch.Tensor,
+                  free_pages: torch.Tensor, free_count: torch.Tensor, page_block_size: int,
+                  stream: torch.cuda.Stream | None = None) -> None:
+    """Give back the pages of cache_seqlens[b] tokens that keep_lens[b] tokens
+    do not need (0: the request is finished).  Their block_table entries
+    become -1; the lengths are not changed.  Releasing what the last
+    assign_pages took leaves the stack as it was."""
+    lib = load_library()
+    B = _check_pool(block_table, {"cache_seqlens": cache_seqlens, "keep_lens": keep_lens}, free_pages,
+                    free_count)
+    with _on_device(block_table.device):
+        check(lib.fd_release_pages(
+            _ptr(block_table), block_table.shape[1], _ptr(cache_seqlens), _ptr(keep_lens),
+            _ptr(free_pages), _ptr(free_count), B, int(page_block_size), free_pages.shape[0],
+            _stream_handle(stream, block_table.device)))
 
 
 def combine_lse(part_o: torch.Tensor, part_lse: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,
@@ -339,5 +577,6 @@ def combine_lse(part_o: torch.Tensor, part_lse: torch.Tensor, out_dtype: torch.d
     return (out, lse) if return_lse else out
 
 
-__all__ = ["run_kernel", "flash_decode", "DecodePlan", "append_kv", "combine_lse", "last_error",
-           "device_status", "workspace_size", "FlashDecodeError"]
+__all__ = ["run_kernel", "flash_decode", "DecodePlan", "append_kv", "append_kv_slots", "gather_kv",
+           "assign_pages", "release_pages", "combine_lse", "last_error", "device_status",
+           "workspace_size", "FlashDecodeError"]

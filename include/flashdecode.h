@@ -29,6 +29,7 @@ extern "C" {
 #define FD_DTYPE_FP16 1
 #define FD_DTYPE_FP32 2 /* output only */
 #define FD_DTYPE_E4M3 3 /* K/V cache only (fd_decode_paged_fp8) */
+#define FD_DTYPE_E2M1 4 /* K/V cache only, block-scaled (fd_decode_paged_fp4) */
 
 /* status codes */
 #define FD_OK 0
@@ -40,6 +41,8 @@ extern "C" {
 #define FD_ERR_BAD_PAGE 6       /* a block_table id inside a sequence's range
                                    lies outside [0, num_blocks) (reported by
                                    fd_device_status; those rows read as 0)   */
+#define FD_ERR_NO_PAGES 7       /* a step's new tokens did not all get slots
+                                   (fd_assign_pages, by fd_device_status)    */
 
 /*
  * run_kernel - drop-in for the reference operator surface.
@@ -218,6 +221,145 @@ int fd_append_kv_paged_fp8(const void* k_new, const void* v_new, void* k_cache, 
                            int64_t num_blocks, int src_dtype, void* stream);
 
 /*
+ * The 4-bit block-scaled cache (FD_DTYPE_E2M1): the row of headdim values of
+ * one token and KV head is stored as headdim / 2 bytes of e2m1 codes (two a
+ * byte, the even element in the low half; e2m1 holds +-{0 .5 1 1.5 2 3 4 6})
+ * and headdim / 16 e4m3 scales, one for each 16 consecutive values:
+ *   value = e2m1 * block scale * k_scale[h]   (v_scale[h] for V).
+ * k_cache / v_cache             [num_blocks, page, Hkv, headdim / 2] bytes
+ * k_block_scale / v_block_scale [num_blocks, Hkv, page, headdim / 16] e4m3
+ * k_scale / v_scale             [Hkv] fp32, positive
+ * Quantising 16 values x with largest magnitude a: block scale
+ * s = e4m3(a / (6 k_scale[h])), saturated at 448; codes e2m1(x / (s k_scale[h])),
+ * saturated at 6; both rounded to nearest even in fp32.  s = 0 stores zeros; a
+ * NaN among the values makes the block's scale NaN.  A token costs 0.28 of the
+ * bytes of a 16-bit cache and 0.56 of an e4m3 one.
+ *
+ * fd_decode_paged_fp4 - fd_decode_paged_mq over such a cache, with an optional
+ * append as in fd_decode_paged_fp8 (k_new / v_new 16-bit rows of q's type
+ * [B, seqlen_new, Hkv, headdim], or NULL for both).  Supported: headdim 64,
+ * 128 or 256, any number of query rows, page a multiple of 16, 16-byte aligned
+ * q, new rows, caches and block scales (FD_ERR_UNSUPPORTED otherwise).  Workspace: at least
+ * fd_decode_workspace_size_fp4(...) bytes, 256-byte aligned and zero-filled
+ * before its first use, or NULL (as for fd_decode_paged).
+ * Replaces: nothing in the reference (its caches are bf16, best :1186-1211).
+ */
+int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_block_scale,
+                        void* v_block_scale, const float* k_scale, const float* v_scale,
+                        const void* k_new, const void* v_new, int64_t seqlen_new, void* out,
+                        float* lse, const int32_t* cache_seqlens, const int32_t* block_table,
+                        int64_t block_table_stride, int64_t batch_size, int64_t seqlen_q,
+                        int64_t num_heads, int64_t num_heads_k, int64_t headdim,
+                        int64_t page_block_size, int64_t num_blocks, int q_dtype, int out_dtype,
+                        float softmax_scale, int causal, int64_t max_seqlen_k, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Workspace bytes fd_decode_paged_fp4 needs (0 for unsupported shapes). */
+size_t fd_decode_workspace_size_fp4(int64_t batch_size, int64_t seqlen_q, int64_t num_heads,
+                                    int64_t num_heads_k, int64_t headdim);
+
+/*
+ * fd_append_kv_paged_fp4 - fd_append_kv_paged into a 4-bit block-scaled cache:
+ * the 16-bit rows (src_dtype bf16 or fp16, 16-byte aligned) are quantised as
+ * above.  headdim a multiple of 16; block scales given.
+ * Replaces: nothing in the reference (see fd_decode_paged_fp4).
+ */
+int fd_append_kv_paged_fp4(const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+                           void* k_block_scale, void* v_block_scale, const float* k_scale,
+                           const float* v_scale, const int32_t* cache_seqlens,
+                           const int32_t* block_table, int64_t block_table_stride,
+                           int64_t batch_size, int64_t seqlen_new, int64_t num_heads_k,
+                           int64_t headdim, int64_t page_block_size, int64_t num_blocks,
+                           int src_dtype, void* stream);
+
+/*
+ * fd_append_kv_slots - write packed new rows into the paged cache by slot.
+ *
+ * Replaces: nothing in the reference (the cache update of
+ * flash_attn_with_kvcache takes the same number of rows for every sequence;
+ * this takes the packed rows of a batch of any lengths).  k_new / v_new are
+ * [num_tokens, Hkv, headdim] with the given strides from one token to the
+ * next (in elements; a token's heads are contiguous, so a slice of a fused
+ * projection serves); row t is stored at slot slot_map[t] = page id *
+ * page_block_size + row in the page.  Negative slots are skipped (padding); a
+ * slot past the pool is skipped and reported (FD_ERR_BAD_PAGE by
+ * fd_device_status).  The slots of a call should be distinct: of two rows with
+ * one slot it is not defined which is kept, and they may be mixed.
+ * cache_dtype: src_dtype, FD_DTYPE_E4M3 (with k_scale / v_scale, quantised as
+ * by fd_append_kv_paged_fp8) or FD_DTYPE_E2M1 (with block scales too).  The
+ * last two need headdim a multiple of 16, and 16-byte aligned rows and caches.
+ */
+int fd_append_kv_slots(const void* k_new, int64_t k_token_stride, const void* v_new,
+                       int64_t v_token_stride, void* k_cache, void* v_cache, void* k_block_scale,
+                       void* v_block_scale, const float* k_scale, const float* v_scale,
+                       const int64_t* slot_map, int64_t num_tokens, int64_t num_heads_k,
+                       int64_t headdim, int64_t page_block_size, int64_t num_blocks, int src_dtype,
+                       int cache_dtype, void* stream);
+
+/*
+ * fd_gather_kv_slots - the rows of the given slots as values, [num_tokens,
+ * Hkv, headdim] of out_dtype (bf16, fp16 or fp32; contiguous): the inverse of
+ * fd_append_kv_slots, for moving a cache to another instance or format.
+ * Slots below zero give zeros, as do slots past the pool, which are reported
+ * (FD_ERR_BAD_PAGE).  cache_dtype: any; headdim a multiple of 16, caches and
+ * outputs 16-byte aligned.
+ * Replaces: nothing in the reference.
+ */
+int fd_gather_kv_slots(const void* k_cache, const void* v_cache, const void* k_block_scale,
+                       const void* v_block_scale, const float* k_scale, const float* v_scale,
+                       const int64_t* slot_map, int64_t num_tokens, void* k_out, void* v_out,
+                       int64_t num_heads_k, int64_t headdim, int64_t page_block_size,
+                       int64_t num_blocks, int cache_dtype, int out_dtype, void* stream);
+
+/*
+ * fd_assign_pages - pages and slots for a step's new tokens, on the device.
+ *
+ * Replaces: nothing in the reference, whose block tables are built on the host
+ * (scripts/evaluate_flashattn_submission.py:105-151).  Request b has
+ * max(cache_seqlens[b], 0) tokens stored in the pages of its block_table row
+ * and gets max(new_lens[b], 0) more.  Where they need pages, these come off
+ * the top of the stack free_pages (free_count[0] entries of the num_blocks
+ * allocated; entry free_count[0] - 1 first), in the order of the requests, and
+ * are entered in block_table.  Written:
+ *   seqlens_out [B]   tokens stored afterwards (may be cache_seqlens itself)
+ *   cu_new [B + 1]    prefix sums of new_lens: request b's tokens are rows
+ *                     cu_new[b] .. cu_new[b + 1] - 1 of the packed step
+ *   slot_map [num_slots]  slot of each packed token; -1 past the last one
+ *   free_count[0]     entries left.  free_count[1] belongs to the library: 0
+ *                     before the first call, and 0 again after every call.
+ * A request that does not fit - the stack has too few pages left, or its row
+ * of the table (or 2^31 - 1 tokens) is too short - gets nothing: its slots are
+ * -1 and its length stays.  Once the stack was too small for one request,
+ * later requests that need pages get none either (first come, first served).
+ * That, and a slot_map shorter than the step's tokens, is reported as
+ * FD_ERR_NO_PAGES by fd_device_status; a page id outside the pool (in the
+ * stack, or under a partly filled page) gives slots -1 and FD_ERR_BAD_PAGE.
+ * At most 8192 requests.  One pool serves one stream at a time.
+ */
+int fd_assign_pages(int32_t* block_table, int64_t block_table_stride, const int32_t* cache_seqlens,
+                    const int32_t* new_lens, const int32_t* free_pages, int32_t* free_count,
+                    int64_t batch_size, int64_t page_block_size, int64_t num_blocks,
+                    int32_t* seqlens_out, int32_t* cu_new, int64_t* slot_map, int64_t num_slots,
+                    void* stream);
+
+/*
+ * fd_release_pages - give back the pages a request no longer needs: those of
+ * its max(cache_seqlens[b], 0) tokens that hold none of the first
+ * max(keep_lens[b], 0) (0 for a finished request; the accepted length after
+ * speculation).  Their table entries become -1 and they are pushed on the
+ * stack in reverse order, so that releasing what the last fd_assign_pages took
+ * leaves the stack as it was.  An entry outside the pool is dropped, and so is
+ * a page for which the stack has no room (a page released twice); both are
+ * reported (FD_ERR_BAD_PAGE).  The lengths are not changed.  At most 8192
+ * requests.
+ * Replaces: nothing in the reference.
+ */
+int fd_release_pages(int32_t* block_table, int64_t block_table_stride,
+                     const int32_t* cache_seqlens, const int32_t* keep_lens, int32_t* free_pages,
+                     int32_t* free_count, int64_t batch_size, int64_t page_block_size,
+                     int64_t num_blocks, void* stream);
+
+/*
  * fd_decode_paged_noalloc - fd_decode_paged for callers that cannot allocate
  * device memory: a process whose framework allocator already holds nearly
  * all of the GPU's memory (a library cudaMalloc would fail or fragment that
@@ -337,7 +479,8 @@ const char* fd_last_error_message(void);
  * a bounded in-kernel wait ran out (that call's results are incomplete);
  * FD_ERR_BAD_PAGE: a block_table entry inside a sequence's length was
  * outside [0, num_blocks) (its rows were read as zeros, nothing outside the
- * cache was touched).  FD_OK otherwise.  Synchronises the current device.
+ * cache was touched); FD_ERR_NO_PAGES: fd_assign_pages could not serve every
+ * request.  FD_OK otherwise.  Synchronises the current device.
  * Replaces: nothing in the reference, whose kernels report no errors and
  * gather through block_table unchecked (best :741-742).
  */

@@ -166,6 +166,87 @@ def append_reference_e4m3(k_cache, v_cache, k_new, v_new, k_scale, v_scale, cach
     return kc.view(torch.float8_e4m3fn), vc.view(torch.float8_e4m3fn), lens
 
 
+E2M1_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def quantize_fp4(x: torch.Tensor, scale: torch.Tensor):
+    """4-bit block-scaled form of x [..., Hkv, D] with head scales [Hkv]: codes
+    uint8 [..., Hkv, D / 2] (even element in the low half) and block scales
+    uint8 (e4m3 bits) [..., Hkv, D / 16].  The format of the operator's
+    fd_append_kv_paged_fp4, in its fp32 steps: s = e4m3(amax / (6 g)),
+    code = e2m1(x / (s g)), nearest even, saturating; s = 0 stores zeros."""
+    b = x.cpu().float().unflatten(-1, (-1, 16))
+    g = scale.cpu().float()[:, None]
+    s8 = (b.abs().amax(-1) / (6.0 * g)).clamp(max=448.0).to(torch.float8_e4m3fn)
+    s = s8.float()
+    live = s > 0
+    y = b / torch.where(live, s * g, torch.ones_like(s))[..., None]
+    a = y.abs()
+    code = torch.zeros(y.shape, dtype=torch.uint8)
+    # midpoints between neighbours; a tie goes to the even code
+    for i, mid in enumerate((0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)):
+        code += (a > mid) if i % 2 == 0 else (a >= mid)
+    code |= torch.signbit(y).to(torch.uint8) << 3
+    code = torch.where(live[..., None], code, torch.zeros_like(code)).flatten(-2)
+    return code[..., 0::2] | (code[..., 1::2] << 4), s8.view(torch.uint8)
+
+
+def dequantize_fp4(codes: torch.Tensor, blocks: torch.Tensor, scale: torch.Tensor,
+                   dtype: torch.dtype = torch.float64) -> torch.Tensor:
+    """Values [num_blocks, page, Hkv, D] of a 4-bit cache: codes uint8
+    [num_blocks, page, Hkv, D / 2], block scales uint8 (e4m3 bits)
+    [num_blocks, Hkv, page, D / 16], head scales [Hkv]."""
+    c = codes.cpu()
+    c = torch.stack([c & 15, c >> 4], -1).flatten(-2).long()
+    v = torch.tensor(E2M1_VALUES + tuple(-x for x in E2M1_VALUES), dtype=dtype)[c]
+    s = blocks.cpu().view(torch.float8_e4m3fn).float().to(dtype).permute(0, 2, 1, 3)
+    return v * s.repeat_interleave(16, -1) * scale.cpu().to(dtype)[:, None]
+
+
+def assign_pages_reference(block_table, cache_seqlens, new_lens, free_pages, free_count, page,
+                           num_slots):
+    """The operator's fd_assign_pages in plain loops.  Returns (table, slot
+    map, cu_new, lengths afterwards, free entries left)."""
+    table = block_table.cpu().clone()
+    pool, left = free_pages.cpu().tolist(), int(free_count[0])
+    width = table.shape[1]
+    slots, cu, after, short = [], [0], [], False
+    for b in range(table.shape[0]):
+        L, a = max(int(cache_seqlens[b]), 0), max(int(new_lens[b]), 0)
+        cu.append(cu[-1] + a)
+        have, need = -(-L // page), -(-(L + a) // page)
+        fits = L + a <= width * page
+        if not fits or (need > have and (short or need - have > left)):
+            short = short or fits
+            after.append(L)
+            slots += [-1] * a
+            continue
+        for j in range(have, need):
+            left -= 1
+            table[b, j] = pool[left]
+        after.append(L + a)
+        slots += [int(table[b, t // page]) * page + t % page for t in range(L, L + a)]
+    slots = (slots + [-1] * num_slots)[:num_slots]
+    i32 = torch.int32
+    return (table, torch.tensor(slots, dtype=torch.int64), torch.tensor(cu, dtype=i32),
+            torch.tensor(after, dtype=i32), left)
+
+
+def release_pages_reference(block_table, cache_seqlens, keep_lens, free_pages, free_count, page):
+    """The operator's fd_release_pages in plain loops.  Returns (table, stack,
+    free entries)."""
+    table, pool, left = block_table.cpu().clone(), free_pages.cpu().clone(), int(free_count[0])
+    for b in reversed(range(table.shape[0])):
+        L, keep = max(int(cache_seqlens[b]), 0), max(int(keep_lens[b]), 0)
+        for j in reversed(range(-(-keep // page), min(-(-L // page), table.shape[1]))):
+            id_ = int(table[b, j])
+            table[b, j] = -1
+            if 0 <= id_ < len(pool) and left < len(pool):
+                pool[left] = id_
+                left += 1
+    return table, pool, left
+
+
 def merge_partials(part_o: torch.Tensor, part_lse: torch.Tensor):
     """Merge normalised partials over disjoint KV ranges (natural-log LSE).
 

@@ -1,0 +1,380 @@
+"""Decode over the 4-bit block-scaled cache against a plain implementation in
+64 bits on the dequantised cache.
+
+Tolerance, from the arithmetic of the operator (eps/2 of a type is its half
+step).  K and V dequantise to f16 exactly and products accumulate in fp32, so
+a logit is off by at most E = (D + 8) 2^-24 max_t sum_d |q_d k_td| scale (D
+additions and a few factors).  That changes every weight by a factor within
+e^(+-2E); the weights are also rounded to f16 (2^-11, absolute 2^-25 of the
+row's largest weight), and exp2 and the joining of partial sums cost a few
+2^-22.  With A = sum_t p_t |v_t| (the row's output for |V|):
+  |O - O64|   <= (2^-11 + 2 E + 2^-19) A + L 2^-25 max|v| + eps/2 |O64|
+  |LSE - LSE64| <= E + 2^-19 (1 + |LSE64|)
+"""
+import math
+
+import pytest
+import torch
+
+import flashdecode
+from flashdecode import cases
+from oracle.decode_ref import dequantize_fp4, quantize_fp4
+
+pytestmark = pytest.mark.gpu
+
+FD_ERR_BAD_PAGE = 6
+FP4, E4M3 = torch.float4_e2m1fn_x2, torch.float8_e4m3fn
+
+
+def make(seqlens, Hq, Hkv, D=128, page=256, sq=1, dtype=torch.bfloat16, seed=0, pool_extra=0, extra_len=0,
+         q_std=1.0):
+    """A case whose cache holds random codes and block scales everywhere; the
+    rows behind each sequence's end hold NaN scales."""
+    c = cases.custom_case("fp4", dtype, [max(n, 0) + extra_len for n in seqlens], Hq, Hkv, D=D, page=page,
+                          seed=seed, pool_extra=pool_extra)
+    g = torch.Generator().manual_seed(seed + 1)
+    nb = c.num_blocks
+    t = dict(lens=torch.tensor(seqlens, dtype=torch.int32), bt=c.block_table)
+    t["q"] = (torch.randn((c.B, sq, Hq, D), generator=g) * q_std).to(dtype)
+    t["ks"] = (1 + torch.rand(Hkv, generator=g)) / 512
+    t["vs"] = (1 + torch.rand(Hkv, generator=g)) / 512
+    live = torch.zeros((nb, page), dtype=torch.bool)
+    for b, L in enumerate(seqlens):
+        for j in range(-(-max(L, 0) // page)):
+            live[int(c.block_table[b, j]), :max(L, 0) - j * page] = True
+    for n in ("k", "v"):
+        x = torch.randn((nb, page, Hkv, D), generator=g)
+        codes, blocks = quantize_fp4(x, t[n + "s"])
+        blocks[~live] = 0x7F          # NaN
+        t[n] = codes
+        t[n + "b"] = blocks.permute(0, 2, 1, 3).contiguous()
+    return t
+
+
+def on_gpu(t):
+    d = {n: x.cuda() for n, x in t.items()}
+    for n in ("k", "v"):
+        d[n] = d[n].view(FP4)
+        d[n + "b"] = d[n + "b"].view(E4M3)
+    return d
+
+
+def call(d, **kw):
+    return flashdecode.flash_decode(d["q"], d["k"], d["v"], d["lens"], d["bt"], return_softmax_lse=True,
+                                    k_scale=d["ks"], v_scale=d["vs"], k_block_scale=d["kb"],
+                                    v_block_scale=d["vb"], **kw)
+
+
+def reference(t, causal=False, scale=None, lens=None):
+    """(O, LSE, A, E) in 64 bits; lens as in `t` unless given."""
+    q, bt = t["q"].double(), t["bt"].long()
+    B, sq, Hq, D = q.shape
+    nb, page, Hkv, _ = t["k"].shape
+    scale = 1 / math.sqrt(D) if scale is None else scale
+    K = dequantize_fp4(t["k"].view(torch.uint8), t["kb"].view(torch.uint8), t["ks"])
+    V = dequantize_fp4(t["v"].view(torch.uint8), t["vb"].view(torch.uint8), t["vs"])
+    out = torch.zeros((B, sq, Hq, D), dtype=torch.float64)
+    A, E = torch.zeros_like(out), torch.zeros((B, Hq, sq), dtype=torch.float64)
+    lse = torch.full((B, Hq, sq), -math.inf, dtype=torch.float64)
+    W = torch.zeros_like(out)
+    for b, L in enumerate((t["lens"] if lens is None else lens).tolist()):
+        L = min(max(L, 0), bt.shape[1] * page)
+        ids = bt[b, :-(-L // page)]
+        bad = (ids < 0) | (ids >= nb)
+        kb, vb = K[ids.clamp(0, nb - 1)], V[ids.clamp(0, nb - 1)]
+        kb[bad], vb[bad] = 0, 0
+        kb, vb = kb.flatten(0, 1)[:L], vb.flatten(0, 1)[:L]
+        for i in range(sq):
+            n = L - (sq - 1 - i) if causal else L
+            if n <= 0:
+                continue
+            x = q[b, i].view(Hkv, -1, D)
+            z = torch.einsum("hgd,thd->hgt", x, kb[:n]) * scale
+            p = torch.softmax(z, -1)
+            lse[b, :, i] = torch.logsumexp(z, -1).flatten()
+            out[b, i] = torch.einsum("hgt,thd->hgd", p, vb[:n]).reshape(Hq, D)
+            A[b, i] = torch.einsum("hgt,thd->hgd", p, vb[:n].abs()).reshape(Hq, D)
+            W[b, i] = n * 2.0 ** -25 * vb[:n].abs().amax()
+            mass = torch.einsum("hgd,thd->hgt", x.abs(), kb[:n].abs()).amax(-1) * abs(scale)
+            E[b, :, i] = ((D + 8) * 2.0 ** -24 * mass).flatten()
+    return out, lse, A, E, W
+
+
+def check(out, lse, ref):
+    O, LSE, A, E, W = ref
+    sq = O.shape[1]
+    e = E.permute(0, 2, 1)[..., None]
+    tol = (2.0 ** -11 + 2 * e + 2.0 ** -19) * A + W + torch.finfo(out.dtype).eps / 2 * O.abs()
+    err = (out.cpu().double() - O).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} elements off, max err {float(err.max()):.3e}"
+    got = lse.cpu().double().view_as(LSE) if sq > 1 else lse.cpu().double()[..., None]
+    some = torch.isfinite(LSE)
+    assert torch.equal(some, torch.isfinite(got)) and bool((got[~some] == -math.inf).all())
+    off = (got - LSE)[some].abs()
+    assert bool((off <= (E + 2.0 ** -19 * (1 + LSE.abs()))[some]).all()), float(off.max())
+
+
+RAGGED = [1, 0, 31, 32, 33, 127, 128, 129, 300, 2049]
+
+
+@pytest.mark.parametrize("page", [16, 48, 64, 256])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_lengths_pages_and_head_dims(page, D):
+    t = make(RAGGED, 8, 2, D=D, page=page, seed=page + D)
+    out, lse = call(on_gpu(t))
+    torch.cuda.synchronize()
+    check(out, lse, reference(t))
+    assert flashdecode.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("out_dtype", [None, torch.float32])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 8), (32, 8), (28, 4), (16, 1), (5, 1), (48, 2)])
+def test_types_and_groups(dtype, out_dtype, Hq, Hkv):
+    """Groups of 1 .. 24: one pass of 8 rows, one of 16, and two of 16."""
+    t = make([700, 1, 65, 0, 1500], Hq, Hkv, dtype=dtype, page=64, seed=Hq)
+    out, lse = call(on_gpu(t), out_dtype=out_dtype)
+    torch.cuda.synchronize()
+    assert out.dtype == (out_dtype or dtype)
+    check(out, lse, reference(t))
+
+
+@pytest.mark.parametrize("sq,causal", [(2, True), (4, True), (3, False), (9, True), (1, True)])
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 128), (14, 2, 64), (4, 1, 256)])
+def test_several_query_tokens(sq, causal, Hq, Hkv, D):
+    """Speculated tokens; lengths below sq leave rows that see no key."""
+    t = make([1, 2, 0, 130, 257, 1000, 7], Hq, Hkv, D=D, page=16, sq=sq, seed=sq)
+    out, lse = call(on_gpu(t), causal=causal)
+    torch.cuda.synchronize()
+    check(out, lse, reference(t, causal=causal))
+
+
+@pytest.mark.parametrize("seqlens,Hq,Hkv", [
+    ([70000], 32, 8), ([40000, 3, 17, 9000], 8, 1), ([16 * i * i for i in range(1, 41)], 16, 4),
+])
+def test_long_and_skewed(seqlens, Hq, Hkv):
+    """Pairs cut over many CTAs and joined, beside short ones."""
+    t = make(seqlens, Hq, Hkv, page=256, seed=len(seqlens))
+    d = on_gpu(t)
+    ref = reference(t)
+    first = None
+    for _ in range(3):
+        out, lse = call(d)
+        torch.cuda.synchronize()
+        check(out, lse, ref)
+        first = (out, lse) if first is None else first
+        assert torch.equal(first[0], out) and torch.equal(first[1], lse)   # the same bits every time
+
+
+def test_more_sequences_than_a_launch_takes():
+    t = make([(7 * i) % 61 for i in range(1100)], 4, 2, page=16, seed=9)
+    out, lse = call(on_gpu(t))
+    torch.cuda.synchronize()
+    check(out, lse, reference(t))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_query_magnitudes(dtype):
+    """Rows of very large, very small and zero queries (bf16 rows are brought
+    into f16's range by a power of two)."""
+    t = make([300] * 5, 8, 2, dtype=dtype, page=16, seed=4)
+    f = [1e4, 1e-4, 0.0, 30.0, 1e-6] if dtype == torch.float16 else [1e30, 1e-30, 0.0, 300.0, 1e-38]
+    t["q"] = (t["q"].float() * torch.tensor(f)[:, None, None, None]).to(dtype)
+    for scale in (None, -0.05):
+        s = scale
+        out, lse = call(on_gpu(t), softmax_scale=s)
+        torch.cuda.synchronize()
+        keep = [1, 2, 3, 4] if dtype == torch.bfloat16 else [0, 1, 2, 3, 4]
+        ref = reference(t, scale=s)
+        check(out[keep], lse[keep], tuple(x[keep] for x in ref))
+        assert torch.isfinite(out).all()
+
+
+def test_nan_and_infinity_travel_only_in_their_rows():
+    t = make([200, 200, 200], 8, 2, page=16, seed=6)
+    t["q"][1, 0, 3, 5] = float("nan")
+    t["q"][2, 0, 1, 7] = float("inf")
+    t["vb"][int(t["bt"][0, 2]), 0, 3, 1] = 0x7F       # a NaN scale inside sequence 0, KV head 0
+    out, _ = call(on_gpu(t))
+    torch.cuda.synchronize()
+    nan = torch.isnan(out.cpu())
+    assert nan[1, 0, 3].all() and not nan[1, 0, [0, 1, 2, 4, 5, 6, 7]].any()
+    assert nan[2, 0, 1].all() and not nan[2, 0, [0, 2, 3]].any()
+    assert nan[0, 0, :4, 16:32].all() and not nan[0, 0, :4, 32:].any() and not nan[0, 0, 4:].any()
+
+
+def test_bad_pages_read_as_zeros():
+    for bad in (-1, 10 ** 6):
+        t = make([500, 100], 8, 2, page=16, seed=8)
+        d = on_gpu(t)
+        d["bt"][0, 3] = bad
+        t["bt"] = t["bt"].clone()
+        t["bt"][0, 3] = bad
+        out, lse = call(d)
+        torch.cuda.synchronize()
+        check(out, lse, reference(t))
+        assert flashdecode.device_status() == FD_ERR_BAD_PAGE
+
+
+def test_length_past_the_table_is_cut():
+    t = make([100, 64], 8, 2, page=16, seed=3)
+    d = on_gpu(t)
+    d["lens"] = torch.tensor([5000, 64], dtype=torch.int32, device="cuda")
+    out, lse = call(d)
+    torch.cuda.synchronize()
+    t["kb"] = torch.where(t["kb"] == 0x7F, 0, t["kb"])   # sequence 0 now reaches its page's end
+    t["vb"] = torch.where(t["vb"] == 0x7F, 0, t["vb"])
+    width = t["bt"].shape[1] * 16
+    d2 = on_gpu(t)
+    d2["lens"] = d["lens"]
+    out, lse = call(d2)
+    torch.cuda.synchronize()
+    check(out, lse, reference(t, lens=torch.tensor([width, 64])))
+
+
+@pytest.mark.parametrize("sq", [1, 3])
+def test_fused_append(sq):
+    """k / v given: quantised into the cache, then attended; cache_seqlens
+    unchanged, the rest of the pool too."""
+    seqlens = [0, 15, 16, 700, 255]
+    t = make(seqlens, 8, 2, page=16, sq=sq, seed=sq, extra_len=sq)
+    g = torch.Generator().manual_seed(5)
+    kn, vn = (torch.randn((5, sq, 2, 128), generator=g).bfloat16() for _ in range(2))
+    d = on_gpu(t)
+    out, lse = call(d, causal=True, k=kn.cuda(), v=vn.cuda())
+    torch.cuda.synchronize()
+    for n, new in (("k", kn), ("v", vn)):
+        codes, blocks = quantize_fp4(new, t[n + "s"])
+        for b, L in enumerate(seqlens):
+            for i in range(sq):
+                pg, row = int(t["bt"][b, (L + i) // 16]), (L + i) % 16
+                t[n][pg, row] = codes[b, i]
+                t[n + "b"][pg, :, row] = blocks[b, i]
+        assert torch.equal(d[n].view(torch.uint8).cpu(), t[n])
+        assert torch.equal(d[n + "b"].view(torch.uint8).cpu(), t[n + "b"])
+    assert d["lens"].tolist() == seqlens
+    check(out, lse, reference(t, causal=True, lens=t["lens"] + sq))
+
+
+def test_plan_graph_streams_and_workspace():
+    """The same bits from the eager call, a plan, a captured and replayed
+    plan, another stream and a caller's workspace, also after a 16-bit call
+    used the same stream's scratch."""
+    t = make([5000, 17, 0, 3000], 32, 8, seed=2)
+    d = on_gpu(t)
+    out, lse = call(d)
+    torch.cuda.synchronize()
+    check(out, lse, reference(t))
+    kw = dict(return_softmax_lse=True, k_scale=d["ks"], v_scale=d["vs"], k_block_scale=d["kb"], v_block_scale=d["vb"])
+    plan = flashdecode.DecodePlan(d["q"], d["k"], d["v"], d["lens"], d["bt"], **kw)
+    c16 = cases.custom_case("n", torch.bfloat16, [4000, 900, 5], 32, 8, seed=1)
+    t16 = cases.materialize(c16, "cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            flashdecode.flash_decode(t16["q"], t16["k_cache"], t16["v_cache"], t16["cache_seqlens"], t16["block_table"])
+            o, s = plan()
+            side.synchronize()
+            assert torch.equal(o, out) and torch.equal(s, lse)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan()
+    for _ in range(3):
+        plan.out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(plan.out, out) and torch.equal(plan.lse, lse)
+    n = flashdecode.load_library().fd_decode_workspace_size_fp4(4, 1, 32, 8, 128)
+    ws = torch.zeros((n,), dtype=torch.uint8, device="cuda")
+    for _ in range(2):
+        o, s = call(d, workspace=ws)
+        torch.cuda.synchronize()
+        assert torch.equal(o, out) and torch.equal(s, lse)
+    with pytest.raises(flashdecode.FlashDecodeError):
+        call(d, workspace=ws[:n - 256])
+    assert flashdecode.device_status() == 0
+
+
+def test_serving_steps_together():
+    """Prompts arrive, get pages and slots, are appended and attended; then
+    decode steps with growing lengths; one request leaves and its pages go to
+    a newcomer.  The cache is checked through the attention's results against
+    a reference that keeps each request's quantised rows in plain lists."""
+    page, Hq, Hkv, D, nb = 16, 8, 2, 128, 40
+    g = torch.Generator().manual_seed(11)
+    t = make([0, 0, 0], Hq, Hkv, page=page, seed=1, pool_extra=nb)
+    d = on_gpu(t)
+    assert d["k"].shape[0] >= nb
+    nb = d["k"].shape[0]
+    table = torch.full((3, 12), -1, dtype=torch.int32, device="cuda")
+    lens = torch.zeros((3,), dtype=torch.int32, device="cuda")
+    pool, count = torch.arange(nb, dtype=torch.int32, device="cuda"), torch.tensor([nb, 0], dtype=torch.int32, device="cuda")
+    kw = dict(k_scale=d["ks"], v_scale=d["vs"], k_block_scale=d["kb"], v_block_scale=d["vb"])
+    held = [([], []) for _ in range(3)]
+    steps = [[37, 100, 0], [1, 1, 0], [1, 1, 50], [2, 0, 1], "leave 1", [1, 120, 1], [1, 1, 1]]
+    for new in steps:
+        if new == "leave 1":
+            keep = lens.clone()
+            keep[1] = 0
+            flashdecode.release_pages(table, lens, keep, pool, count, page)
+            lens.copy_(keep)
+            held[1] = ([], [])
+            continue
+        T = sum(new)
+        n = torch.tensor(new, dtype=torch.int32, device="cuda")
+        slots, cu, _ = flashdecode.assign_pages(table, lens, n, pool, count, page, num_slots=T + 2, seqlens_out=lens)
+        k, v = (torch.randn((T + 2, Hkv, D), generator=g).bfloat16() for _ in range(2))
+        flashdecode.append_kv_slots(k.cuda(), v.cuda(), d["k"], d["v"], slots, **kw)
+        cu = cu.tolist()
+        for b in range(3):
+            held[b][0].append(k[cu[b]:cu[b + 1]])
+            held[b][1].append(v[cu[b]:cu[b + 1]])
+        q = torch.randn((3, 1, Hq, D), generator=g).bfloat16()
+        out, lse = flashdecode.flash_decode(q.cuda(), d["k"], d["v"], lens, table, return_softmax_lse=True, **kw)
+        torch.cuda.synchronize()
+        # the reference: contiguous caches of one page a request
+        L = [sum(x.shape[0] for x in h[0]) for h in held]
+        assert lens.tolist() == L
+        ref = dict(q=q, lens=torch.tensor(L), bt=torch.arange(3)[:, None], ks=t["ks"], vs=t["vs"])
+        wide = max(L)
+        for name, i in (("k", 0), ("v", 1)):
+            rows = torch.zeros((3, wide, Hkv, D), dtype=torch.bfloat16)
+            for b in range(3):
+                rows[b, :L[b]] = torch.cat(held[b][i]) if held[b][i] else 0
+            ref[name], blocks = quantize_fp4(rows, t[name + "s"])
+            ref[name + "b"] = blocks.permute(0, 2, 1, 3).contiguous()
+        check(out, lse, reference(ref))
+    assert int(count[0]) == nb - sum(-(-n // page) for n in L)
+    assert flashdecode.device_status() == 0
+
+
+def test_refusals():
+    t = make([100, 20], 8, 2, page=16)
+    d = on_gpu(t)
+
+    def bad(err, **over):
+        x = {**d, **{k: v for k, v in over.items() if k in d}}
+        with pytest.raises(err):
+            call(x, **{k: v for k, v in over.items() if k not in d})
+
+    bad(ValueError, kb=None)
+    bad(ValueError, vb=d["vb"].view(torch.uint8))
+    bad(ValueError, kb=d["kb"].transpose(1, 2))
+    bad(ValueError, ks=None)
+    bad(ValueError, q=d["q"].float())
+    bad(ValueError, q=d["q"][..., :64].contiguous())
+    bad(ValueError, v=d["v"].view(torch.uint8).view(E4M3))
+
+    bad(flashdecode.FlashDecodeError, out_dtype=torch.float16)
+    bad(flashdecode.FlashDecodeError, softmax_scale=float("nan"))
+    for D, page in ((96, 16), (128, 8), (32, 16)):
+        u = on_gpu(make([20], 4, 2, D=D, page=page))
+        with pytest.raises(flashdecode.FlashDecodeError):
+            call(u)
+    with pytest.raises(ValueError):        # block scales with a cache that has none
+        c16 = cases.custom_case("n", torch.bfloat16, [40], 8, 2, seed=1)
+        t16 = cases.materialize(c16, "cuda")
+        flashdecode.flash_decode(t16["q"], t16["k_cache"], t16["v_cache"], t16["cache_seqlens"],
+                                 t16["block_table"], k_block_scale=d["kb"])
