@@ -382,7 +382,6 @@ bool is_short_launch(int64_t block_table_stride, int64_t page_block_size, int64_
 }
 
 int device_sms(int dev) { return ::device_sms(dev); }
-unsigned long long wait_timeout_ns() { return timeout_ns(); }
 bool pdl_enabled() { return ::pdl_enabled(); }
 int env_int(const char* name, int dflt, int lo, int hi) { return ::env_int(name, dflt, lo, hi); }
 void* library_workspace(int dev, size_t bytes, cudaStream_t stream, const char** why) {
@@ -390,15 +389,6 @@ void* library_workspace(int dev, size_t bytes, cudaStream_t stream, const char**
 }
 int64_t seqs_per_launch(int64_t per_seq_cost, int64_t aligned_cost, int64_t hkv, int grid) {
   return ::seqs_per_launch(per_seq_cost, aligned_cost, hkv, grid);
-}
-bool tensor_maps_available() { return encode_fn() != nullptr; }
-CUresult encode_tensor_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* base,
-                           const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
-                           CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
-  const cuuint32_t estride[5] = {1, 1, 1, 1, 1};
-  return encode_fn()(m, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides,
-                     box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 int report_ok() { return set_ok(); }
 

@@ -19,12 +19,19 @@ constexpr int kMaxDevices = 64;
 
 // Split cost model of the 4-bit cache (units and meaning as in fd_api.cu).
 constexpr int kCostTile4 = 2;
-constexpr int kCostSeg4 = 12;
+constexpr int kCostSeg4 = 30;
 constexpr int kCostFloor4 = 0;
 int cost_tile4() { static const int v = fd::env_int("FD_COST_TILE4", kCostTile4, 0, 64); return v; }
 int cost_seg4() { static const int v = fd::env_int("FD_COST_SEG4", kCostSeg4, 1, 256); return v; }
 int cost_floor4() { static const int v = fd::env_int("FD_COST_FLOOR4", kCostFloor4, 0, 1024); return v; }
 int max_lead4() { return cost_seg4() > cost_floor4() ? cost_seg4() : cost_floor4(); }
+
+// A partial for every (sequence, KV head, row tile), and for every KV head of
+// the first and last segment of each CTA.
+fd::WorkspaceLayout fp4_workspace(int64_t batch, int64_t num_heads_k, int64_t qrows, int rows, int grid_max,
+                                  int head_dim) {
+  return fd::workspace_layout(batch, num_heads_k * ((qrows + rows - 1) / rows), rows, 4 * grid_max, head_dim);
+}
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -291,9 +298,8 @@ size_t fd_decode_workspace_size_fp4(int64_t batch_size, int64_t seqlen_q, int64_
   const int64_t nb = batch_size < fd::kMaxBatchPerLaunch ? batch_size : fd::kMaxBatchPerLaunch;
   const int64_t qrows = seqlen_q * (num_heads / num_heads_k);
   const int rows = fd::fp4_rows(static_cast<int>(headdim), qrows);
-  return fd::workspace_layout(nb, num_heads_k * ((qrows + rows - 1) / rows), rows,
-                              fd::fp4_max_grid(static_cast<int>(headdim), rows, sms),
-                              static_cast<int>(headdim)).total;
+  return fp4_workspace(nb, num_heads_k, qrows, rows, fd::fp4_max_grid(static_cast<int>(headdim), rows, sms),
+                       static_cast<int>(headdim)).total;
 }
 
 int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_block_scale,
@@ -337,8 +343,6 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
   if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(k_block_scale, 16) ||
       !aligned(v_block_scale, 16) || !aligned(k_new, 16) || !aligned(v_new, 16))
     return report_error(FD_ERR_UNSUPPORTED, "e2m1 cache: tensors must be 16-byte aligned");
-  if (!fd::tensor_maps_available())
-    return report_error(FD_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   int dev = 0;
   int* status = nullptr;
   st = current_device(&dev, &status);
@@ -351,10 +355,12 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
   const int64_t qrows = seqlen_q * group;
   const int rows = fd::fp4_rows(D, qrows);
   const int64_t row_tiles = (qrows + rows - 1) / rows;
-  const int64_t vheads = num_heads_k * row_tiles;
+  // neighbouring KV heads of a token are read together where their count allows
+  const int heads = num_heads_k % 2 == 0 ? 2 : 1;
+  const int64_t vheads = num_heads_k / heads * row_tiles;
   const int grid_max = fd::fp4_max_grid(D, rows, sms);
   const int64_t nb_max = batch_size < fd::kMaxBatchPerLaunch ? batch_size : fd::kMaxBatchPerLaunch;
-  const fd::WorkspaceLayout wl = fd::workspace_layout(nb_max, vheads, rows, grid_max, D);
+  const fd::WorkspaceLayout wl = fp4_workspace(nb_max, num_heads_k, qrows, rows, grid_max, D);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (ws == nullptr) {
@@ -369,44 +375,12 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
 
   const int64_t kv_max = block_table_stride * page_block_size;
   const int64_t len_bound = max_seqlen_k > 0 && max_seqlen_k < kv_max ? max_seqlen_k : kv_max;
-  const int64_t tiles_bound = (len_bound + fd::kTileTokens - 1) / fd::kTileTokens;
-  const int64_t per_seq_cost = max_lead4() + ((kv_max + fd::kTileTokens - 1) / fd::kTileTokens + 1) *
+  // the schedule's tiles are kTileTokens / heads tokens of `heads` heads
+  const int64_t tiles_bound = (len_bound * heads + fd::kTileTokens - 1) / fd::kTileTokens;
+  const int64_t per_seq_cost = max_lead4() + ((kv_max * heads + fd::kTileTokens - 1) / fd::kTileTokens + 1) *
                                                  (8 + static_cast<int64_t>(cost_tile4()));
   const int64_t per_launch = fd::seqs_per_launch(per_seq_cost, 0, vheads, grid_max);
   if (per_launch == 0) return report_error(FD_ERR_UNSUPPORTED, "sequence too long");
-
-  const int chunk = page_block_size % 32 == 0 ? 32 : 16;
-  fd::Fp4TensorMaps maps;
-  {
-    // codes [num_blocks, page, Hkv, D / 2] bytes, a row of a box is one head's
-    // D / 2 bytes; block scales [num_blocks, Hkv, page * D / 16] in 4-byte words
-    const cuuint64_t rb = static_cast<cuuint64_t>(D / 2), sb = static_cast<cuuint64_t>(D / 16);
-    const cuuint64_t dims[4] = {rb, (cuuint64_t)num_heads_k, (cuuint64_t)page_block_size, (cuuint64_t)num_blocks};
-    const cuuint64_t strides[3] = {rb, rb * num_heads_k, rb * num_heads_k * page_block_size};
-    const cuuint32_t box[4] = {(cuuint32_t)rb, 1, (cuuint32_t)chunk, 1};
-    const cuuint64_t sdims[3] = {(cuuint64_t)page_block_size * sb / 4, (cuuint64_t)num_heads_k,
-                                 (cuuint64_t)num_blocks};
-    const cuuint64_t sstrides[2] = {page_block_size * sb, page_block_size * sb * num_heads_k};
-    const cuuint32_t sbox[3] = {(cuuint32_t)(chunk * sb / 4), 1, 1};
-    const CUtensorMapSwizzle swizzle = D == 64    ? CU_TENSOR_MAP_SWIZZLE_32B
-                                       : D == 128 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                  : CU_TENSOR_MAP_SWIZZLE_128B;
-    const CUtensorMapL2promotion promotion = D == 256   ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
-                                             : D == 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B
-                                                        : CU_TENSOR_MAP_L2_PROMOTION_NONE;
-    CUresult r = fd::encode_tensor_map(&maps.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, k_cache, dims, strides, box,
-                                       swizzle, promotion);
-    if (r == CUDA_SUCCESS)
-      r = fd::encode_tensor_map(&maps.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, v_cache, dims, strides, box, swizzle,
-                                promotion);
-    if (r == CUDA_SUCCESS)
-      r = fd::encode_tensor_map(&maps.k_block, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, k_block_scale, sdims, sstrides,
-                                sbox, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE);
-    if (r == CUDA_SUCCESS)
-      r = fd::encode_tensor_map(&maps.v_block, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, v_block_scale, sdims, sstrides,
-                                sbox, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE);
-    if (r != CUDA_SUCCESS) return report_error(FD_ERR_CUDA, "K/V tensor map encode failed (%d)", (int)r);
-  }
 
   int len_add = 0;
   if (k_new != nullptr) {  // everything the attention would refuse has been checked
@@ -421,6 +395,10 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
     const int64_t nb = batch_size - b0 < per_launch ? batch_size - b0 : per_launch;
     fd::Fp4DecodeParams p{};
     p.q = static_cast<const uint8_t*>(q) + b0 * seqlen_q * num_heads * headdim * es;
+    p.k_cache = static_cast<const uint8_t*>(k_cache);
+    p.v_cache = static_cast<const uint8_t*>(v_cache);
+    p.k_block = static_cast<const uint8_t*>(k_block_scale);
+    p.v_block = static_cast<const uint8_t*>(v_block_scale);
     p.out = static_cast<uint8_t*>(out) + b0 * seqlen_q * num_heads * headdim * oes;
     p.lse = lse != nullptr ? lse + b0 * num_heads * seqlen_q : nullptr;
     p.k_scale = k_scale;
@@ -434,12 +412,12 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
     p.num_heads_k = static_cast<int>(num_heads_k);
     p.group = group;
     p.page = static_cast<int>(page_block_size);
-    p.chunk = chunk;
     p.seqlen_q = static_cast<int>(seqlen_q);
     p.causal = causal ? 1 : 0;
     p.qrows = static_cast<int>(qrows);
     p.row_tiles = static_cast<int>(row_tiles);
     p.rows = rows;
+    p.heads = heads;
     p.len_add = len_add;
     p.scale_log2 = softmax_scale * 1.4426950408889634f;
     p.tickets = reinterpret_cast<unsigned long long*>(ws + wl.tickets_off);
@@ -447,14 +425,13 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
     p.part_o = reinterpret_cast<float*>(ws + wl.o_off);
     p.epoch_word = reinterpret_cast<unsigned long long*>(ws + wl.epoch_off);
     p.err = status;
-    p.timeout_ns = fd::wait_timeout_ns();
     p.cost_tile = cost_tile4();
     p.cost_seg = cost_seg4();
     p.cost_floor = cost_floor4();
     p.pdl = fd::pdl_enabled() ? 1 : 0;
     const int64_t work = nb * vheads * tiles_bound;
     const int grid = static_cast<int>(work < grid_max ? work : grid_max);
-    const cudaError_t e = fd::launch_decode_fp4(maps, p, D, q_dtype, out_dtype == FD_DTYPE_FP32, grid, cs);
+    const cudaError_t e = fd::launch_decode_fp4(p, D, q_dtype, out_dtype == FD_DTYPE_FP32, grid, cs);
     if (e != cudaSuccess) return report_error(FD_ERR_CUDA, "e2m1 launch: %s", cudaGetErrorString(e));
   }
   return fd::report_ok();

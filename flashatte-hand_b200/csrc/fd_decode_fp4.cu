@@ -19,13 +19,13 @@ int fp4_max_grid(int head_dim, int rows, int sms) {
   return per_sm * sms;
 }
 
-cudaError_t launch_decode_fp4(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim,
-                              int q_dtype, bool out_fp32, int grid, cudaStream_t stream) {
+cudaError_t launch_decode_fp4(const Fp4DecodeParams& p, int head_dim, int q_dtype, bool out_fp32,
+                              int grid, cudaStream_t stream) {
   if (q_dtype == 0)
-    return out_fp32 ? launch_fp4_bf16_f32(m, p, head_dim, grid, stream)
-                    : launch_fp4_bf16(m, p, head_dim, grid, stream);
-  return out_fp32 ? launch_fp4_fp16_f32(m, p, head_dim, grid, stream)
-                  : launch_fp4_fp16(m, p, head_dim, grid, stream);
+    return out_fp32 ? launch_fp4_bf16_f32(p, head_dim, grid, stream)
+                    : launch_fp4_bf16(p, head_dim, grid, stream);
+  return out_fp32 ? launch_fp4_fp16_f32(p, head_dim, grid, stream)
+                  : launch_fp4_fp16(p, head_dim, grid, stream);
 }
 
 }  // namespace fd

@@ -18,7 +18,7 @@
 // of two that brings its largest magnitude to [2^13, 2^14): exact for fp16
 // rows (not scaled) and for the bf16 values down to 2^-28 of the row's
 // largest (smaller ones keep an absolute error of 2^-39 of it).  P is rounded
-// to f16 (11 bits, relative to each warp's running maximum).
+// to f16 (11 bits; values below 2^-14 of a row's largest keep 2^-25 of it).
 //
 // Why mma.sync and not tcgen05: the dequantised tiles would have to be
 // written to shared memory (2 bytes a value) and read back by the tensor
@@ -37,12 +37,22 @@
 // so that rows of both parities meet in a quarter-warp (tau below): with the
 // TMA swizzle K's and V's loads are free of bank conflicts at D = 128, 256.
 //
-// A CTA is four warps; each has its own ring of 32-token stages filled by TMA
-// (its lane 0 issues; page ids come from one lookup per 32 stages) and its
-// own softmax state, so the loop has no CTA-wide synchronisation.  The four
-// states are joined when a segment (the CTA's part of a pair) ends, after the
-// next segment's first loads were issued.  Work split and the joining of
-// segments on different CTAs are those of fd_decode_sm100.cuh.
+// Loads.  A row of codes is D / 2 = 64 bytes at a stride of Hkv * 64: a TMA
+// box of such rows was measured to move one row in about 5 cycles of the SM
+// (4.0 TB/s in all at D = 128, 1.8 TB/s with the 32-byte rows of D = 64,
+// however many boxes were in flight, from L2 as from HBM).  So the lanes copy
+// 16 bytes each with cp.async, eight rows an instruction, past L1.
+//
+// A CTA is four warps, and a schedule tile four 32-token stages, one a warp:
+// p.heads (4, 2 or 1) neighbouring KV heads of the same tokens, so that the
+// warps together read whole runs of a token's heads (64-byte pieces read at
+// different times cost 1.27 times the DRAM traffic), times 4 / p.heads stages
+// along the sequence.  Each warp has a ring and a softmax state of its own,
+// and nothing in the loop waits for another warp.  The ring runs across
+// segments (a segment is the CTA's part of a sequence's heads): the next
+// one's first loads are in flight while this one is written out.  Work split
+// and the joining of segments on different CTAs are those of
+// fd_decode_sm100.cuh, a head of a segment at a time.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -62,46 +72,48 @@ namespace {
 constexpr int kFp4Threads = 128;
 constexpr int kFp4Warps = kFp4Threads / 32;
 constexpr int kSubTokens = 32;  // tokens of a stage
+constexpr int kSegRing = 8;     // segments that the loads may be ahead
+static_assert(kTileTokens == kFp4Warps * kSubTokens, "a schedule tile is a stage of each warp");
 
 template <int D, int NT> struct Fp4Geo {
   static constexpr int kRowBytes = D / 2;
   static constexpr int kScaleBytes = D / 16;
   static constexpr int kTileBytes = kSubTokens * kRowBytes;
-  // Block scales of 16 tokens; TMA destinations are 128-byte aligned, so the
-  // 64 bytes of D = 64 are spread when they come in boxes of 16 tokens.
-  static constexpr int kHalfScales = 16 * kScaleBytes < 128 ? 128 : 16 * kScaleBytes;
-  static constexpr int kTileScales = 2 * kHalfScales;
+  static constexpr int kTileScales = kSubTokens * kScaleBytes;
   static constexpr int kStageBytes = 2 * kTileBytes + 2 * kTileScales;
   static constexpr int kRows = 8 * NT;
   // CTAs per SM, and stages that fit beside them
-  static constexpr int kCtas = D == 256 ? 2 : (NT == 1 ? 4 : 3);
-  static constexpr int kStages = D == 64 ? 4 : 2;
+  static constexpr int kCtas = D == 64 ? 3 : 2;
+  static constexpr int kStages = D == 64 ? 5 : D == 128 ? 4 : 2;
   static constexpr int kRowPad = D + 4;  // floats of a row of the join buffer
-  static constexpr int kOffJoin = kFp4Warps * kStages * kStageBytes;       // [2][kRows][kRowPad] floats
-  static constexpr int kOffMl = kOffJoin + 2 * kRows * kRowPad * 4;        // [warps][kRows][2] floats
-  static constexpr int kOffBars = kOffMl + kFp4Warps * kRows * 2 * 4;
-  static constexpr int kOffMisc = kOffBars + kFp4Warps * kStages * 8;
-  static constexpr int kOffPrefix = kOffMisc + 64;
+  static constexpr int kJoinWarp = kRows * kRowPad * 4 + kRows * 2 * 4;  // O, then maximum and sum of each row
+  // the ring; what a warp's lanes share of its loads (page offsets of 16
+  // stages, segments ahead); the join; lengths
+  static constexpr int kOffOffs = kFp4Warps * kStages * kStageBytes;     // [warps][32] code and scale offsets
+  static constexpr int kOffSegs = kOffOffs + kFp4Warps * 32 * 16;        // [warps][kSegRing]
+  static constexpr int kOffJoin = kOffSegs + kFp4Warps * kSegRing * 32;  // [kFp4Warps - 1]
+  static constexpr int kOffMisc = kOffJoin + (kFp4Warps - 1) * kJoinWarp;
+  static constexpr int kOffPrefix = kOffMisc + 16;
   static constexpr int kOffLens = kOffPrefix + (kMaxBatchPerLaunch + 1) * 4;
-  static constexpr int kSmemBytes = kOffLens + kMaxBatchPerLaunch * 4 + 1024;  // slack for alignment
-  static_assert(kTileBytes % 1024 == 0 && kTileScales % 128 == 0, "TMA destinations");
-  static_assert(kStageBytes % (8 * kRowBytes) == 0, "a stage starts on a swizzle period");
-  static_assert(kSmemBytes <= 232448 / kCtas, "shared memory of the resident CTAs");
-  static_assert(kOffBars % 8 == 0 && kOffMisc % 8 == 0, "alignment");
+  static constexpr int kSmemBytes = kOffLens + kMaxBatchPerLaunch * 4;
+  static_assert(kSegRing > kStages + 1, "the loads run at most kStages segments ahead");
+  static_assert(kSmemBytes + 1024 <= 233472 / kCtas, "shared memory of the resident CTAs");
+  static_assert(kStageBytes % 16 == 0 && kOffMisc % 16 == 0 && kJoinWarp % 16 == 0, "alignment");
 };
 
-__device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint64_t* bar, void* dst, int c0,
-                                            int c1, int c2, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
-      : "memory");
+// 16 bytes from global to shared memory past L1; the bytes behind `valid` are
+// written as zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, int valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -110,13 +122,24 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
   return d;
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Read from shared memory here and now: not hoisted, not kept in registers.
+__device__ __forceinline__ int volatile_at(const int* p) { return *reinterpret_cast<const volatile int*>(p); }
+__device__ __forceinline__ int4 volatile_at(const int4* p) {
+  int4 v;
+  asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(smem_u32(p))
+               : "memory");
+  return v;
 }
 
 template <typename T> __device__ __forceinline__ float2 pair_to_float2(uint32_t w);
@@ -146,8 +169,21 @@ template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, ui
   }
 }
 
-// 16-byte chunk of row `row` that the TMA put chunk `chunk` at: the swizzle
-// exchanges chunks by address bits 7.., i.e. by the row.
+// N consecutive values, rounded once, in 16-byte stores where they fill them.
+template <typename O, int N> __device__ __forceinline__ void store_row(O* dst, const float (&x)[N]) {
+  if constexpr (sizeof(O) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<float4*>(dst + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) dst[i] = fp4_out<O>(x[i]);
+  }
+}
+
+// Place of 16-byte chunk `chunk` of row `row` in a tile of RB-byte rows: the
+// chunks of a row are exchanged by the row, so that the loads of K (16 bytes
+// of 8 rows) and of V (8 bytes of 4 rows) touch every bank once.
 template <int RB> __device__ __forceinline__ int swizzled(int row, int chunk) {
   if constexpr (RB == 32) return chunk ^ ((row >> 2) & 1);
   else if constexpr (RB == 64) return chunk ^ ((row >> 1) & 3);
@@ -156,59 +192,46 @@ template <int RB> __device__ __forceinline__ int swizzled(int row, int chunk) {
 
 template <typename T, typename OutT, int D, int NT, bool MULTI>
 __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
-    decode_fp4_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                      const __grid_constant__ CUtensorMap tm_kb, const __grid_constant__ CUtensorMap tm_vb,
-                      const Fp4DecodeParams p) {
+    decode_fp4_kernel(const __grid_constant__ Fp4DecodeParams p) {
   using G = Fp4Geo<D, NT>;
   constexpr int RB = G::kRowBytes, SB = G::kScaleBytes;
   constexpr int KW = D / 32;        // words of K a lane takes from a row
   constexpr int VW = D / 64;        // words of V a lane takes from a token
   constexpr int MT = D / 16;        // 16-dim tiles of O^T
   constexpr int KS = D / 16;        // 16-dim steps of S^T
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_addr = smem_u32(smem_raw);
-  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int r = lane >> 2, c = lane & 3;
 
   uint8_t* ring = smem + warp * G::kStages * G::kStageBytes;
-  float* join = reinterpret_cast<float*>(smem + G::kOffJoin);
-  float* ml = reinterpret_cast<float*>(smem + G::kOffMl);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::kOffBars) + warp * G::kStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + G::kOffMisc);
-  volatile int* last_flag = reinterpret_cast<volatile int*>(smem + G::kOffMisc + 4);
-  unsigned long long* launch_epoch = reinterpret_cast<unsigned long long*>(smem + G::kOffMisc + 8);
+  longlong2* offs = reinterpret_cast<longlong2*>(smem + G::kOffOffs) + warp * 32;
+  int4* seg_ring = reinterpret_cast<int4*>(smem + G::kOffSegs) + warp * kSegRing * 2;
+  unsigned long long* launch_epoch = reinterpret_cast<unsigned long long*>(smem + G::kOffMisc);
+  volatile int* last_flag = reinterpret_cast<volatile int*>(smem + G::kOffMisc + 8);  // [2]
   int* prefix = reinterpret_cast<int*>(smem + G::kOffPrefix);
   int* lens = reinterpret_cast<int*>(smem + G::kOffLens);
 
   const int batch = p.batch, cta = blockIdx.x;
-  const int vheads = p.num_heads_k * p.row_tiles;  // a pair is (sequence, KV head, row tile)
-  const int64_t max_len = p.bt_stride * static_cast<int64_t>(p.page);
+  const int HW = p.heads, TW = kFp4Warps / HW;    // warps over heads, warps over tokens
+  const int hw = warp & (HW - 1), tw = warp / HW;
+  const int step = TW * kSubTokens;               // tokens of a schedule tile
+  // a pair of the schedule is (sequence, HW KV heads, row tile)
   const float neg_inf = -__int_as_float(0x7f800000);
-  // bytes from the block scales of a stage's token 0 to those of token 16
-  const int half_scales = p.chunk == 16 ? G::kHalfScales : 16 * SB;
 
   // ------------------------------------------------------------ prologue
-  if (tid == 0) {
-    pdl_launch_dependents();
-    uint64_t* all = reinterpret_cast<uint64_t*>(smem + G::kOffBars);
-    for (int i = 0; i < kFp4Warps * G::kStages; ++i) mbar_init(all + i, 1);
-    *abort_flag = 0;
-    fence_mbar_init();
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
-    tma_prefetch_desc(&tm_kb);
-    tma_prefetch_desc(&tm_vb);
-  }
+  if (tid == 0) pdl_launch_dependents();
   const CostModel cm{p.cost_tile, p.cost_seg, p.cost_floor};
   pdl_wait_prerequisites();
   unsigned long long epoch_ld = 0;
   if (tid == 0) epoch_ld = *reinterpret_cast<volatile unsigned long long*>(p.epoch_word);
   for (int b = tid; b < batch; b += kFp4Threads) {
     const int stored = __ldg(p.seqlens + b);
+    const int64_t max_len = p.bt_stride * static_cast<int64_t>(p.page);
     const int64_t want = static_cast<int64_t>(stored < 0 ? 0 : stored) + p.len_add;
-    const int64_t cap = max_len < 0x7fffffff ? max_len : 0x7fffffff;
-    const int len = static_cast<int>(want > cap ? cap : want);
+    const int64_t cap = max_len < 0x1fffffff ? max_len : 0x1fffffff;
+    // The schedule counts tiles of kTileTokens; a tile here is `step` tokens
+    // of HW heads, so lengths are given to it times HW.
+    const int len = static_cast<int>(want > cap ? cap : want) * HW;
     lens[b] = len;
     prefix[b + 1] = cm.pair_cost(len);
   }
@@ -216,7 +239,6 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     prefix[0] = 0;
     *launch_epoch = epoch_ld & kEpochMax;
   }
-  fence_proxy_async_smem();
   __syncthreads();
   if (warp == 0) {
     int carry = 0;
@@ -234,114 +256,208 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     }
   }
   __syncthreads();
-  // Every CTA counts itself once it has read the epoch; the last one hands
-  // the next launch a new epoch (see fd_decode_sm100.cuh).
-  if (tid == 0) {
-    const unsigned long long e = *launch_epoch;
-    if (ticket_arrive(p.epoch_word + 1, e, static_cast<int>(gridDim.x))) {
-      p.epoch_word[0] = e % kEpochMax + 1ull;
-      p.epoch_word[1] = 0ull;
-    }
-  }
-  Schedule sched;
-  sched.cost_prefix = prefix;
-  sched.lens = lens;
-  sched.max_len = max_len;
-  sched.total = static_cast<int64_t>(vheads) * prefix[batch];
-  sched.batch = batch;
-  sched.hkv = vheads;
-  sched.cm = cm;
-  sched.align_m = 0;
-  sched.align_cost = 0;
-  {
+  // The schedule is asked at segment ends only: what it needs is read from
+  // shared memory there, so that the loop's registers hold none of it.
+  auto schedule = [&]() {
+    Schedule x;
+    x.cost_prefix = prefix;
+    x.lens = lens;
+    x.max_len = 0;
+    x.total = static_cast<int64_t>(p.num_heads_k / p.heads * p.row_tiles) * volatile_at(prefix + p.batch);
+    x.batch = p.batch;
+    x.hkv = p.num_heads_k / p.heads * p.row_tiles;
+    x.cm = CostModel{p.cost_tile, p.cost_seg, p.cost_floor};
+    x.align_m = 0;
+    x.align_cost = 0;
     // every range longer than the costliest tile: none inside a pair is empty
-    const int64_t g = div_u32(sched.total, cm.max_lead() + cm.full() + 1);
-    sched.grid = static_cast<int>(g < 1 ? 1 : (g < gridDim.x ? g : gridDim.x));
-  }
-  const int64_t range_end = sched.range_start(cta + 1);
+    const int64_t g = div_u32(x.total, x.cm.max_lead() + x.cm.full() + 1);
+    x.grid = static_cast<int>(g < 1 ? 1 : (g < gridDim.x ? g : gridDim.x));
+    return x;
+  };
 
   // ------------------------------------------------------------ loads
-  const uint64_t policy = policy_evict_first();
-  // Page ids of the warp's next 32 stages, one per lane (two with 16-token
-  // boxes); num_blocks, which the TMA fills with zeros, for a bad id.
-  int page_ids[2] = {0, 0};
-  int64_t stage_no = 0;  // stages this warp has used so far (ring position and parity)
-  struct Walk {
-    int b, kvh, tok0, end, count;  // this warp's stages: tokens tok0 + 128 k .. < end, k < count
+  // The cursor of the loads, a ring ahead of the multiplication: pc_left
+  // tiles of the segment entered last (seg_ring[seg_w - 1]) are left, the
+  // next, its pc_k-th, at token pc_tok.  offs[2 i + g] are the byte offsets
+  // (codes; block scales; -1: no page) of tokens 16 g .. of the warp's stage
+  // 16 n + i of the segment, next_* the page id and row (-1: no tokens) of
+  // the same entry of batch n + 1.
+  int pc_left = 0, pc_tok = 0, pc_end = 0, pc_k = 0, next_id = 0, next_row = -1, seg_w = 0;
+  // A copy instruction moves 16 bytes a lane: half the lanes rows of K, half
+  // of V, so that a lane needs one pointer; kCopies of them are 16 tokens.
+  constexpr int kChunks = RB / 16;          // 16-byte chunks of a row of codes
+  constexpr int kRowsPer = 16 / kChunks;    // rows of K, and of V, of one instruction
+  constexpr int kCopies = 16 / kRowsPer;
+  const int64_t row_bytes = static_cast<int64_t>(p.num_heads_k) * RB;
+  const int lr = (lane & 15) / kChunks, lc = lane % kChunks;
+  const uint8_t* code_src = (lane < 16 ? p.k_cache : p.v_cache) + lr * row_bytes + lc * 16;
+  const int64_t copy_step = kRowsPer * row_bytes;
+  const uint32_t code_dst = smem_u32(ring) + (lane < 16 ? 0 : G::kTileBytes) + lr * RB;
+  // block scales: kScaleChunks 16-byte chunks of K, then of V (in two
+  // instructions at D = 256); a chunk's group of 16 tokens and first token
+  constexpr int kScaleChunks = G::kTileScales / 16;  // 8, 16 or 32
+  constexpr int kScaleCopies = 2 * kScaleChunks > 32 ? 2 : 1;
+  const int sx = lane % kScaleChunks, sg = sx / (kScaleChunks / 2), s_first = sx * 16 / SB;
+  const uint8_t* scale_src =
+      (kScaleCopies == 1 && lane >= kScaleChunks ? p.v_block : p.k_block) + (sx % (kScaleChunks / 2)) * 16;
+  const uint32_t scale_dst = smem_u32(ring) + 2 * G::kTileBytes + lane * 16;
+  auto entry = [&](int i) { return seg_ring + (i & (kSegRing - 1)) * 2; };
+  auto segment_of = [&](int i) {
+    const int4 x = volatile_at(entry(i)), y = volatile_at(entry(i) + 1);
+    Segment g;
+    g.b = x.x; g.kvh = x.y; g.tile0 = x.z; g.ntiles = x.w;
+    g.seqlen = y.x; g.pair = y.y; g.nseg = y.z; g.cfirst = y.w;
+    return g;
   };
-  auto walk_of = [&](const Segment& s) {
-    Walk w;
-    w.b = s.b;
-    w.kvh = s.kvh / p.row_tiles;
-    w.tok0 = s.tile0 * kTileTokens + warp * kSubTokens;
-    const int64_t stop = static_cast<int64_t>(s.tile0 + s.ntiles) * kTileTokens;
-    w.end = static_cast<int>(stop < s.seqlen ? stop : s.seqlen);
-    w.count = w.end > w.tok0 ? (w.end - w.tok0 + kTileTokens - 1) / kTileTokens : 0;
-    return w;
+  auto fetch_ids = [&](int k0) {  // batch of stages k0 ..
+    const int4 x = volatile_at(entry(seg_w - 1));
+    const int tok = (x.z + k0 + (lane >> 1)) * step + tw * kSubTokens + (lane & 1) * 16;
+    next_row = -1;
+    if (k0 + (lane >> 1) < x.w && tok < pc_end) {
+      const uint32_t pg = static_cast<uint32_t>(tok) / static_cast<uint32_t>(p.page);
+      next_row = static_cast<int>(static_cast<uint32_t>(tok) - pg * static_cast<uint32_t>(p.page));
+      next_id = __ldg(p.block_table + x.x * p.bt_stride + pg);
+    }
   };
-  auto load_ids = [&](const Walk& w, int k0) {
-    const int tok = w.tok0 + (k0 + lane) * kTileTokens;
-    const int32_t* row = p.block_table + w.b * p.bt_stride;
+  auto turn_batch = [&](int k0) {  // next_* become offs, and the batch after it is fetched
+    __syncwarp();
+    longlong2 o;
+    o.x = o.y = -1;
+    if (next_row >= 0 && (next_id < 0 || next_id >= p.num_blocks)) {
+      report_status(p.err, kStatusBadPage);  // its rows are read as zeros
+    } else if (next_row >= 0) {
+      const int head = volatile_at(entry(seg_w - 1)).y / p.row_tiles * HW + hw;
+      o.x = (static_cast<int64_t>(next_id) * p.page + next_row) * row_bytes + head * RB;
+      o.y = ((static_cast<int64_t>(next_id) * p.num_heads_k + head) * p.page + next_row) * SB;
+    }
+    offs[lane] = o;
+    __syncwarp();
+    fetch_ids(k0 + 16);
+  };
+  auto enter = [&](const Segment& g) {  // publish a segment and prepare its loads
+    __syncwarp();
+    if (lane == 0) {
+      entry(seg_w)[0] = make_int4(g.b, g.kvh, g.tile0, g.ntiles);
+      entry(seg_w)[1] = make_int4(g.seqlen, g.pair, g.nseg, g.cfirst);
+    }
+    __syncwarp();
+    ++seg_w;
+    pc_left = g.ntiles;
+    pc_end = g.seqlen / HW;
+    pc_tok = g.tile0 * step + tw * kSubTokens;
+    pc_k = 0;
+    fetch_ids(0);
+    turn_batch(0);
+  };
+  // Copies the cursor's stage to ring slot `slot`, and moves the cursor on.
+  auto issue = [&](int slot) {
+    if (pc_left > 0) {
+      const uint32_t at = slot * G::kStageBytes;
+      const longlong2* o2 = offs + (pc_k & 15) * 2;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int t = tok + 16 * u;
-      int id = 0;
-      if (k0 + lane < w.count && t < w.end && (u == 0 || p.chunk == 16)) {
-        id = __ldg(row + static_cast<uint32_t>(t) / static_cast<uint32_t>(p.page));
-        if (id < 0 || id >= p.num_blocks) {
-          report_status(p.err, kStatusBadPage);
-          id = static_cast<int>(p.num_blocks);
+      for (int g = 0; g < 2; ++g) {  // 16 tokens of one page
+        const int64_t off = o2[g].x;
+        const uint8_t* src = code_src + off;
+        if (off >= 0) {
+#pragma unroll
+          for (int i = 0; i < kCopies; ++i) {
+            copy16(code_dst + at + (g * 16 + i * kRowsPer) * RB + swizzled<RB>(i * kRowsPer + lr, lc) * 16, src, 16);
+            src += copy_step;
+          }
+        } else {  // no page: zeros
+#pragma unroll
+          for (int i = 0; i < kCopies; ++i)
+            copy16(code_dst + at + (g * 16 + i * kRowsPer) * RB + swizzled<RB>(i * kRowsPer + lr, lc) * 16, code_src, 0);
         }
       }
-      page_ids[u] = id;
-    }
-  };
-  auto issue = [&](const Walk& w, int k, int64_t no) {
-    const int id0 = __shfl_sync(0xffffffffu, page_ids[0], k & 31);
-    const int id1 = __shfl_sync(0xffffffffu, page_ids[1], k & 31);
-    if (lane == 0) {
-      const int slot = static_cast<int>(no % G::kStages);
-      uint8_t* st = ring + slot * G::kStageBytes;
-      uint64_t* bar = bars + slot;
-      const int t = w.tok0 + k * kTileTokens;
-      const int row0 = static_cast<int>(static_cast<uint32_t>(t) % static_cast<uint32_t>(p.page));
-      const bool wide = p.chunk == kSubTokens;
-      const int boxes = wide || t + 16 >= w.end ? 1 : 2;
-      const int box_tokens = wide ? kSubTokens : 16;
-      mbar_arrive_expect_tx(bar, static_cast<uint32_t>(boxes * box_tokens * 2 * (RB + SB)));
-      for (int u = 0; u < boxes; ++u) {
-        const int id = u == 0 ? id0 : id1;
-        const int row = u == 0 ? row0
-                               : static_cast<int>(static_cast<uint32_t>(t + 16) % static_cast<uint32_t>(p.page));
-        tma_load_4d(&tm_k, bar, st + u * 16 * RB, 0, w.kvh, row, id, policy);
-        tma_load_4d(&tm_v, bar, st + G::kTileBytes + u * 16 * RB, 0, w.kvh, row, id, policy);
-        tma_load_3d(&tm_kb, bar, st + 2 * G::kTileBytes + u * G::kHalfScales, row * (SB / 4), w.kvh, id, policy);
-        tma_load_3d(&tm_vb, bar, st + 2 * G::kTileBytes + G::kTileScales + u * G::kHalfScales,
-                    row * (SB / 4), w.kvh, id, policy);
+      // The block scales of tokens behind the sequence's end hold whatever
+      // memory held, NaN too, and 0 * NaN would reach O: they are written as
+      // zeros.
+      if (lane < 2 * kScaleChunks) {
+        const int64_t off = o2[sg].y;
+        int valid = off < 0 ? 0 : 16;
+        if (pc_tok + kSubTokens > pc_end) {
+          const int left = (pc_end - pc_tok - s_first) * SB;
+          valid = left <= 0 ? 0 : (left < valid ? left : valid);
+        }
+        const uint8_t* src = scale_src + (off < 0 ? 0 : off);
+        copy16(scale_dst + at, src, valid);
+        if constexpr (kScaleCopies == 2) copy16(scale_dst + at + G::kTileScales, src + (p.v_block - p.k_block), valid);
+      }
+      ++pc_k;
+      pc_tok += step;
+      if (--pc_left == 0) {
+        const Schedule sched = schedule();
+        Segment nx;
+        if (sched.next(segment_of(seg_w - 1), sched.range_start(cta + 1), nx)) enter(nx);
+      } else if ((pc_k & 15) == 0) {
+        turn_batch(pc_k);
       }
     }
+    copy_commit();  // one group a stage, empty ones too, so that the count of groups stays fixed
   };
-  // First loads of a segment.
-  auto start = [&](const Walk& w) {
-    load_ids(w, 0);
-    for (int k = 0; k < G::kStages && k < w.count; ++k) issue(w, k, stage_no + k);
-  };
-
-  // ------------------------------------------------------------ segments
-  Segment seg{};
-  bool have = sched.first(cta, seg);
-  Walk w{};
-  if (have) {
-    w = walk_of(seg);
-    start(w);
+  {
+    const Schedule sched = schedule();
+    Segment g;
+    if (sched.first(cta, g)) enter(g);
   }
-  bool failed = false;
-  while (have) {
-    const int row_tile = seg.kvh - w.kvh * p.row_tiles;
-    const int row_base = row_tile * p.rows;
-    const int nrows = p.qrows - row_base < G::kRows ? p.qrows - row_base : G::kRows;
-    // ---- query fragments: lane (r, c) holds values c * D / 4 .. of row r
+  // ------------------------------------------------------------ segments
+  int slot = 0;
+  // The lane's places in a stage.  tau: token of row r of an 8-token half
+  // tile (neighbours swapped in every second pair); tx, ty: tau of rows 2 c
+  // and 2 c + 1.  Rows 8, 16 and 24 further on have the same swizzle.
+  const int tau = r ^ ((r >> 1) & 1);
+  const int tx = (2 * c) ^ (c & 1), ty = (2 * c + 1) ^ (c & 1);
+  int k_at, k_at2 = 0, v_at[2];
+  if constexpr (D == 256) {
+    k_at = tau * RB + swizzled<RB>(tau, 2 * c) * 16;
+    k_at2 = tau * RB + swizzled<RB>(tau, 2 * c + 1) * 16;
+    v_at[0] = tx * RB + swizzled<RB>(tx, r) * 16;
+    v_at[1] = ty * RB + swizzled<RB>(ty, r) * 16;
+  } else if constexpr (D == 128) {
+    k_at = tau * RB + swizzled<RB>(tau, c) * 16;
+    v_at[0] = tx * RB + swizzled<RB>(tx, r >> 1) * 16 + (r & 1) * 8;
+    v_at[1] = ty * RB + swizzled<RB>(ty, r >> 1) * 16 + (r & 1) * 8;
+  } else {
+    k_at = tau * RB + swizzled<RB>(tau, c >> 1) * 16 + (c & 1) * 8;
+    v_at[0] = tx * RB + swizzled<RB>(tx, r >> 2) * 16 + (r & 3) * 4;
+    v_at[1] = ty * RB + swizzled<RB>(ty, r >> 2) * 16 + (r & 3) * 4;
+  }
+  const int ks_at = 2 * G::kTileBytes + tau * SB + c * (D / 64);
+  const int vs_at[2] = {2 * G::kTileBytes + G::kTileScales + tx * SB + r * (D / 8) / 16,
+                        2 * G::kTileBytes + G::kTileScales + ty * SB + r * (D / 8) / 16};
+
+  for (int seg_r = 0; seg_r < seg_w; ++seg_r) {
+    int ntiles, t0, seqlen;
+    {
+      const Segment g = segment_of(seg_r);
+      ntiles = g.ntiles;
+      t0 = g.tile0 * step + tw * kSubTokens;
+      seqlen = g.seqlen / HW;
+    }
+    // sequence, KV head, first query row of the pass and its rows
+    struct Place {
+      int b, kvh, row_base, nrows;
+    };
+    auto place = [&]() {
+      const int4 x = volatile_at(entry(seg_r));
+      Place g;
+      g.b = x.x;
+      g.kvh = x.y / p.row_tiles * HW + hw;
+      g.row_base = (x.y % p.row_tiles) * p.rows;
+      g.nrows = p.qrows - g.row_base < G::kRows ? p.qrows - g.row_base : G::kRows;
+      return g;
+    };
+    // ---- query fragments: lane (r, c) holds values c * D / 4 .. of row r.
+    // The logits' factor is made positive (its sign goes to the query, and a
+    // factor of zero too), so that the largest product is the largest logit.
     uint32_t qf[NT][KS][2];
+    float qfac[NT][2];  // per column of the lane (query rows 2 c, 2 c + 1 of each 8)
+    {
+    const Place at = place();
+    const int b = at.b, kvh = at.kvh, row_base = at.row_base, nrows = at.nrows;
+    const float factor = __ldg(p.k_scale + kvh) * p.scale_log2;
+    const float sign = factor > 0.f ? 1.f : (factor < 0.f ? -1.f : factor);
     float row_inv[NT];  // 2^-k of the row's scaling
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -352,14 +468,14 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
         const int h = row_base + n, qi = MULTI ? h / p.group : 0, g = h - qi * p.group;
         const uint4* src = reinterpret_cast<const uint4*>(
             static_cast<const T*>(p.q) +
-            ((static_cast<int64_t>(seg.b) * p.seqlen_q + qi) * p.num_heads + w.kvh * p.group + g) * D + c * (D / 4));
+            ((static_cast<int64_t>(b) * p.seqlen_q + qi) * p.num_heads + kvh * p.group + g) * D + c * (D / 4));
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) raw[i] = __ldg(src + i);
       } else {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) raw[i] = make_uint4(0, 0, 0, 0);
       }
-      float sc = 1.f;
+      float sc = sign;
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         float mx = 0.f;
 #pragma unroll
@@ -376,7 +492,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
         if (mx > 0.f && mx <= 3.4e38f) {
           int k = 13 - (((__float_as_int(mx) >> 23) & 0xff) - 127);
           k = k > 126 ? 126 : (k < -126 ? -126 : k);
-          sc = __int_as_float((k + 127) << 23);
+          sc = __int_as_float((k + 127) << 23) * sign;
           row_inv[nt] = __int_as_float((127 - k) << 23);
         }
       }
@@ -389,31 +505,24 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
           if constexpr (std::is_same<T, __nv_bfloat16>::value) {
             const float2 f = pair_to_float2<T>(x[j]);
             h = pack_half2(f.x * sc, f.y * sc);
+          } else {
+            h = hmul2_bits(h, pack_half2(sc, sc));
           }
           qf[nt][2 * i + (j >> 1)][j & 1] = h;  // step s: values 4 s .. 4 s + 3 of the lane's
         }
       }
     }
-    // Per column of the lane (query rows 2 c, 2 c + 1 of each 8): the factor
-    // of the logits, and how far from the end the row's last key lies.
-    float qfac[NT][2];
-    int seen[NT][2];
-    {
-      const float f = __ldg(p.k_scale + w.kvh) * p.scale_log2;
+    const float f = factor == 0.f ? 1.f : fabsf(factor);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          qfac[nt][e] = f * __shfl_sync(0xffffffffu, row_inv[nt], (2 * c + e) * 4);
-          const int h = row_base + nt * 8 + 2 * c + e;
-          seen[nt][e] = seg.seqlen + ((MULTI && p.causal) ? h / p.group - (p.seqlen_q - 1) : 0);
-        }
-      }
+      for (int e = 0; e < 2; ++e) qfac[nt][e] = f * __shfl_sync(0xffffffffu, row_inv[nt], (2 * c + e) * 4);
     }
-    const int all_seen = seg.seqlen - ((MULTI && p.causal) ? p.seqlen_q - 1 : 0);  // by every row
+    const int all_seen = seqlen - ((MULTI && p.causal) ? p.seqlen_q - 1 : 0);  // keys that every row sees
 
     float acc[MT][NT][4];
     float m[NT][2], l[NT][2];
+    float m_use[NT][2];  // m, or 0 while no key was seen (then every P is 0)
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -423,124 +532,134 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = neg_inf;
+      m_use[nt][0] = m_use[nt][1] = 0.f;
       l[nt][0] = l[nt][1] = 0.f;
     }
-    // token of row i of an 8-token half tile: neighbours swapped in every second pair
-    const int tau = r ^ ((r >> 1) & 1);
-    const int tx = (2 * c) ^ (c & 1), ty = (2 * c + 1) ^ (c & 1);  // tau(2 c), tau(2 c + 1)
 
-    for (int k = 0; k < w.count; ++k) {
-      const int64_t no = stage_no + k;
-      const int slot = static_cast<int>(no % G::kStages);
-      if (!failed && !mbar_wait_bounded(bars + slot, static_cast<uint32_t>((no / G::kStages) & 1), abort_flag,
-                                        p.timeout_ns))
-        failed = true;
-      failed = __any_sync(0xffffffffu, failed);
-      if (failed) break;
+    // Before the first segment's first tile the ring is filled, by rounds that
+    // only issue (one place in the code: it is long, and cold at a launch's start).
+    for (int k = seg_r == 0 ? -G::kStages : 0; k < ntiles; ++k) {
+      if (k >= 0) {
+      copy_wait<G::kStages - 1>();
+      __syncwarp();  // every lane's copies of the stage have landed
       const uint8_t* st = ring + slot * G::kStageBytes;
-      const uint8_t* sk = st + 2 * G::kTileBytes;
-      const uint8_t* sv = sk + G::kTileScales;
-      const int t0 = w.tok0 + k * kTileTokens;
 
-      // ---- S^T = K . Q^T, two tiles of 16 tokens
+      // ---- S^T = K . Q^T, two tiles of 16 tokens side by side
       float s[2][NT][4];
+      uint32_t kw[2][2][KW];               // [tile][rows r, r + 8]: the lane's codes
+      uint32_t kf[2][2][(D + 127) / 128];  // and the f16 pairs of their block scales
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
-        const int ra = mt * 16 + tau, rb = ra + 8;
-        uint32_t ka[KW], kb[KW];
-        if constexpr (KW == 8) {
-          uint32_t x[4], y[4];
-          load_words<4>(st + ra * RB + swizzled<RB>(ra, 2 * c) * 16, x);
-          load_words<4>(st + ra * RB + swizzled<RB>(ra, 2 * c + 1) * 16, y);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { ka[i] = x[i]; ka[4 + i] = y[i]; }
-          load_words<4>(st + rb * RB + swizzled<RB>(rb, 2 * c) * 16, x);
-          load_words<4>(st + rb * RB + swizzled<RB>(rb, 2 * c + 1) * 16, y);
+        for (int half = 0; half < 2; ++half) {
+          const int row = mt * 16 + half * 8;
+          const uint8_t* sc = st + ks_at + row * SB;
+          if constexpr (D == 256) {
+            uint32_t x[4], y[4];
+            load_words<4>(st + k_at + row * RB, x);
+            load_words<4>(st + k_at2 + row * RB, y);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { kb[i] = x[i]; kb[4 + i] = y[i]; }
-        } else if constexpr (KW == 4) {
-          load_words<4>(st + ra * RB + swizzled<RB>(ra, c) * 16, ka);
-          load_words<4>(st + rb * RB + swizzled<RB>(rb, c) * 16, kb);
-        } else {
-          load_words<2>(st + ra * RB + swizzled<RB>(ra, c >> 1) * 16 + (c & 1) * 8, ka);
-          load_words<2>(st + rb * RB + swizzled<RB>(rb, c >> 1) * 16 + (c & 1) * 8, kb);
+            for (int i = 0; i < 4; ++i) { kw[mt][half][i] = x[i]; kw[mt][half][4 + i] = y[i]; }
+            const uint32_t q = *reinterpret_cast<const uint32_t*>(sc);
+            kf[mt][half][0] = e4m3x2_to_half2(q);
+            kf[mt][half][1] = e4m3x2_to_half2(q >> 16);
+          } else if constexpr (D == 128) {
+            load_words<4>(st + k_at + row * RB, kw[mt][half]);
+            kf[mt][half][0] = e4m3x2_to_half2(*reinterpret_cast<const uint16_t*>(sc));
+          } else {
+            load_words<2>(st + k_at + row * RB, kw[mt][half]);
+            kf[mt][half][0] = e4m3x2_to_half2(*sc);
+          }
         }
-        // block scales of the lane's values: D / 64 bytes of a row
-        uint32_t wa, wb;
-        const uint8_t* sa = sk + mt * half_scales + tau * SB;
-        if constexpr (D == 256) {
-          wa = *reinterpret_cast<const uint32_t*>(sa + 4 * c);
-          wb = *reinterpret_cast<const uint32_t*>(sa + 8 * SB + 4 * c);
-        } else if constexpr (D == 128) {
-          wa = *reinterpret_cast<const uint16_t*>(sa + 2 * c);
-          wb = *reinterpret_cast<const uint16_t*>(sa + 8 * SB + 2 * c);
-        } else {
-          wa = sa[c];
-          wb = sa[8 * SB + c];
-        }
+      }
 #pragma unroll
-        for (int wi = 0; wi < KW; ++wi) {
-          const int blk = wi / 2;  // two words a block
-          const uint32_t pa = e4m3x2_to_half2(wa >> (16 * (blk / 2))), pb = e4m3x2_to_half2(wb >> (16 * (blk / 2)));
-          const uint32_t fa = __byte_perm(pa, pa, blk & 1 ? 0x3232 : 0x1010);
-          const uint32_t fb = __byte_perm(pb, pb, blk & 1 ? 0x3232 : 0x1010);
-          uint32_t ha[4], hb[4];
-          e2m1x8_to_half2x4(ka[wi], ha);
-          e2m1x8_to_half2x4(kb[wi], hb);
+      for (int wi = 0; wi < KW; ++wi) {
+        const int blk = wi / 2;  // two words a block
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            ha[j] = hmul2_bits(ha[j], fa);
-            hb[j] = hmul2_bits(hb[j], fb);
+        for (int mt = 0; mt < 2; ++mt) {
+          uint32_t h[2][4];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t pair = kf[mt][half][blk / 2];
+            const uint32_t f = __byte_perm(pair, pair, blk & 1 ? 0x3232 : 0x1010);
+            e2m1x8_to_half2x4(kw[mt][half][wi], h[half]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[half][j] = hmul2_bits(h[half][j], f);
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(s[mt][nt], ha[0], hb[0], ha[1], hb[1], qf[nt][2 * wi][0], qf[nt][2 * wi][1]);
-            mma_f16(s[mt][nt], ha[2], hb[2], ha[3], hb[3], qf[nt][2 * wi + 1][0], qf[nt][2 * wi + 1][1]);
+            mma_f16(s[mt][nt], h[0][0], h[1][0], h[0][1], h[1][1], qf[nt][2 * wi][0], qf[nt][2 * wi][1]);
+            mma_f16(s[mt][nt], h[0][2], h[1][2], h[0][3], h[1][3], qf[nt][2 * wi + 1][0], qf[nt][2 * wi + 1][1]);
           }
         }
       }
 
-      // ---- softmax over the stage (log2 domain)
-      const bool edge = t0 + kSubTokens > all_seen;  // some row does not see some token
+      // ---- softmax over the warp's 32 tokens (log2 domain)
+      if (t0 + kSubTokens > all_seen) {  // some row does not see some token
+        const int len = volatile_at(entry(seg_r) + 1).x / HW, base = MULTI ? place().row_base : 0;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+          for (int e = 0; e < 2; ++e) {
+            // causal: row (qi, g) sees the keys up to its own position
+            const int seen =
+                len + ((MULTI && p.causal) ? (base + nt * 8 + 2 * c + e) / p.group - (p.seqlen_q - 1) : 0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = s[mt][nt][e] * qfac[nt][e & 1];
-            const int t = t0 + mt * 16 + tau + (e >> 1) * 8;
-            s[mt][nt][e] = edge && t >= seen[nt][e & 1] ? neg_inf : x;
+            for (int mt = 0; mt < 2; ++mt) {
+              if (t0 + mt * 16 + tau >= seen) s[mt][nt][e] = neg_inf;
+              if (t0 + mt * 16 + tau + 8 >= seen) s[mt][nt][e + 2] = neg_inf;
+            }
+          }
+      }
+      // The reference of the exponents need not be the maximum: it is raised
+      // (and O, l rescaled) only when a logit exceeds it by more than 8, so
+      // that P stays below 2^8, well inside f16, and most stages need no
+      // reduction over the tokens' lanes.  Rounded up, it bounds the exact
+      // products that the exponents subtract it from, however large.
+      bool above = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float mx = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+          above = above || __fmul_ru(mx, qfac[nt][e]) - m[nt][e] > 8.f;
+        }
+      if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float m_new = fmaxf(m[nt][e], __fmul_ru(mx, qfac[nt][e]));
+            const float alpha = m_new == m[nt][e] ? 1.f : fast_exp2(m[nt][e] - m_new);
+            m[nt][e] = m_new;
+            m_use[nt][e] = m_new == neg_inf ? 0.f : m_new;
+            l[nt][e] *= alpha;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              acc[i][nt][e] *= alpha;
+              acc[i][nt][e + 2] *= alpha;
+            }
           }
       }
       uint32_t pt[2][NT][2];  // P^T fragments of each 16 tokens
-      bool moved = false;
-      float alpha[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float m_new = fmaxf(m[nt][e], mx);
-          const float m_use = m_new == neg_inf ? 0.f : m_new;
-          alpha[nt][e] = fast_exp2(m[nt][e] - m_use);
-          moved = moved || m_new != m[nt][e];
-          m[nt][e] = m_new;
-          float sum = 0.f;
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
-            s[mt][nt][e] = fast_exp2(s[mt][nt][e] - m_use);
-            s[mt][nt][e + 2] = fast_exp2(s[mt][nt][e + 2] - m_use);
-            sum += s[mt][nt][e] + s[mt][nt][e + 2];
+            s[mt][nt][e] = fast_exp2(fmaf(s[mt][nt][e], qfac[nt][e], -m_use[nt][e]));
+            s[mt][nt][e + 2] = fast_exp2(fmaf(s[mt][nt][e + 2], qfac[nt][e], -m_use[nt][e]));
           }
-          l[nt][e] = fmaf(l[nt][e], alpha[nt][e], sum);
+          l[nt][e] += (s[0][nt][e] + s[0][nt][e + 2]) + (s[1][nt][e] + s[1][nt][e + 2]);
         }
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
@@ -548,46 +667,29 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
           pt[mt][nt][1] = transpose8x8(pack_half2(s[mt][nt][2], s[mt][nt][3]));
         }
       }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][nt][e] *= alpha[nt][e & 1];
-      }
 
       // ---- O^T += V^T . P^T
-      const bool tail = t0 + kSubTokens > seg.seqlen;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        const int rows[4] = {ks * 16 + tx, ks * 16 + ty, ks * 16 + tx + 8, ks * 16 + ty + 8};
-        uint32_t v[4][VW];
-        uint32_t sc[4];
+        uint32_t v[4][VW], sc[4];  // tokens tx, ty, tx + 8, ty + 8 of the 16
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int row = rows[u];
-          const uint8_t* base = st + G::kTileBytes + row * RB;
-          const uint8_t* sb = sv + ks * half_scales + (row - ks * 16) * SB;
-          if constexpr (D == 256) {
-            load_words<4>(base + swizzled<RB>(row, r) * 16, v[u]);
-            sc[u] = *reinterpret_cast<const uint16_t*>(sb + 2 * r);
-          } else if constexpr (D == 128) {
-            load_words<2>(base + swizzled<RB>(row, r >> 1) * 16 + (r & 1) * 8, v[u]);
-            sc[u] = sb[r];
-          } else {
-            load_words<1>(base + swizzled<RB>(row, r >> 2) * 16 + (r & 3) * 4, v[u]);
-            sc[u] = sb[r >> 1];
-          }
-          // Rows past the sequence hold whatever memory held, NaN scales too,
-          // and 0 * NaN would reach O: their scales are zeroed.
-          if (tail && t0 + row >= seg.seqlen) sc[u] = 0u;
+          const int row = ks * 16 + (u >> 1) * 8;
+          load_words<VW>(st + G::kTileBytes + v_at[u & 1] + row * RB, v[u]);
+          const uint8_t* sb = st + vs_at[u & 1] + row * SB;
+          sc[u] = D == 256 ? *reinterpret_cast<const uint16_t*>(sb) : *sb;
         }
 #pragma unroll
         for (int wi = 0; wi < VW; ++wi) {
-          const int sh = D == 256 ? 8 * (wi >> 1) : 0;  // the word's block
-          const uint32_t f0 = e4m3x2_to_half2(((sc[0] >> sh) & 0xFFu) | (((sc[1] >> sh) & 0xFFu) << 8));
-          const uint32_t f1 = e4m3x2_to_half2(((sc[2] >> sh) & 0xFFu) | (((sc[3] >> sh) & 0xFFu) << 8));
+          uint32_t w0, w1;  // the block scales of the word's block, of two tokens each
+          if constexpr (D == 256) {
+            w0 = __byte_perm(sc[0], sc[1], wi < 2 ? 0x0040 : 0x0051);
+            w1 = __byte_perm(sc[2], sc[3], wi < 2 ? 0x0040 : 0x0051);
+          } else {
+            w0 = sc[0] + sc[1] * 256u;
+            w1 = sc[2] + sc[3] * 256u;
+          }
+          const uint32_t f0 = e4m3x2_to_half2(w0), f1 = e4m3x2_to_half2(w1);
           // even codes of both tokens in one word, odd codes in another
           uint32_t e0[4], o0[4], e1[4], o1[4];
           e2m1x8_to_half2x4((v[0][wi] & 0x0F0F0F0Fu) | ((v[1][wi] << 4) & 0xF0F0F0F0u), e0);
@@ -604,204 +706,227 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
           }
         }
       }
-
+      t0 += step;
+      }
       // ---- refill the stage
-      const int kn = k + G::kStages;
-      __syncwarp();  // every lane has read the stage
-      if (kn < w.count) {
-        if ((kn & 31) == 0) load_ids(w, kn);
-        issue(w, kn, no + G::kStages);
-      }
-    }
-    stage_no += w.count;
-
-    // ---- next segment's first loads
-    Segment nx{};
-    const bool have_nx = sched.next(seg, range_end, nx);
-    const Walk done = w;
-    if (have_nx && !failed) {
-      w = walk_of(nx);
-      start(w);
+      __syncwarp();  // every lane has read it
+      issue(slot);
+      slot = slot + 1 == G::kStages ? 0 : slot + 1;
     }
 
-    // ---- join the warps
+    // ---- the rows' sums; warps that share a head are joined on its first
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float x = l[nt][e];
-        x += __shfl_xor_sync(0xffffffffu, x, 4);
-        x += __shfl_xor_sync(0xffffffffu, x, 8);
-        x += __shfl_xor_sync(0xffffffffu, x, 16);
-        if (r == 0) {
-          float* d = ml + (warp * G::kRows + nt * 8 + 2 * c + e) * 2;
-          d[0] = m[nt][e];
-          d[1] = x;
-        }
+        l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4);
+        l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
+        l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
       }
-    __syncthreads();
-    const bool stop = *abort_flag != 0;
-    // O of this warp relative to the CTA's maximum
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = nt * 8 + 2 * c + e;
-        float mm = neg_inf;
-#pragma unroll
-        for (int i = 0; i < kFp4Warps; ++i) mm = fmaxf(mm, ml[(i * G::kRows + row) * 2]);
-        const float f = m[nt][e] == mm ? 1.f : fast_exp2(m[nt][e] - mm);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          acc[i][nt][e] *= f;
-          acc[i][nt][e + 2] *= f;
-        }
-      }
-    // Lane (r, c) holds dims r * D / 8 + 2 i (entries e) and + 2 i + 1
-    // (entries e + 2) of rows 2 c + e.  Warps 2, 3 leave their sums for 0, 1,
-    // which add them; the two halves are added when they are written out.
-    auto at = [&](int half, int nt, int e) {
-      return join + (half * G::kRows + nt * 8 + 2 * c + e) * G::kRowPad + r * (D / 8);
-    };
-#pragma unroll
-    for (int phase = 0; phase < 2; ++phase) {
-      if ((phase == 0) == (warp >= 2)) {
+    if (TW > 1) {
+      // Lane (r, c) holds dims r * D / 8 + 2 i (entries e) and + 2 i + 1
+      // (entries e + 2) of rows 2 c + e.
+      if (tw > 0) {
+        float* buf = reinterpret_cast<float*>(smem + G::kOffJoin + (warp - HW) * G::kJoinWarp);
+        float* ml = buf + G::kRows * G::kRowPad;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float4* d = reinterpret_cast<float4*>(at(warp & 1, nt, e));
+            const int row = nt * 8 + 2 * c + e;
+            float4* d = reinterpret_cast<float4*>(buf + row * G::kRowPad + r * (D / 8));
 #pragma unroll
-            for (int i = 0; i < MT; i += 2) {
-              float4 x = make_float4(acc[i][nt][e], acc[i][nt][e + 2], acc[i + 1][nt][e], acc[i + 1][nt][e + 2]);
-              if (phase == 1) {
-                const float4 y = d[i / 2];
-                x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-              }
-              d[i / 2] = x;
+            for (int i = 0; i < MT; i += 2)
+              d[i / 2] = make_float4(acc[i][nt][e], acc[i][nt][e + 2], acc[i + 1][nt][e], acc[i + 1][nt][e + 2]);
+            if (r == 0) {
+              ml[row * 2] = m[nt][e];
+              ml[row * 2 + 1] = l[nt][e];
             }
           }
       }
       __syncthreads();
+      if (tw == 0) {
+        for (int o = 1; o < TW; ++o) {
+          const float* buf = reinterpret_cast<const float*>(smem + G::kOffJoin + (warp + (o - 1) * HW) * G::kJoinWarp);
+          const float* ml = buf + G::kRows * G::kRowPad;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int row = nt * 8 + 2 * c + e;
+              const float mo = ml[row * 2], mm = fmaxf(m[nt][e], mo);
+              // equal references (both -inf too) weigh 1, so that NaN sums stay
+              const float fa = m[nt][e] == mm ? 1.f : fast_exp2(m[nt][e] - mm);
+              const float fb = mo == mm ? 1.f : fast_exp2(mo - mm);
+              m[nt][e] = mm;
+              l[nt][e] = fmaf(l[nt][e], fa, ml[row * 2 + 1] * fb);
+              const float4* d = reinterpret_cast<const float4*>(buf + row * G::kRowPad + r * (D / 8));
+#pragma unroll
+              for (int i = 0; i < MT; i += 2) {
+                const float4 x = d[i / 2];
+                acc[i][nt][e] = fmaf(acc[i][nt][e], fa, x.x * fb);
+                acc[i][nt][e + 2] = fmaf(acc[i][nt][e + 2], fa, x.y * fb);
+                acc[i + 1][nt][e] = fmaf(acc[i + 1][nt][e], fa, x.z * fb);
+                acc[i + 1][nt][e + 2] = fmaf(acc[i + 1][nt][e + 2], fa, x.w * fb);
+              }
+            }
+        }
+      }
+      __syncthreads();  // the buffers are free again
     }
 
     // ---- write: the output, or a partial of a pair cut by range boundaries
-    constexpr int kLanes = D / 4;                        // threads of a row, 4 dims each
-    constexpr int kRowsPerPass = kFp4Threads / kLanes;
-    const int d4 = (tid % kLanes) * 4;
-    const int64_t part = static_cast<int64_t>(cta) + seg.pair;
-    const bool direct = seg.nseg == 1;
-    auto write_row = [&](int row, float4 o, float lse2) {
+    const Place at = place();
+    const int b = at.b, kvh = at.kvh, row_base = at.row_base, nrows = at.nrows;
+    const int4 sb = volatile_at(entry(seg_r) + 1);
+    const int pair = sb.y, nseg = sb.z, cfirst = sb.w;
+    const int64_t part = (static_cast<int64_t>(cta) + pair) * HW + hw;
+    const float vs = __ldg(p.v_scale + kvh);
+    const int rows = p.rows;
+    // out and lse places of row `row`
+    auto out_at = [&](int row) {
       const int h = row_base + row, qi = MULTI ? h / p.group : 0, g = h - qi * p.group;
-      const int64_t head = done.kvh * p.group + g;
-      OutT* dst = static_cast<OutT*>(p.out) +
-                  ((static_cast<int64_t>(done.b) * p.seqlen_q + qi) * p.num_heads + head) * D + d4;
-      dst[0] = fp4_out<OutT>(o.x);
-      dst[1] = fp4_out<OutT>(o.y);
-      dst[2] = fp4_out<OutT>(o.z);
-      dst[3] = fp4_out<OutT>(o.w);
-      if (p.lse != nullptr && d4 == 0)
-        p.lse[(static_cast<int64_t>(done.b) * p.num_heads + head) * p.seqlen_q + qi] =
-            lse2 == neg_inf ? neg_inf : lse2 * 0.69314718055994531f;
+      return static_cast<OutT*>(p.out) +
+             ((static_cast<int64_t>(b) * p.seqlen_q + qi) * p.num_heads + kvh * p.group + g) * D;
     };
-    const float vs = __ldg(p.v_scale + done.kvh);
-    if (!stop) {
-      for (int row = tid / kLanes; row < nrows; row += kRowsPerPass) {
-        float mm = neg_inf, ll = 0.f;
+    auto put_lse = [&](int row, float lse2) {
+      const int h = row_base + row, qi = MULTI ? h / p.group : 0, g = h - qi * p.group;
+      if (p.lse != nullptr)
+        p.lse[(static_cast<int64_t>(b) * p.num_heads + kvh * p.group + g) * p.seqlen_q + qi] =
+            lse2 * 0.69314718055994531f;
+    };
+    if (tw == 0) {
 #pragma unroll
-        for (int i = 0; i < kFp4Warps; ++i) mm = fmaxf(mm, ml[(i * G::kRows + row) * 2]);
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < kFp4Warps; ++i) {
-          const float mi = ml[(i * G::kRows + row) * 2];
-          ll = fmaf(mi == mm ? 1.f : fast_exp2(mi - mm), ml[(i * G::kRows + row) * 2 + 1], ll);
+        for (int e = 0; e < 2; ++e) {
+          const int row = nt * 8 + 2 * c + e;
+          if (row >= nrows) continue;
+          const bool some = !(l[nt][e] == 0.f);  // a row that saw a key (NaN stays NaN)
+          const float inv = some ? vs / l[nt][e] : 0.f;
+          const float lse2 = some ? m[nt][e] + fast_log2(l[nt][e]) : neg_inf;
+          float o[D / 8];
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            o[2 * i] = some ? acc[i][nt][e] * inv : 0.f;
+            o[2 * i + 1] = some ? acc[i][nt][e + 2] * inv : 0.f;
+          }
+          if (nseg == 1) {
+            store_row<OutT, D / 8>(out_at(row) + r * (D / 8), o);
+            if (r == 0) put_lse(row, lse2);
+          } else {
+            store_row<float, D / 8>(p.part_o + (part * rows + row) * D + r * (D / 8), o);
+            if (r == 0) p.part_lse[part * rows + row] = lse2;
+          }
         }
-        const float4 x = *reinterpret_cast<const float4*>(join + row * G::kRowPad + d4);
-        const float4 y = *reinterpret_cast<const float4*>(join + (G::kRows + row) * G::kRowPad + d4);
-        const bool some = !(ll == 0.f);  // a row that saw a key (NaN stays NaN)
-        const float inv = some ? vs / ll : 0.f;
-        const float4 o = some ? make_float4((x.x + y.x) * inv, (x.y + y.y) * inv, (x.z + y.z) * inv,
-                                            (x.w + y.w) * inv)
-                              : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float lse2 = some ? mm + fast_log2(ll) : neg_inf;
-        if (direct) {
-          write_row(row, o, lse2);
-        } else {
-          *reinterpret_cast<float4*>(p.part_o + (part * p.rows + row) * D + d4) = o;
-          if (d4 == 0) p.part_lse[part * p.rows + row] = lse2;
-        }
-      }
     }
-    if (!direct && !stop) {
+    if (nseg == 1) continue;
+    int last = 0;
+    if (tw == 0) {
       __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        const int is_last = ticket_arrive(p.tickets + seg.pair, *launch_epoch, seg.nseg) ? 1 : 0;
-        if (is_last) *reinterpret_cast<volatile unsigned long long*>(p.tickets + seg.pair) = 0ull;
-        *last_flag = is_last;
+      __syncwarp();
+      if (lane == 0) {
+        unsigned long long* ticket = p.tickets + static_cast<int64_t>(pair) * HW + hw;
+        last = ticket_arrive(ticket, *launch_epoch, nseg) ? 1 : 0;
+        // every segment of the pair has counted itself: clear for later launches
+        if (last) *reinterpret_cast<volatile unsigned long long*>(ticket) = 0ull;
       }
+      last = __shfl_sync(0xffffffffu, last, 0);
+    }
+    if (TW > 1) {  // the head's other warps take a share of the rows
+      if (tw == 0 && lane == 0) last_flag[hw] = last;
       __syncthreads();
-      if (*last_flag) {
-        __threadfence();
-        const int64_t base = static_cast<int64_t>(seg.cfirst) + seg.pair;
-        const float* plse = p.part_lse + base * p.rows;
-        const float* po = p.part_o + base * p.rows * D + d4;
-        for (int row = tid / kLanes; row < nrows; row += kRowsPerPass) {
-          float mm = neg_inf;
-          for (int j = 0; j < seg.nseg; ++j) mm = fmaxf(mm, __ldcg(plse + static_cast<int64_t>(j) * p.rows + row));
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          float den = 0.f;
-          constexpr int kBatch = 8;
-          for (int j0 = 0; j0 < seg.nseg; j0 += kBatch) {
-            float4 x[kBatch];
-            float lj[kBatch];
+      last = last_flag[hw];
+      __syncthreads();
+    }
+    if (!last) continue;
+    __threadfence();
+    // The last of the pair's segments joins them: partial j of the head is
+    // part (cfirst + j + pair) * HW + hw.  A warp takes a row at a time and
+    // adds kBatch partials per round, their loads in flight together; the
+    // weights are kept relative to a running maximum.
+    const int64_t first = (static_cast<int64_t>(cfirst) + pair) * HW + hw;
+    const float* plse = p.part_lse + first * rows;
+    const float* po = p.part_o + first * rows * D;
+    const int64_t lse_step = static_cast<int64_t>(HW) * rows, o_step = lse_step * D;
+    constexpr int kVec = D >= 128 ? 4 : 2, kPieces = D / (32 * kVec);
+    constexpr int kBatch = D == 256 ? 8 : 16;
+#pragma unroll 1
+    for (int row = tw; row < nrows; row += TW) {
+      float mm = neg_inf, den = 0.f, o[kPieces][kVec];
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-              const int64_t j = j0 + u;
-              lj[u] = neg_inf;
-              x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (j < seg.nseg) {
-                lj[u] = __ldcg(plse + j * p.rows + row);
-                x[u] = __ldcg(reinterpret_cast<const float4*>(po + (j * p.rows + row) * D));
-              }
-            }
+      for (int q = 0; q < kPieces; ++q)
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-              const float wj = lj[u] == neg_inf ? 0.f : fast_exp2(lj[u] - mm);
-              if (lj[u] != neg_inf) {
-                o.x = fmaf(wj, x[u].x, o.x);
-                o.y = fmaf(wj, x[u].y, o.y);
-                o.z = fmaf(wj, x[u].z, o.z);
-                o.w = fmaf(wj, x[u].w, o.w);
-                den += wj;
+        for (int i = 0; i < kVec; ++i) o[q][i] = 0.f;
+#pragma unroll 1
+      for (int j0 = 0; j0 < nseg; j0 += kBatch) {
+        float x[kBatch][kPieces][kVec], lj[kBatch];
+        const float* src = po + j0 * o_step + row * D + lane * kVec;
+        const float* lsrc = plse + j0 * lse_step + row;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          lj[u] = neg_inf;
+          if (j0 + u < nseg) {
+            lj[u] = __ldcg(lsrc);
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q) {
+              if constexpr (kVec == 4) {
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(src + q * 32 * kVec));
+                x[u][q][0] = y.x; x[u][q][1] = y.y; x[u][q][2] = y.z; x[u][q][3] = y.w;
+              } else {
+                const float2 y = __ldcg(reinterpret_cast<const float2*>(src + q * 32 * kVec));
+                x[u][q][0] = y.x; x[u][q][1] = y.y;
               }
             }
           }
-          const bool some = !(den == 0.f);
-          const float inv = some ? 1.f / den : 0.f;
-          o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
-          write_row(row, o, some ? mm + fast_log2(den) : neg_inf);
+          src += o_step;
+          lsrc += lse_step;
+        }
+        float m_new = mm;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) m_new = fmaxf(m_new, lj[u]);
+        const float alpha = m_new == mm ? 1.f : fast_exp2(mm - m_new);
+        mm = m_new;
+        den *= alpha;
+#pragma unroll
+        for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) o[q][i] *= alpha;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          if (lj[u] == neg_inf) continue;  // empty (or past the last)
+          const float wj = fast_exp2(lj[u] - m_new);
+          den += wj;
+#pragma unroll
+          for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) o[q][i] = fmaf(wj, x[u][q][i], o[q][i]);
         }
       }
+      const bool some = !(den == 0.f);
+      const float inv = some ? 1.f / den : 0.f;
+      OutT* dst = out_at(row);
+#pragma unroll
+      for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) dst[q * 32 * kVec + lane * kVec + i] = fp4_out<OutT>(o[q][i] * inv);
+      if (lane == 0) put_lse(row, some ? mm + fast_log2(den) : neg_inf);
     }
-    __syncthreads();  // join, ml and last_flag are reused by the next segment
-    seg = nx;
-    have = have_nx && !stop;
-    if (__syncthreads_or(failed)) break;
   }
-  if (*abort_flag) {
-    if (tid == 0) {
-      report_status(p.err, kStatusTimeout);
-      // Let copies in flight land before the CTA's shared memory is released (bounded: 2 ms).
-      const uint64_t t0 = globaltimer_ns();
-      while (globaltimer_ns() - t0 < 2000000ull) {
-      }
+  // Every CTA counts itself once it has read the epoch; the last one hands
+  // the next launch a new epoch (see fd_decode_sm100.cuh).  Here at the end,
+  // the counter's round trips delay no load.
+  if (tid == 0) {
+    const unsigned long long e = *launch_epoch;
+    if (ticket_arrive(p.epoch_word + 1, e, static_cast<int>(gridDim.x))) {
+      p.epoch_word[0] = e % kEpochMax + 1ull;
+      p.epoch_word[1] = 0ull;
     }
-    __syncthreads();
   }
 }
 
 template <typename T, typename OutT, int D, int NT, bool MULTI>
-cudaError_t launch_fp4_typed(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int grid, cudaStream_t stream) {
+cudaError_t launch_fp4_typed(const Fp4DecodeParams& p, int grid, cudaStream_t stream) {
   using G = Fp4Geo<D, NT>;
   auto kern = decode_fp4_kernel<T, OutT, D, NT, MULTI>;
   static unsigned long long configured = 0;
@@ -824,30 +949,30 @@ cudaError_t launch_fp4_typed(const Fp4TensorMaps& m, const Fp4DecodeParams& p, i
   attr[0].val.programmaticStreamSerializationAllowed = p.pdl ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, m.k, m.v, m.k_block, m.v_block, p);
+  return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
 template <typename T, typename OutT>
-cudaError_t launch_fp4(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid,
+cudaError_t launch_fp4(const Fp4DecodeParams& p, int head_dim, int grid,
                        cudaStream_t stream) {
   const bool multi = p.seqlen_q > 1 || p.causal;
   const bool two = p.rows == 16;
   switch (head_dim) {
     case 64:
       if (two)
-        return multi ? launch_fp4_typed<T, OutT, 64, 2, true>(m, p, grid, stream)
-                     : launch_fp4_typed<T, OutT, 64, 2, false>(m, p, grid, stream);
-      return multi ? launch_fp4_typed<T, OutT, 64, 1, true>(m, p, grid, stream)
-                   : launch_fp4_typed<T, OutT, 64, 1, false>(m, p, grid, stream);
+        return multi ? launch_fp4_typed<T, OutT, 64, 2, true>(p, grid, stream)
+                     : launch_fp4_typed<T, OutT, 64, 2, false>(p, grid, stream);
+      return multi ? launch_fp4_typed<T, OutT, 64, 1, true>(p, grid, stream)
+                   : launch_fp4_typed<T, OutT, 64, 1, false>(p, grid, stream);
     case 128:
       if (two)
-        return multi ? launch_fp4_typed<T, OutT, 128, 2, true>(m, p, grid, stream)
-                     : launch_fp4_typed<T, OutT, 128, 2, false>(m, p, grid, stream);
-      return multi ? launch_fp4_typed<T, OutT, 128, 1, true>(m, p, grid, stream)
-                   : launch_fp4_typed<T, OutT, 128, 1, false>(m, p, grid, stream);
+        return multi ? launch_fp4_typed<T, OutT, 128, 2, true>(p, grid, stream)
+                     : launch_fp4_typed<T, OutT, 128, 2, false>(p, grid, stream);
+      return multi ? launch_fp4_typed<T, OutT, 128, 1, true>(p, grid, stream)
+                   : launch_fp4_typed<T, OutT, 128, 1, false>(p, grid, stream);
     default:
-      return multi ? launch_fp4_typed<T, OutT, 256, 1, true>(m, p, grid, stream)
-                   : launch_fp4_typed<T, OutT, 256, 1, false>(m, p, grid, stream);
+      return multi ? launch_fp4_typed<T, OutT, 256, 1, true>(p, grid, stream)
+                   : launch_fp4_typed<T, OutT, 256, 1, false>(p, grid, stream);
   }
 }
 

@@ -3,9 +3,8 @@
 
 namespace fd {
 
-cudaError_t launch_fp4_bf16(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid,
-                          cudaStream_t stream) {
-  return launch_fp4<__nv_bfloat16, __nv_bfloat16>(m, p, head_dim, grid, stream);
+cudaError_t launch_fp4_bf16(const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream) {
+  return launch_fp4<__nv_bfloat16, __nv_bfloat16>(p, head_dim, grid, stream);
 }
 
 }  // namespace fd

@@ -3,9 +3,8 @@
 
 namespace fd {
 
-cudaError_t launch_fp4_fp16(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid,
-                          cudaStream_t stream) {
-  return launch_fp4<__half, __half>(m, p, head_dim, grid, stream);
+cudaError_t launch_fp4_fp16(const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream) {
+  return launch_fp4<__half, __half>(p, head_dim, grid, stream);
 }
 
 }  // namespace fd

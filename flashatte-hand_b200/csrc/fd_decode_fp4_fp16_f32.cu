@@ -3,9 +3,8 @@
 
 namespace fd {
 
-cudaError_t launch_fp4_fp16_f32(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid,
-                          cudaStream_t stream) {
-  return launch_fp4<__half, float>(m, p, head_dim, grid, stream);
+cudaError_t launch_fp4_fp16_f32(const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream) {
+  return launch_fp4<__half, float>(p, head_dim, grid, stream);
 }
 
 }  // namespace fd

@@ -149,6 +149,10 @@ cudaError_t launch_release_pages(const ReleasePagesParams& p, cudaStream_t strea
 // Decode over a 4-bit block-scaled cache (fd_decode_fp4.cuh).
 struct Fp4DecodeParams {
   const void* q;                 // [B, seqlen_q, Hq, D]
+  const uint8_t* k_cache;        // [num_blocks, page, Hkv, D / 2] codes
+  const uint8_t* v_cache;
+  const uint8_t* k_block;        // [num_blocks, Hkv, page, D / 16] e4m3 block scales
+  const uint8_t* v_block;
   void* out;                     // [B, seqlen_q, Hq, D]
   float* lse;                    // [B, Hq, seqlen_q], nullable
   const float* k_scale;          // [Hkv]
@@ -156,33 +160,30 @@ struct Fp4DecodeParams {
   const int32_t* seqlens;
   const int32_t* block_table;
   int64_t bt_stride, num_blocks;
-  int batch, num_heads, num_heads_k, group, page, chunk;
+  int batch, num_heads, num_heads_k, group, page;
   int seqlen_q, causal, qrows;   // qrows = seqlen_q * group
   int row_tiles, rows;           // query rows are taken `rows` at a time, in row_tiles passes
+  int heads;                     // KV heads that a CTA takes together: 4, 2 or 1
   int len_add;
   float scale_log2;
   float* part_o;                 // [slots, rows, D] normalised partial O
   float* part_lse;               // [slots, rows] log2-domain partial LSE
-  unsigned long long* tickets;   // arrival counters, as DecodeParams::tickets
+  unsigned long long* tickets;   // arrival counters of (pair, head), as DecodeParams::tickets
   unsigned long long* epoch_word;
   int* err;
-  unsigned long long timeout_ns;
   int cost_tile, cost_seg, cost_floor;
   int pdl;
-};
-struct Fp4TensorMaps {
-  CUtensorMap k, v, k_block, v_block;
 };
 // Query rows of one pass for this head dim (8 or 16).
 int fp4_rows(int head_dim, int64_t qrows);
 // Most CTAs a launch uses on a device of `sms` SMs.
 int fp4_max_grid(int head_dim, int rows, int sms);
-cudaError_t launch_fp4_bf16(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream);
-cudaError_t launch_fp4_bf16_f32(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream);
-cudaError_t launch_fp4_fp16(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream);
-cudaError_t launch_fp4_fp16_f32(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream);
-cudaError_t launch_decode_fp4(const Fp4TensorMaps& m, const Fp4DecodeParams& p, int head_dim,
-                              int q_dtype, bool out_fp32, int grid, cudaStream_t stream);
+cudaError_t launch_fp4_bf16(const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream);
+cudaError_t launch_fp4_bf16_f32(const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream);
+cudaError_t launch_fp4_fp16(const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream);
+cudaError_t launch_fp4_fp16_f32(const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream);
+cudaError_t launch_decode_fp4(const Fp4DecodeParams& p, int head_dim, int q_dtype, bool out_fp32,
+                              int grid, cudaStream_t stream);
 
 // Workspace carve-up for the tensor-core kernel: [epoch_off, lse_off) must
 // be zero before the workspace's first use (the kernel keeps it consistent
@@ -258,18 +259,12 @@ bool uses_tensor_core_path(const void* q, const void* k_cache, const void* v_cac
 
 // What the entry points outside fd_api.cu share with it.
 int device_sms(int dev);
-unsigned long long wait_timeout_ns();
 bool pdl_enabled();
 int env_int(const char* name, int dflt, int lo, int hi);
 // Library-owned workspace of (current device `dev`, `stream`); nullptr and *why on failure.
 void* library_workspace(int dev, size_t bytes, cudaStream_t stream, const char** why);
 // Sequences a launch of `grid` CTAs may take (see fd_api.cu); 0: not even one fits.
 int64_t seqs_per_launch(int64_t per_seq_cost, int64_t aligned_cost, int64_t hkv, int grid);
-// cuTensorMapEncodeTiled with interleave and out-of-bounds fill none.
-bool tensor_maps_available();
-CUresult encode_tensor_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* base,
-                           const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
-                           CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion);
 int report_ok();
 
 // Record `code` and a printf-style message as this thread's last error (what
