@@ -68,8 +68,9 @@ int check_cache(const void* k_cache, const void* v_cache, const void* k_block, c
 
 fd::SlotParams slot_params(void* k_cache, void* v_cache, void* k_block, void* v_block,
                            const float* k_scale, const float* v_scale, int64_t num_heads_k,
-                           int64_t headdim, int64_t page, int64_t num_blocks, int* status) {
+                           int64_t headdim, int64_t page, int64_t num_blocks, int dev, int* status) {
   fd::SlotParams p{};
+  p.sms = fd::device_sms(dev);
   p.k_cache = k_cache;
   p.v_cache = v_cache;
   p.k_block = static_cast<uint8_t*>(k_block);
@@ -127,7 +128,7 @@ int fd_append_kv_slots(const void* k_new, int64_t k_token_stride, const void* v_
   st = current_device(&dev, &status);
   if (st != FD_OK) return st;
   fd::SlotParams p = slot_params(k_cache, v_cache, k_block_scale, v_block_scale, k_scale, v_scale,
-                                 num_heads_k, headdim, page_block_size, num_blocks, status);
+                                 num_heads_k, headdim, page_block_size, num_blocks, dev, status);
   p.k = k_new;
   p.v = v_new;
   p.k_stride = k_token_stride;
@@ -164,7 +165,7 @@ int fd_gather_kv_slots(const void* k_cache, const void* v_cache, const void* k_b
   fd::SlotParams p = slot_params(const_cast<void*>(k_cache), const_cast<void*>(v_cache),
                                  const_cast<void*>(k_block_scale), const_cast<void*>(v_block_scale),
                                  k_scale, v_scale, num_heads_k, headdim, page_block_size, num_blocks,
-                                 status);
+                                 dev, status);
   p.k_out = k_out;
   p.v_out = v_out;
   p.slot_map = slot_map;
@@ -197,7 +198,7 @@ int fd_append_kv_paged_fp4(const void* k_new, const void* v_new, void* k_cache, 
   st = current_device(&dev, &status);
   if (st != FD_OK) return st;
   fd::SlotParams p = slot_params(k_cache, v_cache, k_block_scale, v_block_scale, k_scale, v_scale,
-                                 num_heads_k, headdim, page_block_size, num_blocks, status);
+                                 num_heads_k, headdim, page_block_size, num_blocks, dev, status);
   p.k = k_new;
   p.v = v_new;
   p.k_stride = p.v_stride = num_heads_k * headdim;
@@ -270,6 +271,8 @@ int fd_release_pages(int32_t* block_table, int64_t block_table_stride,
   int* status = nullptr;
   const int st = current_device(&dev, &status);
   if (st != FD_OK) return st;
+  const int sms = fd::device_sms(dev);
+  if (sms <= 0) return report_error(FD_ERR_CUDA, "cannot query SM count");
   fd::ReleasePagesParams p;
   p.block_table = block_table;
   p.seqlens = cache_seqlens;
@@ -281,7 +284,7 @@ int fd_release_pages(int32_t* block_table, int64_t block_table_stride,
   p.batch = static_cast<int>(batch_size);
   p.page = static_cast<int>(page_block_size);
   p.err = status;
-  const cudaError_t e = fd::launch_release_pages(p, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = fd::launch_release_pages(p, sms, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return report_error(FD_ERR_CUDA, "release launch: %s", cudaGetErrorString(e));
   return fd::report_ok();
 }

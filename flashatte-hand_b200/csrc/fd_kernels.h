@@ -110,7 +110,8 @@ struct SlotParams {
   const int32_t* seqlens; const int32_t* block_table;
   int64_t bt_stride, num_blocks, rows;
   int seqlen_new, num_heads_k, head_dim, page;
-  int rows_per_cta;                      // set by the launcher
+  int rows_at, rows_per_cta;             // set by the launcher
+  int sms;                               // SMs of the device
   int* err;
 };
 cudaError_t launch_append_slots(const SlotParams& p, int src_dtype, int cache_dtype, cudaStream_t stream);
@@ -144,7 +145,7 @@ struct ReleasePagesParams {
   int* err;
 };
 cudaError_t launch_assign_pages(const AssignPagesParams& p, int sms, cudaStream_t stream);
-cudaError_t launch_release_pages(const ReleasePagesParams& p, cudaStream_t stream);
+cudaError_t launch_release_pages(const ReleasePagesParams& p, int sms, cudaStream_t stream);
 
 // Decode over a 4-bit block-scaled cache (fd_decode_fp4.cuh).
 struct Fp4DecodeParams {

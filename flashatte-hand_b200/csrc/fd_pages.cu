@@ -175,39 +175,79 @@ __global__ void __launch_bounds__(kPagesThreads) assign_pages_kernel(const Assig
     const int b = find_owner(pre, B, static_cast<int>(k));
     p.block_table[b * p.bt_stride + pages_of(len[b], page) + (k - pre[b])] = fresh_page(static_cast<int>(k));
   }
+  // Slots, four consecutive tokens a thread: one search, then steps along the
+  // page, the pages and the requests.
   const int total = tok[B];
-  for (int64_t t = first; t < p.num_slots; t += stride_all) {
-    int64_t slot = -1;
-    if (t < total) {
-      const int b = find_owner(tok, B, static_cast<int>(t));
-      const int L = len[b];
-      if (L >= 0) {
-        const uint32_t pos = static_cast<uint32_t>(L) + static_cast<uint32_t>(t - tok[b]);
-        const int j = static_cast<int>(pos / static_cast<uint32_t>(page));
-        const int have = pages_of(L, page);
-        int id;
-        if (j < have) {
-          id = p.block_table[b * p.bt_stride + j];
-          if (id < 0 || id >= p.num_blocks) {
-            report_status(p.err, kStatusBadPage);
-            id = -1;
-          }
-        } else {
-          id = fresh_page(pre[b] + j - have);
+  const bool wide = (reinterpret_cast<uintptr_t>(p.slot_map) & 15u) == 0;
+  for (int64_t t0 = static_cast<int64_t>(first) * 4; t0 < p.num_slots; t0 += static_cast<int64_t>(stride_all) * 4) {
+    long long slot[4] = {-1, -1, -1, -1};
+    if (t0 < total) {
+      int b = find_owner(tok, B, static_cast<int>(t0));
+      int end = 0, row = 0, j = 0, have = 0;  // the request's last token + 1; the token's row of page column j
+      int64_t base = -1;                      // slot of the page's row 0
+      bool enter = true;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = static_cast<int>(t0) + i;
+        if (t >= total) break;
+        if (!enter && t >= end) {
+          do ++b; while (t >= tok[b + 1]);
+          enter = true;
         }
-        if (id >= 0)
-          slot = static_cast<int64_t>(id) * page + (pos - static_cast<uint32_t>(j) * static_cast<uint32_t>(page));
+        const int L = len[b];
+        bool fetch = false;
+        if (enter) {
+          end = tok[b + 1];
+          if (L >= 0) {
+            const uint32_t pos = static_cast<uint32_t>(L) + static_cast<uint32_t>(t - tok[b]);
+            j = static_cast<int>(pos / static_cast<uint32_t>(page));
+            row = static_cast<int>(pos - static_cast<uint32_t>(j) * static_cast<uint32_t>(page));
+            have = pages_of(L, page);
+            fetch = true;
+          }
+          enter = false;
+        } else if (++row == page) {
+          row = 0;
+          ++j;
+          fetch = true;
+        }
+        if (L < 0) continue;
+        if (fetch) {
+          int id;
+          if (j < have) {
+            id = p.block_table[b * p.bt_stride + j];
+            if (id < 0 || id >= p.num_blocks) {
+              report_status(p.err, kStatusBadPage);
+              id = -1;
+            }
+          } else {
+            id = fresh_page(pre[b] + j - have);
+          }
+          base = id < 0 ? -1 : static_cast<int64_t>(id) * page;
+        }
+        if (base >= 0) slot[i] = base + row;
       }
     }
-    p.slot_map[t] = slot;
+    if (wide && t0 + 4 <= p.num_slots) {
+      longlong2* d = reinterpret_cast<longlong2*>(p.slot_map + t0);
+      d[0] = make_longlong2(slot[0], slot[1]);
+      d[1] = make_longlong2(slot[2], slot[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t0 + i < p.num_slots) p.slot_map[t0 + i] = slot[i];
+    }
   }
 }
 
 // Pages beyond ceil(keep_b / P) of each request go back to the stack.  They
 // are pushed in reverse order (last request first, last page first), so that
-// giving back what one assign took leaves the stack as it was.  One CTA: the
-// pushes are dense (an entry outside the pool is dropped and reported), which
-// makes every position depend on all entries before it.
+// giving back what one assign took leaves the stack as it was.  With f the
+// number of a page among the R given back, its place is count + R - 1 - f:
+// the CTAs work apart, and the last to finish writes the count.  An entry
+// outside the pool leaves a hole there, which that CTA closes.  Only if the
+// stack has no room for all (a page released twice) does one CTA push them in
+// order, since then each one's place depends on all before it.
 __global__ void __launch_bounds__(kReleaseThreads) release_pages_kernel(const ReleasePagesParams p) {
   extern __shared__ int pages_smem[];
   __shared__ longlong2 sums[kReleaseThreads / 32];
@@ -245,6 +285,53 @@ __global__ void __launch_bounds__(kReleaseThreads) release_pages_kernel(const Re
   if (tid == 0) pre[B] = clamp_i32(total);
   __syncthreads();
   const int R = pre[B];
+  if (static_cast<int64_t>(count) + R <= p.num_blocks) {
+    int bad = 0;
+    const int stride_all = static_cast<int>(gridDim.x) * kReleaseThreads;
+    for (int64_t f = static_cast<int64_t>(blockIdx.x) * kReleaseThreads + tid; f < R; f += stride_all) {
+      const int b = find_owner(pre, B, static_cast<int>(f));
+      int32_t* e = p.block_table + b * p.bt_stride + from[b] + (f - pre[b]);
+      int id = *e;
+      *e = -1;
+      if (id < 0 || id >= p.num_blocks) {
+        report_status(p.err, kStatusBadPage);
+        id = -1;
+        bad = 1;
+      }
+      p.free_pages[count + R - 1 - f] = id;
+    }
+    bad = __syncthreads_or(bad);
+    __shared__ int arrivals;
+    if (tid == 0) {
+      // CTAs done in the low half, those that met a bad entry in the high
+      __threadfence();
+      const int add = 1 + (bad ? 1 << 16 : 0);
+      arrivals = gridDim.x > 1 ? atomicAdd(p.free_count + 1, add) + add : add;
+      __threadfence();
+    }
+    __syncthreads();
+    if ((arrivals & 0xFFFF) != static_cast<int>(gridDim.x)) return;
+    int good_all = R;
+    if (arrivals >> 16) {  // close the holes, in order
+      good_all = 0;
+      for (int64_t base = 0; base < R; base += kReleaseThreads) {
+        const int64_t i = base + tid;
+        const int id = i < R ? __ldcg(p.free_pages + count + i) : -1;
+        int64_t good = id >= 0 ? 1 : 0, none = 0, all, all_none;
+        const int64_t mine_good = good;
+        block_scan2<kReleaseThreads>(good, none, all, all_none, sums);
+        // every entry of this round has been read, and places only move down
+        if (id >= 0) p.free_pages[count + good_all + good - mine_good] = id;
+        good_all += static_cast<int>(all);
+      }
+    }
+    if (tid == 0) {
+      p.free_count[0] = count + good_all;
+      p.free_count[1] = 0;
+    }
+    return;
+  }
+  if (blockIdx.x != 0) return;
   int64_t pushed = 0;
   for (int64_t base = 0; base < R; base += kReleaseThreads * kReleaseBatch) {
     // entry u of the thread: number base + tid * batch + u from the end
@@ -306,11 +393,14 @@ cudaError_t launch_assign_pages(const AssignPagesParams& p, int sms, cudaStream_
   return cudaGetLastError();
 }
 
-cudaError_t launch_release_pages(const ReleasePagesParams& p, cudaStream_t stream) {
+cudaError_t launch_release_pages(const ReleasePagesParams& p, int sms, cudaStream_t stream) {
   const size_t smem = (2 * static_cast<size_t>(p.batch) + 1) * sizeof(int);
   cudaError_t e = allow_smem(release_pages_kernel, smem);
   if (e != cudaSuccess) return e;
-  release_pages_kernel<<<1, kReleaseThreads, smem, stream>>>(p);
+  // a CTA for every 8 pages of a thread that the table could hold
+  const int64_t most = (p.batch * p.bt_stride + 8 * kReleaseThreads - 1) / (8 * kReleaseThreads);
+  const unsigned grid = static_cast<unsigned>(most < sms ? most : sms);
+  release_pages_kernel<<<grid, kReleaseThreads, smem, stream>>>(p);
   return cudaGetLastError();
 }
 

@@ -48,7 +48,10 @@ __device__ __forceinline__ Place place_of_slot(int64_t slot, int page, int64_t n
   Place at{-1, 0};
   if (slot < 0) return at;
   int64_t pg;
-  if (slot <= static_cast<int64_t>(UINT32_MAX)) {  // a 64-bit division is a long sequence
+  if ((page & (page - 1)) == 0) {
+    pg = slot >> (31 - __clz(page));
+    at.row = static_cast<int>(slot) & (page - 1);
+  } else if (slot <= static_cast<int64_t>(UINT32_MAX)) {  // a 64-bit division is a long sequence
     const uint32_t s = static_cast<uint32_t>(slot), q = s / static_cast<uint32_t>(page);
     pg = q;
     at.row = static_cast<int>(s - q * static_cast<uint32_t>(page));
@@ -78,61 +81,58 @@ __device__ __forceinline__ Place place_of_row(const SlotParams& p, int64_t r, bo
   return at;
 }
 
-// x / d for |d| normal and away from the ends of the range, correctly
-// rounded: one Newton correction of x * (1 / d) with the exact remainder
-// (Markstein's theorem: a correctly rounded reciprocal makes it exact).
-// Rounding to e2m1 then sees the tie cases exactly, which a plain product
-// with the reciprocal would miss.
-struct Divider {
-  float d, r;
-  bool plain;
-  __device__ __forceinline__ explicit Divider(float divisor) : d(divisor) {
-    const float a = fabsf(divisor);
-    plain = !(a > 1e-25f && a < 1e25f);
-    r = __frcp_rn(divisor);
-  }
-  __device__ __forceinline__ float operator()(float x) const {
-    if (plain) return x / d;
-    const float q = x * r;
-    // infinite quotients have no remainder (and saturate anyway)
-    return fabsf(q) < 1e30f ? fmaf(fmaf(-q, d, x), r, q) : q;
-  }
-};
+// x / d, correctly rounded, for r = 1 / d correctly rounded and nothing near
+// the ends of the range: one Newton correction of x r with the exact
+// remainder (Markstein's theorem).  Rounding to e2m1 then sees the tie cases
+// exactly, which a plain product with the reciprocal would miss.
+__device__ __forceinline__ float divide(float x, float d, float r) {
+  const float q = x * r;
+  return fmaf(fmaf(-q, d, x), r, q);
+}
 
 __device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
   return static_cast<uint32_t>(
       __nv_cvt_float2_to_fp4x2(make_float2(lo, hi), __NV_E2M1, cudaRoundNearest));
 }
 
-// max that keeps a NaN, so that a NaN among the values becomes the block's scale
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float m;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
-  return m;
-}
-
 // One block of 16 values to 8 bytes of codes and a scale byte.  A block with
 // a NaN gets a NaN scale and zero codes: all of it reads back as NaN.
 template <typename T>
 __device__ __forceinline__ uint2 quantize_block(const uint32_t (&w)[8], float head_scale, uint8_t& scale) {
-  float x[16];
-  float amax = 0.f;
+  // The largest magnitude: 16-bit floats without their sign order as whole
+  // numbers, NaN above infinity above all else.
+  uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 f = to_float2<T>(w[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-    amax = max_nan(amax, max_nan(fabsf(f.x), fabsf(f.y)));
-  }
+  for (int i = 0; i < 8; ++i) top = __vmaxu2(top, w[i] & 0x7FFF7FFFu);
+  top = top > (top << 16) ? top & 0xFFFF0000u : top << 16;
+  const float amax = to_float2<T>(top).y;
   const uint32_t s8 = static_cast<uint32_t>(
       __nv_cvt_float_to_fp8(__fdiv_rn(amax, 6.f * head_scale), __NV_SATFINITE, __NV_E4M3));
   scale = static_cast<uint8_t>(s8);
   const float s = e4m3_to_float(s8);
   if (!(s > 0.f)) return make_uint2(0u, 0u);
-  const Divider div(s * head_scale);
+  const float d = s * head_scale;
   uint32_t c[2] = {0u, 0u};
+  // the quotients are at most amax / d: with both well inside the range (and
+  // no infinity among the values) no step of divide() leaves it
+  if (amax < 1e30f && d > 1e-25f && d < 1e25f && amax < d * 1e25f) {
+    const float r = __frcp_rn(d);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i >> 2] |= e2m1x2(div(x[2 * i]), div(x[2 * i + 1])) << (8 * (i & 3));
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = to_float2<T>(w[i]);
+      c[i >> 2] |= e2m1x2(divide(f.x, d, r), divide(f.y, d, r)) << (8 * (i & 3));
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      uint32_t x = w[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) x = i == j ? w[j] : x;
+      const float2 f = to_float2<T>(x);
+      const uint32_t byte = e2m1x2(f.x / d, f.y / d) << (8 * (i & 3));
+      if (i < 4) c[0] |= byte; else c[1] |= byte;
+    }
+  }
   return make_uint2(c[0], c[1]);
 }
 
@@ -149,45 +149,62 @@ __device__ __forceinline__ uint4 quantize_e4m3(const uint32_t (&w)[8], float sca
 
 enum CacheKind { kNative = 0, kE4m3 = 1, kFp4 = 2 };
 
-// A CTA covers rows_per_cta rows; a row is num_heads_k * head_dim / 16 units.
+// A row is `units` = num_heads_k * head_dim / 16 units of 16 values.  A CTA
+// covers rows_per_cta rows, rows_at of them side by side (one row in several
+// rounds if it has more units than the CTA threads), so that what depends on
+// the unit alone is computed once a thread.
+template <typename F>
+__device__ __forceinline__ void for_units(const SlotParams& p, F&& body) {
+  const int units = p.num_heads_k * (p.head_dim / 16);
+  const int dr = units < kSlotThreads ? threadIdx.x / units : 0;
+  if (dr >= p.rows_at) return;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.rows_per_cta;
+  const int64_t r1 = r0 + p.rows_per_cta < p.rows ? r0 + p.rows_per_cta : p.rows;
+  for (int u = threadIdx.x - dr * units; u < units; u += kSlotThreads)
+    body(u, units, r0 + dr, r1);
+}
+
 template <typename T, int KIND>
 __global__ void __launch_bounds__(kSlotThreads) append_slots_kernel(const SlotParams p) {
-  const int units = p.num_heads_k * (p.head_dim / 16), per_head = p.head_dim / 16;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.rows_per_cta;
-  for (int i = threadIdx.x; i < p.rows_per_cta * units; i += kSlotThreads) {
-    const int dr = i / units, u = i - dr * units;
-    const int64_t r = r0 + dr;
-    if (r >= p.rows) return;
-    const Place at = place_of_row(p, r, u == 0);
-    if (at.page < 0) continue;
-    const uint4* ks = reinterpret_cast<const uint4*>(static_cast<const T*>(p.k) + r * p.k_stride + u * 16);
-    const uint4* vs = reinterpret_cast<const uint4*>(static_cast<const T*>(p.v) + r * p.v_stride + u * 16);
-    const uint4 k0 = __ldg(ks), k1 = __ldg(ks + 1), v0 = __ldg(vs), v1 = __ldg(vs + 1);
-    const int64_t dst = (at.page * p.page + at.row) * units + u;  // unit of the cache
-    if constexpr (KIND == kNative) {
-      uint4* kd = static_cast<uint4*>(p.k_cache) + dst * 2;
-      uint4* vd = static_cast<uint4*>(p.v_cache) + dst * 2;
-      kd[0] = k0; kd[1] = k1;
-      vd[0] = v0; vd[1] = v1;
-    } else {
-      const int h = u / per_head;
-      uint32_t kw[8], vw[8];
-      unpack(k0, k1, kw);
-      unpack(v0, v1, vw);
-      const float kg = __ldg(p.k_scale + h), vg = __ldg(p.v_scale + h);
-      if constexpr (KIND == kE4m3) {
-        static_cast<uint4*>(p.k_cache)[dst] = quantize_e4m3<T>(kw, kg);
-        static_cast<uint4*>(p.v_cache)[dst] = quantize_e4m3<T>(vw, vg);
+  for_units(p, [&](int u, int units, int64_t r0, int64_t r1) {
+    const int per_head = p.head_dim / 16, h = u / per_head;
+    const T* kr = static_cast<const T*>(p.k) + u * 16;
+    const T* vr = static_cast<const T*>(p.v) + u * 16;
+    float kg = 1.f, vg = 1.f;
+    if constexpr (KIND != kNative) {
+      kg = __ldg(p.k_scale + h);
+      vg = __ldg(p.v_scale + h);
+    }
+    for (int64_t r = r0; r < r1; r += p.rows_at) {
+      const uint4* ks = reinterpret_cast<const uint4*>(kr + r * p.k_stride);
+      const uint4* vs = reinterpret_cast<const uint4*>(vr + r * p.v_stride);
+      const uint4 k0 = __ldcs(ks), k1 = __ldcs(ks + 1), v0 = __ldcs(vs), v1 = __ldcs(vs + 1);
+      const Place at = place_of_row(p, r, u == 0);
+      if (at.page < 0) continue;
+      const int64_t dst = (at.page * p.page + at.row) * units + u;  // unit of the cache
+      if constexpr (KIND == kNative) {
+        uint4* kd = static_cast<uint4*>(p.k_cache) + dst * 2;
+        uint4* vd = static_cast<uint4*>(p.v_cache) + dst * 2;
+        kd[0] = k0; kd[1] = k1;
+        vd[0] = v0; vd[1] = v1;
       } else {
-        const int64_t sd = ((at.page * p.num_heads_k + h) * p.page + at.row) * per_head + (u - h * per_head);
-        uint8_t s;
-        static_cast<uint2*>(p.k_cache)[dst] = quantize_block<T>(kw, kg, s);
-        p.k_block[sd] = s;
-        static_cast<uint2*>(p.v_cache)[dst] = quantize_block<T>(vw, vg, s);
-        p.v_block[sd] = s;
+        uint32_t kw[8], vw[8];
+        unpack(k0, k1, kw);
+        unpack(v0, v1, vw);
+        if constexpr (KIND == kE4m3) {
+          static_cast<uint4*>(p.k_cache)[dst] = quantize_e4m3<T>(kw, kg);
+          static_cast<uint4*>(p.v_cache)[dst] = quantize_e4m3<T>(vw, vg);
+        } else {
+          const int64_t sd = ((at.page * p.num_heads_k + h) * p.page + at.row) * per_head + (u - h * per_head);
+          uint8_t s;
+          static_cast<uint2*>(p.k_cache)[dst] = quantize_block<T>(kw, kg, s);
+          p.k_block[sd] = s;
+          static_cast<uint2*>(p.v_cache)[dst] = quantize_block<T>(vw, vg, s);
+          p.v_block[sd] = s;
+        }
       }
     }
-  }
+  });
 }
 
 // 16-bit rows that are not 16-byte aligned or not a multiple of 16 values.
@@ -280,42 +297,42 @@ __device__ __forceinline__ void load16(const void* cache, int64_t src, float sca
 
 template <typename C, typename O, int KIND>
 __global__ void __launch_bounds__(kSlotThreads) gather_slots_kernel(const SlotParams p) {
-  const int units = p.num_heads_k * (p.head_dim / 16), per_head = p.head_dim / 16;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.rows_per_cta;
-  for (int i = threadIdx.x; i < p.rows_per_cta * units; i += kSlotThreads) {
-    const int dr = i / units, u = i - dr * units;
-    const int64_t r = r0 + dr;
-    if (r >= p.rows) return;
-    const Place at = place_of_slot(p.slot_map[r], p.page, p.num_blocks, p.err, u == 0);
-    float k[16], v[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) k[j] = v[j] = 0.f;
-    if (at.page >= 0) {
-      const int64_t src = (at.page * p.page + at.row) * units + u;
-      const int h = u / per_head;
-      float kg = 1.f, vg = 1.f, kb = 1.f, vb = 1.f;
-      if constexpr (KIND != kNative) {
-        kg = __ldg(p.k_scale + h);
-        vg = __ldg(p.v_scale + h);
-      }
-      if constexpr (KIND == kFp4) {
-        const int64_t sd = ((at.page * p.num_heads_k + h) * p.page + at.row) * per_head + (u - h * per_head);
-        kb = e4m3_to_float(__ldg(p.k_block + sd));
-        vb = e4m3_to_float(__ldg(p.v_block + sd));
-      }
-      load16<C, KIND>(p.k_cache, src, kg, kb, k);
-      load16<C, KIND>(p.v_cache, src, vg, vb, v);
+  for_units(p, [&](int u, int units, int64_t r0, int64_t r1) {
+    const int per_head = p.head_dim / 16, h = u / per_head;
+    float kg = 1.f, vg = 1.f;
+    if constexpr (KIND != kNative) {
+      kg = __ldg(p.k_scale + h);
+      vg = __ldg(p.v_scale + h);
     }
-    store16<O>(p.k_out, r * units + u, k);
-    store16<O>(p.v_out, r * units + u, v);
-  }
+    for (int64_t r = r0; r < r1; r += p.rows_at) {
+      const Place at = place_of_slot(p.slot_map[r], p.page, p.num_blocks, p.err, u == 0);
+      float k[16], v[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) k[j] = v[j] = 0.f;
+      if (at.page >= 0) {
+        const int64_t src = (at.page * p.page + at.row) * units + u;
+        float kb = 1.f, vb = 1.f;
+        if constexpr (KIND == kFp4) {
+          const int64_t sd = ((at.page * p.num_heads_k + h) * p.page + at.row) * per_head + (u - h * per_head);
+          kb = e4m3_to_float(__ldg(p.k_block + sd));
+          vb = e4m3_to_float(__ldg(p.v_block + sd));
+        }
+        load16<C, KIND>(p.k_cache, src, kg, kb, k);
+        load16<C, KIND>(p.v_cache, src, vg, vb, v);
+      }
+      store16<O>(p.k_out, r * units + u, k);
+      store16<O>(p.v_out, r * units + u, v);
+    }
+  });
 }
 
-// Rows per CTA and the grid that covers `rows` of them: about two units a thread.
+// Rows side by side in a CTA, rows per CTA (up to 8 rounds, while the grid
+// still covers the device several times) and the grid.
 unsigned slot_grid(SlotParams& p) {
   const int units = p.num_heads_k * (p.head_dim / 16);
-  int n = units > 0 ? 2 * kSlotThreads / units : 1;
-  p.rows_per_cta = n < 1 ? 1 : n;
+  p.rows_at = units < kSlotThreads ? kSlotThreads / units : 1;
+  const int64_t rounds = p.rows / (static_cast<int64_t>(p.rows_at) * p.sms * 16);
+  p.rows_per_cta = p.rows_at * static_cast<int>(rounds < 1 ? 1 : (rounds < 8 ? rounds : 8));
   return static_cast<unsigned>((p.rows + p.rows_per_cta - 1) / p.rows_per_cta);
 }
 

@@ -46,11 +46,15 @@ def _stream_handle(stream, dev: torch.device) -> int:
     return torch.cuda.current_stream(idx).cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_NO_SWITCH = contextlib.nullcontext()
+
+
 def _on_device(dev: torch.device):
     """Context that makes `dev` current, or nothing when it already is (the
     device switch costs more than the rest of a small call)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if dev.index is None or dev.index == _current_device():
+        return _NO_SWITCH
     return torch.cuda.device(dev)
 
 
@@ -463,23 +467,23 @@ def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_map: torch.Tens
     return outs[0], outs[1]
 
 
-def _check_pool(block_table, lens: dict, free_pages, free_count) -> int:
+def _check_int32(name: str, t: torch.Tensor, shape) -> None:
+    if not t.is_cuda:
+        raise ValueError("flashdecode runs on CUDA tensors only (no CPU path)")
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}")
+
+
+def _check_pool(block_table, free_pages, free_count) -> int:
     """Checks that assign_pages and release_pages share; returns B."""
     if block_table.dim() != 2:
         raise ValueError("block_table must be [B, max_blocks]")
-    B = block_table.shape[0]
-    tensors = {"block_table": block_table, "free_pages": free_pages, "free_count": free_count, **lens}
-    for name, t in tensors.items():
-        if not t.is_cuda:
-            raise ValueError("flashdecode runs on CUDA tensors only (no CPU path)")
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 tensor")
-    for name, t in lens.items():
-        if t.shape != (B,):
-            raise ValueError(f"{name} must be [B] = [{B}]")
-    if free_pages.dim() != 1 or free_count.shape != (2,):
-        raise ValueError("free_pages must be [num_blocks] and free_count [2]")
-    return B
+    if free_pages.dim() != 1:
+        raise ValueError("free_pages must be [num_blocks]")
+    _check_int32("block_table", block_table, block_table.shape)
+    _check_int32("free_pages", free_pages, free_pages.shape)
+    _check_int32("free_count", free_count, (2,))
+    return block_table.shape[0]
 
 
 def assign_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, new_lens: torch.Tensor,
@@ -505,8 +509,9 @@ def assign_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, new_len
     reports FD_ERR_NO_PAGES; requests are served in order.
     """
     lib = load_library()
-    B = _check_pool(block_table, {"cache_seqlens": cache_seqlens, "new_lens": new_lens}, free_pages,
-                    free_count)
+    B = _check_pool(block_table, free_pages, free_count)
+    _check_int32("cache_seqlens", cache_seqlens, (B,))
+    _check_int32("new_lens", new_lens, (B,))
     dev = block_table.device
     if slot_map is None:
         if num_slots is None:
@@ -517,16 +522,18 @@ def assign_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, new_len
         raise ValueError("slot_map must be a contiguous int64 [num_slots] CUDA tensor")
     if cu_new_lens is None:
         cu_new_lens = torch.empty((B + 1,), dtype=torch.int32, device=dev)
+    else:
+        _check_int32("cu_new_lens", cu_new_lens, (B + 1,))
     if seqlens_out is None:
         seqlens_out = torch.empty((B,), dtype=torch.int32, device=dev)
-    for name, t, n in (("cu_new_lens", cu_new_lens, B + 1), ("seqlens_out", seqlens_out, B)):
-        if not t.is_cuda or t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 [{n}] CUDA tensor")
+    else:
+        _check_int32("seqlens_out", seqlens_out, (B,))
     with _on_device(dev):
         check(lib.fd_assign_pages(
-            _ptr(block_table), block_table.shape[1], _ptr(cache_seqlens), _ptr(new_lens),
-            _ptr(free_pages), _ptr(free_count), B, int(page_block_size), free_pages.shape[0],
-            _ptr(seqlens_out), _ptr(cu_new_lens), _ptr(slot_map), slot_map.shape[0],
+            block_table.data_ptr(), block_table.shape[1], cache_seqlens.data_ptr(),
+            new_lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), B,
+            int(page_block_size), free_pages.shape[0], seqlens_out.data_ptr(),
+            cu_new_lens.data_ptr(), slot_map.data_ptr(), slot_map.shape[0],
             _stream_handle(stream, dev)))
     return slot_map, cu_new_lens, seqlens_out
 
@@ -539,13 +546,14 @@ def release_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, keep_l
     become -1; the lengths are not changed.  Releasing what the last
     assign_pages took leaves the stack as it was."""
     lib = load_library()
-    B = _check_pool(block_table, {"cache_seqlens": cache_seqlens, "keep_lens": keep_lens}, free_pages,
-                    free_count)
+    B = _check_pool(block_table, free_pages, free_count)
+    _check_int32("cache_seqlens", cache_seqlens, (B,))
+    _check_int32("keep_lens", keep_lens, (B,))
     with _on_device(block_table.device):
         check(lib.fd_release_pages(
-            _ptr(block_table), block_table.shape[1], _ptr(cache_seqlens), _ptr(keep_lens),
-            _ptr(free_pages), _ptr(free_count), B, int(page_block_size), free_pages.shape[0],
-            _stream_handle(stream, block_table.device)))
+            block_table.data_ptr(), block_table.shape[1], cache_seqlens.data_ptr(),
+            keep_lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), B,
+            int(page_block_size), free_pages.shape[0], _stream_handle(stream, block_table.device)))
 
 
 def combine_lse(part_o: torch.Tensor, part_lse: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,

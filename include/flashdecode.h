@@ -348,7 +348,8 @@ int fd_assign_pages(int32_t* block_table, int64_t block_table_stride, const int3
  * max(keep_lens[b], 0) (0 for a finished request; the accepted length after
  * speculation).  Their table entries become -1 and they are pushed on the
  * stack in reverse order, so that releasing what the last fd_assign_pages took
- * leaves the stack as it was.  An entry outside the pool is dropped, and so is
+ * leaves the stack as it was (what lies past free_count[0] is not defined).  An
+ * entry outside the pool is dropped, and so is
  * a page for which the stack has no room (a page released twice); both are
  * reported (FD_ERR_BAD_PAGE).  The lengths are not changed.  At most 8192
  * requests.

@@ -60,8 +60,8 @@ def release_and_check(s, lens, keep, page):
     flashdecode.release_pages(s["table"], lens, keep, s["pool"], s["count"], page)
     torch.cuda.synchronize()
     assert torch.equal(s["table"].cpu(), table)
-    assert torch.equal(s["pool"].cpu(), pool)
     assert s["count"].tolist() == [left, 0]
+    assert torch.equal(s["pool"][:left].cpu(), pool[:left])   # past the count nothing is defined
 
 
 @pytest.mark.parametrize("page", [1, 16, 48, 256])
