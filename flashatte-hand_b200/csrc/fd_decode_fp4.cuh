@@ -537,7 +537,8 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     }
 
     // Before the first segment's first tile the ring is filled, by rounds that
-    // only issue (one place in the code: it is long, and cold at a launch's start).
+    // only issue: one place in the code, which is long, and cold when a launch
+    // starts.  (The query is read first: behind a full ring it waited 2 us.)
     for (int k = seg_r == 0 ? -G::kStages : 0; k < ntiles; ++k) {
       if (k >= 0) {
       copy_wait<G::kStages - 1>();
@@ -821,96 +822,117 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
         }
     }
     if (nseg == 1) continue;
+    constexpr int kAt = D == 256 ? 2 : 4;
     int last = 0;
     if (tw == 0) {
       __threadfence();
       __syncwarp();
       if (lane == 0) {
         unsigned long long* ticket = p.tickets + static_cast<int64_t>(pair) * HW + hw;
-        last = ticket_arrive(ticket, *launch_epoch, nseg) ? 1 : 0;
+        last = ticket_add(ticket, *launch_epoch, nseg) ? 1 : 0;
         // every segment of the pair has counted itself: clear for later launches
         if (last) *reinterpret_cast<volatile unsigned long long*>(ticket) = 0ull;
       }
       last = __shfl_sync(0xffffffffu, last, 0);
     }
-    if (TW > 1) {  // the head's other warps take a share of the rows
+    // with more rows than one round takes, the head's other warps take a share
+    const int ways = nrows > kAt ? TW : 1;
+    if (ways > 1) {
       if (tw == 0 && lane == 0) last_flag[hw] = last;
       __syncthreads();
       last = last_flag[hw];
       __syncthreads();
     }
-    if (!last) continue;
+    if (!last) continue;  // (warps tw > 0 that have no share, too)
     __threadfence();
     // The last of the pair's segments joins them: partial j of the head is
-    // part (cfirst + j + pair) * HW + hw.  A warp takes a row at a time and
-    // adds kBatch partials per round, their loads in flight together; the
-    // weights are kept relative to a running maximum.
+    // part (cfirst + j + pair) * HW + hw.  A round is kAt partials of kAt rows
+    // (of the warp's rows tw, tw + ways, ..), all their loads in flight: lane
+    // kAt v + u holds the weight of partial u of row v, relative to a running
+    // maximum.  Short code on purpose: it runs once, and cold instructions
+    // cost more than the loads (16 partials unrolled took 2 to 10 us longer).
     const int64_t first = (static_cast<int64_t>(cfirst) + pair) * HW + hw;
-    const float* plse = p.part_lse + first * rows;
-    const float* po = p.part_o + first * rows * D;
-    const int64_t lse_step = static_cast<int64_t>(HW) * rows, o_step = lse_step * D;
+    const int64_t lse_step = static_cast<int64_t>(HW) * rows;
     constexpr int kVec = D >= 128 ? 4 : 2, kPieces = D / (32 * kVec);
-    constexpr int kBatch = D == 256 ? 8 : 16;
+    const int lu = lane & (kAt - 1), lv = lane / kAt;
 #pragma unroll 1
-    for (int row = tw; row < nrows; row += TW) {
-      float mm = neg_inf, den = 0.f, o[kPieces][kVec];
+    for (int row0 = tw; row0 < nrows; row0 += kAt * ways) {
+      float mm = neg_inf, den = 0.f;  // of row lv
+      float o[kAt][kPieces][kVec];
 #pragma unroll
-      for (int q = 0; q < kPieces; ++q)
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) o[q][i] = 0.f;
-#pragma unroll 1
-      for (int j0 = 0; j0 < nseg; j0 += kBatch) {
-        float x[kBatch][kPieces][kVec], lj[kBatch];
-        const float* src = po + j0 * o_step + row * D + lane * kVec;
-        const float* lsrc = plse + j0 * lse_step + row;
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          lj[u] = neg_inf;
-          if (j0 + u < nseg) {
-            lj[u] = __ldcg(lsrc);
-#pragma unroll
-            for (int q = 0; q < kPieces; ++q) {
-              if constexpr (kVec == 4) {
-                const float4 y = __ldcg(reinterpret_cast<const float4*>(src + q * 32 * kVec));
-                x[u][q][0] = y.x; x[u][q][1] = y.y; x[u][q][2] = y.z; x[u][q][3] = y.w;
-              } else {
-                const float2 y = __ldcg(reinterpret_cast<const float2*>(src + q * 32 * kVec));
-                x[u][q][0] = y.x; x[u][q][1] = y.y;
-              }
-            }
-          }
-          src += o_step;
-          lsrc += lse_step;
-        }
-        float m_new = mm;
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) m_new = fmaxf(m_new, lj[u]);
-        const float alpha = m_new == mm ? 1.f : fast_exp2(mm - m_new);
-        mm = m_new;
-        den *= alpha;
+      for (int v = 0; v < kAt; ++v)
 #pragma unroll
         for (int q = 0; q < kPieces; ++q)
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) o[q][i] *= alpha;
+          for (int i = 0; i < kVec; ++i) o[v][q][i] = 0.f;
+#pragma unroll 1
+      for (int j0 = 0; j0 < nseg; j0 += kAt) {
+        const int64_t at_row = first * rows + row0 + j0 * lse_step;
+        const bool mine = lv < kAt && row0 + lv * ways < nrows && j0 + lu < nseg;
+        const float lj = mine ? __ldcg(p.part_lse + at_row + lv * ways + lu * lse_step) : neg_inf;
+        float x[kAt][kAt][kPieces][kVec];
+        const float* src = p.part_o + at_row * D + lane * kVec;
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          if (lj[u] == neg_inf) continue;  // empty (or past the last)
-          const float wj = fast_exp2(lj[u] - m_new);
-          den += wj;
+        for (int u = 0; u < kAt; ++u) {
+#pragma unroll
+          for (int v = 0; v < kAt; ++v) {
+            if (j0 + u < nseg && row0 + v * ways < nrows) {
+#pragma unroll
+              for (int q = 0; q < kPieces; ++q) {
+                const float* at_v = src + v * ways * D + q * 32 * kVec;
+                if constexpr (kVec == 4) {
+                  const float4 y = __ldcg(reinterpret_cast<const float4*>(at_v));
+                  x[v][u][q][0] = y.x; x[v][u][q][1] = y.y; x[v][u][q][2] = y.z; x[v][u][q][3] = y.w;
+                } else {
+                  const float2 y = __ldcg(reinterpret_cast<const float2*>(at_v));
+                  x[v][u][q][0] = y.x; x[v][u][q][1] = y.y;
+                }
+              }
+            }
+          }
+          src += lse_step * D;
+        }
+        float m_new = fmaxf(lj, __shfl_xor_sync(0xffffffffu, lj, 1));
+        if constexpr (kAt == 4) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, 2));
+        m_new = fmaxf(mm, m_new);
+        const float w = lj == neg_inf ? 0.f : fast_exp2(lj - m_new);  // 0: empty, or past the last
+        const float alpha = m_new == mm ? 1.f : fast_exp2(mm - m_new);
+        mm = m_new;
+        float sum = w + __shfl_xor_sync(0xffffffffu, w, 1);
+        if constexpr (kAt == 4) sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        den = fmaf(den, alpha, sum);
+#pragma unroll
+        for (int v = 0; v < kAt; ++v) {
+          const float av = __shfl_sync(0xffffffffu, alpha, v * kAt);
 #pragma unroll
           for (int q = 0; q < kPieces; ++q)
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) o[q][i] = fmaf(wj, x[u][q][i], o[q][i]);
+            for (int i = 0; i < kVec; ++i) o[v][q][i] *= av;
+#pragma unroll
+          for (int u = 0; u < kAt; ++u) {
+            const float wu = __shfl_sync(0xffffffffu, w, v * kAt + u);
+            if (wu == 0.f) continue;
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+              for (int i = 0; i < kVec; ++i) o[v][q][i] = fmaf(wu, x[v][u][q][i], o[v][q][i]);
+          }
         }
       }
       const bool some = !(den == 0.f);
       const float inv = some ? 1.f / den : 0.f;
-      OutT* dst = out_at(row);
+      if (lv < kAt && lu == 0 && row0 + lv * ways < nrows)
+        put_lse(row0 + lv * ways, some ? mm + fast_log2(den) : neg_inf);
 #pragma unroll
-      for (int q = 0; q < kPieces; ++q)
+      for (int v = 0; v < kAt; ++v) {
+        const float iv = __shfl_sync(0xffffffffu, inv, v * kAt);
+        if (row0 + v * ways >= nrows) continue;
+        OutT* dst = out_at(row0 + v * ways) + lane * kVec;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) dst[q * 32 * kVec + lane * kVec + i] = fp4_out<OutT>(o[q][i] * inv);
-      if (lane == 0) put_lse(row, some ? mm + fast_log2(den) : neg_inf);
+        for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) dst[q * 32 * kVec + i] = fp4_out<OutT>(o[v][q][i] * iv);
+      }
     }
   }
   // Every CTA counts itself once it has read the epoch; the last one hands

@@ -40,6 +40,16 @@ __device__ __forceinline__ bool ticket_arrive(unsigned long long* t, unsigned lo
   }
 }
 
+// The same arrival in one round trip where the counter already carries the
+// epoch (every arrival of a pair but the first): count first, look after.  A
+// counter of another epoch is only made larger, and is overwritten as above.
+__device__ __forceinline__ bool ticket_add(unsigned long long* t, unsigned long long epoch, int nseg) {
+  const unsigned long long old = atomicAdd(t, 1ull);
+  if ((old >> kTicketCountBits) == epoch)
+    return (old & kTicketCountMask) + 1ull == static_cast<unsigned long long>(nseg);
+  return ticket_arrive(t, epoch, nseg);
+}
+
 // ---------------------------------------------------------------- schedule
 // Work is split in cost space.  In units where the K/V bytes of a full
 // 128-token tile cost kFullTile = 8, a tile also costs `tile_fixed` (its
