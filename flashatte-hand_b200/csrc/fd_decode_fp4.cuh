@@ -279,9 +279,10 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   // The cursor of the loads, a ring ahead of the multiplication: pc_left
   // tiles of the segment entered last (seg_ring[seg_w - 1]) are left, the
   // next, its pc_k-th, at token pc_tok.  offs[2 i + g] are the byte offsets
-  // (codes; block scales; -1: no page) of tokens 16 g .. of the warp's stage
-  // 16 n + i of the segment, next_* the page id and row (-1: no tokens) of
-  // the same entry of batch n + 1.
+  // (codes; block scales) of tokens 16 g .. of the warp's stage 16 n + i of
+  // the segment, plus 16, the bytes that a lane copies from there - or 0 and
+  // so no bytes where there is no page; next_* the page id and row (-1: no
+  // tokens) of the same entry of batch n + 1.
   int pc_left = 0, pc_tok = 0, pc_end = 0, pc_k = 0, next_id = 0, next_row = -1, seg_w = 0;
   // A copy instruction moves 16 bytes a lane: half the lanes rows of K, half
   // of V, so that a lane needs one pointer; kCopies of them are 16 tokens.
@@ -290,7 +291,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   constexpr int kCopies = 16 / kRowsPer;
   const int64_t row_bytes = static_cast<int64_t>(p.num_heads_k) * RB;
   const int lr = (lane & 15) / kChunks, lc = lane % kChunks;
-  const uint8_t* code_src = (lane < 16 ? p.k_cache : p.v_cache) + lr * row_bytes + lc * 16;
+  const uint8_t* code_src = (lane < 16 ? p.k_cache : p.v_cache) + lr * row_bytes + lc * 16 - 16;
   const int64_t copy_step = kRowsPer * row_bytes;
   const uint32_t code_dst = smem_u32(ring) + (lane < 16 ? 0 : G::kTileBytes) + lr * RB;
   // block scales: kScaleChunks 16-byte chunks of K, then of V (in two
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   constexpr int kScaleCopies = 2 * kScaleChunks > 32 ? 2 : 1;
   const int sx = lane % kScaleChunks, sg = sx / (kScaleChunks / 2), s_first = sx * 16 / SB;
   const uint8_t* scale_src =
-      (kScaleCopies == 1 && lane >= kScaleChunks ? p.v_block : p.k_block) + (sx % (kScaleChunks / 2)) * 16;
+      (kScaleCopies == 1 && lane >= kScaleChunks ? p.v_block : p.k_block) + (sx % (kScaleChunks / 2)) * 16 - 16;
   const uint32_t scale_dst = smem_u32(ring) + 2 * G::kTileBytes + lane * 16;
   auto entry = [&](int i) { return seg_ring + (i & (kSegRing - 1)) * 2; };
   auto segment_of = [&](int i) {
@@ -322,13 +323,13 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   auto turn_batch = [&](int k0) {  // next_* become offs, and the batch after it is fetched
     __syncwarp();
     longlong2 o;
-    o.x = o.y = -1;
+    o.x = o.y = 0;
     if (next_row >= 0 && (next_id < 0 || next_id >= p.num_blocks)) {
       report_status(p.err, kStatusBadPage);  // its rows are read as zeros
     } else if (next_row >= 0) {
       const int head = volatile_at(entry(seg_w - 1)).y / p.row_tiles * HW + hw;
-      o.x = (static_cast<int64_t>(next_id) * p.page + next_row) * row_bytes + head * RB;
-      o.y = ((static_cast<int64_t>(next_id) * p.num_heads_k + head) * p.page + next_row) * SB;
+      o.x = (static_cast<int64_t>(next_id) * p.page + next_row) * row_bytes + head * RB + 16;
+      o.y = ((static_cast<int64_t>(next_id) * p.num_heads_k + head) * p.page + next_row) * SB + 16;
     }
     offs[lane] = o;
     __syncwarp();
@@ -349,52 +350,33 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     fetch_ids(0);
     turn_batch(0);
   };
-  // Copies the cursor's stage to ring slot `slot`, and moves the cursor on.
-  auto issue = [&](int slot) {
-    if (pc_left > 0) {
-      const uint32_t at = slot * G::kStageBytes;
-      const longlong2* o2 = offs + (pc_k & 15) * 2;
+  // Copies a stage, entries o2[0 .. 1] of offs, to the ring at byte `at`.
+  auto copy_stage = [&](const longlong2* o2, uint32_t at) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {  // 16 tokens of one page
-        const int64_t off = o2[g].x;
-        const uint8_t* src = code_src + off;
-        if (off >= 0) {
+    for (int g = 0; g < 2; ++g) {  // 16 tokens of one page
+      const int64_t off = o2[g].x;
+      const int valid = static_cast<int>(off) & 16;
+      const uint8_t* src = code_src + off;
 #pragma unroll
-          for (int i = 0; i < kCopies; ++i) {
-            copy16(code_dst + at + (g * 16 + i * kRowsPer) * RB + swizzled<RB>(i * kRowsPer + lr, lc) * 16, src, 16);
-            src += copy_step;
-          }
-        } else {  // no page: zeros
-#pragma unroll
-          for (int i = 0; i < kCopies; ++i)
-            copy16(code_dst + at + (g * 16 + i * kRowsPer) * RB + swizzled<RB>(i * kRowsPer + lr, lc) * 16, code_src, 0);
-        }
-      }
-      // The block scales of tokens behind the sequence's end hold whatever
-      // memory held, NaN too, and 0 * NaN would reach O: they are written as
-      // zeros.
-      if (lane < 2 * kScaleChunks) {
-        const int64_t off = o2[sg].y;
-        int valid = off < 0 ? 0 : 16;
-        if (pc_tok + kSubTokens > pc_end) {
-          const int left = (pc_end - pc_tok - s_first) * SB;
-          valid = left <= 0 ? 0 : (left < valid ? left : valid);
-        }
-        const uint8_t* src = scale_src + (off < 0 ? 0 : off);
-        copy16(scale_dst + at, src, valid);
-        if constexpr (kScaleCopies == 2) copy16(scale_dst + at + G::kTileScales, src + (p.v_block - p.k_block), valid);
-      }
-      ++pc_k;
-      pc_tok += step;
-      if (--pc_left == 0) {
-        const Schedule sched = schedule();
-        Segment nx;
-        if (sched.next(segment_of(seg_w - 1), sched.range_start(cta + 1), nx)) enter(nx);
-      } else if ((pc_k & 15) == 0) {
-        turn_batch(pc_k);
+      for (int i = 0; i < kCopies; ++i) {
+        copy16(code_dst + at + (g * 16 + i * kRowsPer) * RB + swizzled<RB>(i * kRowsPer + lr, lc) * 16, src, valid);
+        src += copy_step;
       }
     }
-    copy_commit();  // one group a stage, empty ones too, so that the count of groups stays fixed
+    // The block scales of tokens behind the sequence's end hold whatever
+    // memory held, NaN too, and 0 * NaN would reach O: they are written as
+    // zeros.
+    if (2 * kScaleChunks >= 32 || lane < 2 * kScaleChunks) {
+      const int64_t off = o2[sg].y;
+      int valid = static_cast<int>(off) & 16;
+      if (pc_tok + kSubTokens > pc_end) {
+        const int left = (pc_end - pc_tok - s_first) * SB;
+        valid = left <= 0 ? 0 : (left < valid ? left : valid);
+      }
+      const uint8_t* src = scale_src + off;
+      copy16(scale_dst + at, src, valid);
+      if constexpr (kScaleCopies == 2) copy16(scale_dst + at + G::kTileScales, src + (p.v_block - p.k_block), valid);
+    }
   };
   {
     const Schedule sched = schedule();
@@ -402,7 +384,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     if (sched.first(cta, g)) enter(g);
   }
   // ------------------------------------------------------------ segments
-  int slot = 0;
+  uint32_t at = 0;  // byte of the ring's next stage
   // The lane's places in a stage.  tau: token of row r of an 8-token half
   // tile (neighbours swapped in every second pair); tx, ty: tau of rows 2 c
   // and 2 c + 1.  Rows 8, 16 and 24 further on have the same swizzle.
@@ -454,8 +436,8 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     uint32_t qf[NT][KS][2];
     float qfac[NT][2];  // per column of the lane (query rows 2 c, 2 c + 1 of each 8)
     {
-    const Place at = place();
-    const int b = at.b, kvh = at.kvh, row_base = at.row_base, nrows = at.nrows;
+    const Place pl = place();
+    const int b = pl.b, kvh = pl.kvh, row_base = pl.row_base, nrows = pl.nrows;
     const float factor = __ldg(p.k_scale + kvh) * p.scale_log2;
     const float sign = factor > 0.f ? 1.f : (factor < 0.f ? -1.f : factor);
     float row_inv[NT];  // 2^-k of the row's scaling
@@ -539,11 +521,23 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     // Before the first segment's first tile the ring is filled, by rounds that
     // only issue: one place in the code, which is long, and cold when a launch
     // starts.  (The query is read first: behind a full ring it waited 2 us.)
-    for (int k = seg_r == 0 ? -G::kStages : 0; k < ntiles; ++k) {
+    // The rounds run in batches between which the cursor needs attention (its
+    // segment or its page offsets end), so that the inner loop holds none of
+    // that: its branches and the jumps over its code cost 100 cycles a round.
+    for (int k = seg_r == 0 ? -G::kStages : 0; k < ntiles;) {
+      const bool more = pc_left > 0;
+      int n = ntiles - k;
+      if (more) {
+        const int turn = 16 - (pc_k & 15), calm = pc_left < turn ? pc_left : turn;
+        n = n < calm ? n : calm;
+      }
+      const longlong2* o2 = offs + (pc_k & 15) * 2;
+#pragma unroll 1
+      for (const int stop = k + n; k < stop; ++k) {
       if (k >= 0) {
       copy_wait<G::kStages - 1>();
       __syncwarp();  // every lane's copies of the stage have landed
-      const uint8_t* st = ring + slot * G::kStageBytes;
+      const uint8_t* st = ring + at;
 
       // ---- S^T = K . Q^T, two tiles of 16 tokens side by side
       float s[2][NT][4];
@@ -711,8 +705,25 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       }
       // ---- refill the stage
       __syncwarp();  // every lane has read it
-      issue(slot);
-      slot = slot + 1 == G::kStages ? 0 : slot + 1;
+      if (more) {
+        copy_stage(o2, at);
+        o2 += 2;
+        pc_tok += step;
+      }
+      copy_commit();  // one group a stage, empty ones too, so that the count of groups stays fixed
+      at = at == (G::kStages - 1) * G::kStageBytes ? 0 : at + G::kStageBytes;
+      }
+      if (more) {
+        pc_k += n;
+        pc_left -= n;
+        if (pc_left == 0) {
+          const Schedule sched = schedule();
+          Segment nx;
+          if (sched.next(segment_of(seg_w - 1), sched.range_start(cta + 1), nx)) enter(nx);
+        } else if ((pc_k & 15) == 0) {
+          turn_batch(pc_k);
+        }
+      }
     }
 
     // ---- the rows' sums; warps that share a head are joined on its first
@@ -777,8 +788,8 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     }
 
     // ---- write: the output, or a partial of a pair cut by range boundaries
-    const Place at = place();
-    const int b = at.b, kvh = at.kvh, row_base = at.row_base, nrows = at.nrows;
+    const Place pl = place();
+    const int b = pl.b, kvh = pl.kvh, row_base = pl.row_base, nrows = pl.nrows;
     const int4 sb = volatile_at(entry(seg_r) + 1);
     const int pair = sb.y, nseg = sb.z, cfirst = sb.w;
     const int64_t part = (static_cast<int64_t>(cta) + pair) * HW + hw;
