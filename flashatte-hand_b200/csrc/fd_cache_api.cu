@@ -21,16 +21,18 @@ constexpr int kMaxDevices = 64;
 constexpr int kCostTile4 = 2;
 constexpr int kCostSeg4 = 30;
 constexpr int kCostFloor4 = 0;
+constexpr int kAlignTiles4 = 12;
 int cost_tile4() { static const int v = fd::env_int("FD_COST_TILE4", kCostTile4, 0, 64); return v; }
 int cost_seg4() { static const int v = fd::env_int("FD_COST_SEG4", kCostSeg4, 1, 256); return v; }
 int cost_floor4() { static const int v = fd::env_int("FD_COST_FLOOR4", kCostFloor4, 0, 1024); return v; }
+int align_tiles4() { static const int v = fd::env_int("FD_ALIGN_TILES4", kAlignTiles4, 0, 4096); return v; }
 int max_lead4() { return cost_seg4() > cost_floor4() ? cost_seg4() : cost_floor4(); }
 
 // A partial for every (sequence, KV head, row tile), and for every KV head of
 // the first and last segment of each CTA.
 fd::WorkspaceLayout fp4_workspace(int64_t batch, int64_t num_heads_k, int64_t qrows, int rows, int grid_max,
                                   int head_dim) {
-  return fd::workspace_layout(batch, num_heads_k * ((qrows + rows - 1) / rows), rows, 4 * grid_max, head_dim);
+  return fd::workspace_layout(batch, num_heads_k * ((qrows + rows - 1) / rows), rows, 2 * grid_max, head_dim);
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -382,7 +384,8 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
   const int64_t tiles_bound = (len_bound * heads + fd::kTileTokens - 1) / fd::kTileTokens;
   const int64_t per_seq_cost = max_lead4() + ((kv_max * heads + fd::kTileTokens - 1) / fd::kTileTokens + 1) *
                                                  (8 + static_cast<int64_t>(cost_tile4()));
-  const int64_t per_launch = fd::seqs_per_launch(per_seq_cost, 0, vheads, grid_max);
+  const int64_t aligned_cost = max_lead4() + static_cast<int64_t>(align_tiles4()) * (8 + cost_tile4()) + 1;
+  const int64_t per_launch = fd::seqs_per_launch(per_seq_cost, aligned_cost, num_heads_k * row_tiles, grid_max);
   if (per_launch == 0) return report_error(FD_ERR_UNSUPPORTED, "sequence too long");
 
   int len_add = 0;
@@ -431,6 +434,7 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
     p.cost_tile = cost_tile4();
     p.cost_seg = cost_seg4();
     p.cost_floor = cost_floor4();
+    p.align_tiles = align_tiles4();
     p.pdl = fd::pdl_enabled() ? 1 : 0;
     const int64_t work = nb * vheads * tiles_bound;
     const int grid = static_cast<int>(work < grid_max ? work : grid_max);

@@ -44,10 +44,10 @@
 // 16 bytes each with cp.async, eight rows an instruction, past L1.
 //
 // A CTA is four warps, and a schedule tile four 32-token stages, one a warp:
-// p.heads (4, 2 or 1) neighbouring KV heads of the same tokens, so that the
-// warps together read whole runs of a token's heads (64-byte pieces read at
-// different times cost 1.27 times the DRAM traffic), times 4 / p.heads stages
-// along the sequence.  Each warp has a ring and a softmax state of its own,
+// HW = 2 neighbouring KV heads of the same tokens (1 where their number is odd,
+// and in short launches), so that the warps together read 128-byte runs (one
+// head a CTA cost 1.27 times the DRAM traffic), times 4 / HW stages along the
+// sequence.  Each warp has a ring and a softmax state of its own,
 // and nothing in the loop waits for another warp.  The ring runs across
 // segments (a segment is the CTA's part of a sequence's heads): the next
 // one's first loads are in flight while this one is written out.  Work split
@@ -93,7 +93,7 @@ template <int D, int NT> struct Fp4Geo {
   static constexpr int kOffSegs = kOffOffs + kFp4Warps * 32 * 16;        // [warps][kSegRing]
   static constexpr int kOffJoin = kOffSegs + kFp4Warps * kSegRing * 32;  // [kFp4Warps - 1]
   static constexpr int kOffMisc = kOffJoin + (kFp4Warps - 1) * kJoinWarp;
-  static constexpr int kOffPrefix = kOffMisc + 16;
+  static constexpr int kOffPrefix = kOffMisc + 32;
   static constexpr int kOffLens = kOffPrefix + (kMaxBatchPerLaunch + 1) * 4;
   static constexpr int kSmemBytes = kOffLens + kMaxBatchPerLaunch * 4;
   static_assert(kSegRing > kStages + 1, "the loads run at most kStages segments ahead");
@@ -129,6 +129,15 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// p + n * step in one instruction of the FMA pipe (a 64-bit addition is two of
+// the ALU's, which bounds the loop).
+__device__ __forceinline__ const uint8_t* plus_multiple(const uint8_t* p, uint32_t step, uint32_t n) {
+  if (n == 0) return p;
+  uint64_t d;
+  asm("mad.wide.u32 %0, %1, %2, %3;" : "=l"(d) : "r"(step), "r"(n), "l"(reinterpret_cast<uint64_t>(p)));
+  return reinterpret_cast<const uint8_t*>(d);
 }
 
 // Read from shared memory here and now: not hoisted, not kept in registers.
@@ -208,14 +217,11 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   int4* seg_ring = reinterpret_cast<int4*>(smem + G::kOffSegs) + warp * kSegRing * 2;
   unsigned long long* launch_epoch = reinterpret_cast<unsigned long long*>(smem + G::kOffMisc);
   volatile int* last_flag = reinterpret_cast<volatile int*>(smem + G::kOffMisc + 8);  // [2]
+  int* align_word = reinterpret_cast<int*>(smem + G::kOffMisc + 16);
   int* prefix = reinterpret_cast<int*>(smem + G::kOffPrefix);
   int* lens = reinterpret_cast<int*>(smem + G::kOffLens);
 
   const int batch = p.batch, cta = blockIdx.x;
-  const int HW = p.heads, TW = kFp4Warps / HW;    // warps over heads, warps over tokens
-  const int hw = warp & (HW - 1), tw = warp / HW;
-  const int step = TW * kSubTokens;               // tokens of a schedule tile
-  // a pair of the schedule is (sequence, HW KV heads, row tile)
   const float neg_inf = -__int_as_float(0x7f800000);
 
   // ------------------------------------------------------------ prologue
@@ -224,20 +230,40 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   pdl_wait_prerequisites();
   unsigned long long epoch_ld = 0;
   if (tid == 0) epoch_ld = *reinterpret_cast<volatile unsigned long long*>(p.epoch_word);
+  // Short launches: where every CTA's share is m = ceil(pairs / grid) whole
+  // (sequence, KV head, row tile) pairs of at most align_tiles / m tiles of
+  // kTileTokens, each CTA takes m whole pairs, a head at a time: no pair is
+  // cut, so no partial, arrival or joining lengthens a launch that is one
+  // latency chain (see fd_decode_sm100.cuh).
+  const int pairs = batch * p.num_heads_k * p.row_tiles;
+  const int align_m = (pairs + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  const int align_max = p.align_tiles / align_m;
+  bool is_short = align_max > 0;
   for (int b = tid; b < batch; b += kFp4Threads) {
     const int stored = __ldg(p.seqlens + b);
     const int64_t max_len = p.bt_stride * static_cast<int64_t>(p.page);
     const int64_t want = static_cast<int64_t>(stored < 0 ? 0 : stored) + p.len_add;
     const int64_t cap = max_len < 0x1fffffff ? max_len : 0x1fffffff;
-    // The schedule counts tiles of kTileTokens; a tile here is `step` tokens
-    // of HW heads, so lengths are given to it times HW.
-    const int len = static_cast<int>(want > cap ? cap : want) * HW;
+    const int len = static_cast<int>(want > cap ? cap : want);
     lens[b] = len;
-    prefix[b + 1] = cm.pair_cost(len);
+    is_short = is_short && seq_tiles(len) <= align_max;
+  }
+  const bool aligned = __syncthreads_and(is_short) != 0;
+  const int HW = aligned ? 1 : p.heads, TW = kFp4Warps / HW;  // warps over heads, warps over tokens
+  const int hw = warp & (HW - 1), tw = warp / HW;
+  const int step = TW * kSubTokens;                           // tokens of a schedule tile
+  // A pair of the schedule is (sequence, HW KV heads, row tile).  It counts
+  // tiles of kTileTokens; a tile here is `step` tokens of HW heads, so lengths
+  // are given to it times HW.
+  for (int b = tid; b < batch; b += kFp4Threads) {
+    const int len = lens[b] * HW;
+    lens[b] = len;
+    prefix[b + 1] = aligned ? cm.max_lead() + p.align_tiles * cm.full() + 1 : cm.pair_cost(len);
   }
   if (tid == 0) {
     prefix[0] = 0;
     *launch_epoch = epoch_ld & kEpochMax;
+    *align_word = aligned ? align_m : 0;
   }
   __syncthreads();
   if (warp == 0) {
@@ -263,15 +289,19 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     x.cost_prefix = prefix;
     x.lens = lens;
     x.max_len = 0;
-    x.total = static_cast<int64_t>(p.num_heads_k / p.heads * p.row_tiles) * volatile_at(prefix + p.batch);
+    x.total = static_cast<int64_t>(p.num_heads_k / HW * p.row_tiles) * volatile_at(prefix + p.batch);
     x.batch = p.batch;
-    x.hkv = p.num_heads_k / p.heads * p.row_tiles;
+    x.hkv = p.num_heads_k / HW * p.row_tiles;
     x.cm = CostModel{p.cost_tile, p.cost_seg, p.cost_floor};
-    x.align_m = 0;
-    x.align_cost = 0;
-    // every range longer than the costliest tile: none inside a pair is empty
-    const int64_t g = div_u32(x.total, x.cm.max_lead() + x.cm.full() + 1);
-    x.grid = static_cast<int>(g < 1 ? 1 : (g < gridDim.x ? g : gridDim.x));
+    x.align_m = volatile_at(align_word);
+    x.align_cost = x.cm.max_lead() + p.align_tiles * x.cm.full() + 1;
+    if (x.align_m > 0) {
+      x.grid = (x.batch * x.hkv + x.align_m - 1) / x.align_m;
+    } else {
+      // every range longer than the costliest tile: none inside a pair is empty
+      const int64_t g = div_u32(x.total, x.cm.max_lead() + x.cm.full() + 1);
+      x.grid = static_cast<int>(g < 1 ? 1 : (g < gridDim.x ? g : gridDim.x));
+    }
     return x;
   };
 
@@ -292,7 +322,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   const int64_t row_bytes = static_cast<int64_t>(p.num_heads_k) * RB;
   const int lr = (lane & 15) / kChunks, lc = lane % kChunks;
   const uint8_t* code_src = (lane < 16 ? p.k_cache : p.v_cache) + lr * row_bytes + lc * 16 - 16;
-  const int64_t copy_step = kRowsPer * row_bytes;
+  const uint32_t copy_step = kRowsPer * static_cast<uint32_t>(row_bytes);
   const uint32_t code_dst = smem_u32(ring) + (lane < 16 ? 0 : G::kTileBytes) + lr * RB;
   // block scales: kScaleChunks 16-byte chunks of K, then of V (in two
   // instructions at D = 256); a chunk's group of 16 tokens and first token
@@ -358,10 +388,9 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       const int valid = static_cast<int>(off) & 16;
       const uint8_t* src = code_src + off;
 #pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        copy16(code_dst + at + (g * 16 + i * kRowsPer) * RB + swizzled<RB>(i * kRowsPer + lr, lc) * 16, src, valid);
-        src += copy_step;
-      }
+      for (int i = 0; i < kCopies; ++i)
+        copy16(code_dst + at + (g * 16 + i * kRowsPer) * RB + swizzled<RB>(i * kRowsPer + lr, lc) * 16,
+               plus_multiple(src, copy_step, i), valid);
     }
     // The block scales of tokens behind the sequence's end hold whatever
     // memory held, NaN too, and 0 * NaN would reach O: they are written as

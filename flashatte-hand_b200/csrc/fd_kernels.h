@@ -164,7 +164,7 @@ struct Fp4DecodeParams {
   int batch, num_heads, num_heads_k, group, page;
   int seqlen_q, causal, qrows;   // qrows = seqlen_q * group
   int row_tiles, rows;           // query rows are taken `rows` at a time, in row_tiles passes
-  int heads;                     // KV heads that a CTA takes together: 4, 2 or 1
+  int heads;                     // KV heads that a CTA takes together: 2 or 1
   int len_add;
   float scale_log2;
   float* part_o;                 // [slots, rows, D] normalised partial O
@@ -173,6 +173,7 @@ struct Fp4DecodeParams {
   unsigned long long* epoch_word;
   int* err;
   int cost_tile, cost_seg, cost_floor;
+  int align_tiles;               // short launches: most tiles of a CTA (0: never)
   int pdl;
 };
 // Query rows of one pass for this head dim (8 or 16).
