@@ -52,11 +52,15 @@ def parse():
     ap.add_argument("--no-e2e", action="store_true")
     ap.add_argument("--shard", default="auto", choices=["auto", "heads"],
                     help="N>1: the config's default partition, or KV-head sharding")
-    ap.add_argument("--kv", default="native", choices=["native", "fp8"],
-                    help="K/V cache storage: the config's dtype, or e4m3 with per-head scales")
+    ap.add_argument("--kv", default="native", choices=["native", "fp8", "fp4"],
+                    help="K/V cache storage: the config's dtype, e4m3 with per-head scales, or "
+                         "e2m1 with block scales")
     ap.add_argument("--contest", action="store_true",
                     help="time the reference evaluator's contest shapes (rank 0, one JSON line)")
     return ap.parse_args()
+
+
+KV_SUFFIX = {"native": "", "fp8": "_e4m3kv", "fp4": "_e2m1kv"}
 
 
 def plan(args, world):
@@ -72,8 +76,7 @@ def plan(args, world):
         scaling, parallel = "strong", f"batch-shard{world}"
     else:
         scaling, parallel = "strong", f"splitkv{world}-p2p"
-    fp8 = args.kv == "fp8"
-    cfg = {"workload": full.name + ("_e4m3kv" if fp8 else ""),
+    cfg = {"workload": full.name + KV_SUFFIX[args.kv],
            "global_batch": full.B * (world if scaling == "weak" else 1),
            "seq_len": int(full.seqlens.max()), "parallelism": parallel,
            "Hq": full.Hq, "Hkv": full.Hkv, "head_dim": full.D, "page": full.page,
@@ -472,14 +475,20 @@ def main():
         total_kv = full.kv_bytes()
         t = cases.materialize(case, "cuda", seed=0)  # same q on every rank
         splitter = fdist.PeerSplitKVDecode(case.B, case.Hq, case.D, case.dtype, "cuda")
-    fp8 = args.kv == "fp8"
-    if fp8:
+    fp8, fp4 = args.kv == "fp8", args.kv == "fp4"
+    kv_share = (1, 1)  # of the 16-bit cache's bytes
+    kv_kw = {}
+    if fp4 and splitter is not None:
+        raise SystemExit("--kv fp4: the cross-GPU split-KV step takes 16-bit and e4m3 caches")
+    if fp8 or fp4:
         del t
         torch.cuda.empty_cache()
         # split-KV ranks share one query (seed 0), as above
-        t = cases.materialize_e4m3(case, "cuda", seed=0 if splitter is not None else rank)
-        total_kv //= 2
-    kv_kw = dict(k_scale=t["k_scale"], v_scale=t["v_scale"]) if fp8 else {}
+        t = (cases.materialize_e4m3 if fp8 else cases.materialize_fp4)(
+            case, "cuda", seed=0 if splitter is not None else rank)
+        kv_share = (1, 2) if fp8 else (9, 32)
+        total_kv = total_kv * kv_share[0] // kv_share[1]
+        kv_kw = {n: t[n] for n in t if n.endswith("_scale")}
     max_len = max(int(case.seqlens.max()), 1)
 
     def make_decode(q, seqlens, bt, out=None, lse=None):
@@ -633,17 +642,17 @@ def main():
 
     per_call_s = ms * 1e-3 / args.steps
     kv_gbs = total_kv / per_call_s / 1e9
-    alg_per_launch = case.algorithmic_bytes(with_lse=True) - (case.kv_bytes() // 2 if fp8 else 0)
+    alg_per_launch = case.algorithmic_bytes(with_lse=True) - (case.kv_bytes() - case.kv_bytes() * kv_share[0] // kv_share[1])
     achieved = alg_per_launch / per_call_s / 1e9
     peak, peak_kind = peaks()
     roofline = {"bound": "hbm", "achieved": round(achieved, 1), "peak": peak, "unit": "GB/s",
                 "frac": round(achieved / peak, 4),
-                "traffic": (profile_traffic(f"cfg{args.config}" + ("_e4m3kv" if fp8 else ""))
+                "traffic": (profile_traffic(f"cfg{args.config}" + KV_SUFFIX[args.kv])
                             if world == 1 else None),
-                "peak_source": peak_kind, "kernel": "decode_sm100_kernel",
+                "peak_source": peak_kind, "kernel": "decode_fp4_kernel" if fp4 else "decode_sm100_kernel",
                 "alg_bytes_per_launch": alg_per_launch}
     cpu = None
-    if world == 1 and args.cpu_seconds > 0 and not fp8:
+    if world == 1 and args.cpu_seconds > 0 and args.kv == "native":
         ct = {k: v.cpu() for k, v in t.items()}
         rate, nseq, dt = cpu_oracle_rate(case, ct, args.cpu_seconds)
         cpu = {"value": round(rate, 4), "unit": "GB/s", "cores": torch.get_num_threads(), "kind": "port",
@@ -654,7 +663,7 @@ def main():
         "steps": args.steps, "warmup": args.warmup, "ms_per_step": round(per_call_s * 1e3, 5),
         "us_per_call": round(per_call_s * 1e6, 2), "pct_of_peak": round(100 * kv_gbs / world / peak, 2),
         "higher_is_better": True, "scaling": scaling, "vs_baseline": None,
-        "dtype": ("e4m3-kv/" if fp8 else "") + ("bf16" if case.dtype == torch.bfloat16 else "fp16"),
+        "dtype": ("e4m3-kv/" if fp8 else "e2m1-kv/" if fp4 else "") + ("bf16" if case.dtype == torch.bfloat16 else "fp16"),
         "data": "synthetic", "config": config,
         "roofline": roofline, "cpu_baseline": cpu, "e2e": e2e,
         "gpu_launches": launches_per_call * args.steps, "clocks": clk.summary(),

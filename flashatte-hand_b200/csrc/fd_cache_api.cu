@@ -17,16 +17,26 @@ using fd::report_error;
 
 constexpr int kMaxDevices = 64;
 
-// Split cost model of the 4-bit cache (units and meaning as in fd_api.cu).
+// Split cost model of the 4-bit cache (units and meaning as in fd_api.cu: a
+// tile, 128 tokens of one head or 64 of two, costs 8 and a bit).  A pair costs
+// its CTA about 4 us beside its tiles (query, joining, partials, arrival), four
+// tiles' time.  Charged in full it balances launches with more pairs than CTAs
+// (config 3: 142 us at 30, 131 us at 45); with fewer pairs it mostly makes the
+// ranges, which must be longer than a pair's share, too coarse (4 speculated
+// tokens of 32 sequences: 47 us at 30, 50 us at 45).
 constexpr int kCostTile4 = 2;
 constexpr int kCostSeg4 = 30;
-constexpr int kCostFloor4 = 0;
+constexpr int kCostSegMany4 = 45;
+// Short launches take whole pairs where no CTA gets more than 12 tiles: eight
+// 1k-token sequences 19.8 -> 16.0 us, but config 1 (16 tiles) 19.8 -> 21.5.
 constexpr int kAlignTiles4 = 12;
 int cost_tile4() { static const int v = fd::env_int("FD_COST_TILE4", kCostTile4, 0, 64); return v; }
-int cost_seg4() { static const int v = fd::env_int("FD_COST_SEG4", kCostSeg4, 1, 256); return v; }
-int cost_floor4() { static const int v = fd::env_int("FD_COST_FLOOR4", kCostFloor4, 0, 1024); return v; }
+int cost_seg4(bool many) {
+  static const int few = fd::env_int("FD_COST_SEG4", kCostSeg4, 1, 256);
+  static const int lot = fd::env_int("FD_COST_SEG4", kCostSegMany4, 1, 256);
+  return many ? lot : few;
+}
 int align_tiles4() { static const int v = fd::env_int("FD_ALIGN_TILES4", kAlignTiles4, 0, 4096); return v; }
-int max_lead4() { return cost_seg4() > cost_floor4() ? cost_seg4() : cost_floor4(); }
 
 // A partial for every (sequence, KV head, row tile), and for every KV head of
 // the first and last segment of each CTA.
@@ -382,9 +392,10 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
   const int64_t len_bound = max_seqlen_k > 0 && max_seqlen_k < kv_max ? max_seqlen_k : kv_max;
   // the schedule's tiles are kTileTokens / heads tokens of `heads` heads
   const int64_t tiles_bound = (len_bound * heads + fd::kTileTokens - 1) / fd::kTileTokens;
-  const int64_t per_seq_cost = max_lead4() + ((kv_max * heads + fd::kTileTokens - 1) / fd::kTileTokens + 1) *
+  const int lead = cost_seg4(batch_size * vheads >= grid_max);
+  const int64_t per_seq_cost = lead + ((kv_max * heads + fd::kTileTokens - 1) / fd::kTileTokens + 1) *
                                                  (8 + static_cast<int64_t>(cost_tile4()));
-  const int64_t aligned_cost = max_lead4() + static_cast<int64_t>(align_tiles4()) * (8 + cost_tile4()) + 1;
+  const int64_t aligned_cost = lead + static_cast<int64_t>(align_tiles4()) * (8 + cost_tile4()) + 1;
   const int64_t per_launch = fd::seqs_per_launch(per_seq_cost, aligned_cost, num_heads_k * row_tiles, grid_max);
   if (per_launch == 0) return report_error(FD_ERR_UNSUPPORTED, "sequence too long");
 
@@ -432,8 +443,8 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
     p.epoch_word = reinterpret_cast<unsigned long long*>(ws + wl.epoch_off);
     p.err = status;
     p.cost_tile = cost_tile4();
-    p.cost_seg = cost_seg4();
-    p.cost_floor = cost_floor4();
+    p.cost_seg = lead;
+    p.cost_floor = 0;
     p.align_tiles = align_tiles4();
     p.pdl = fd::pdl_enabled() ? 1 : 0;
     const int64_t work = nb * vheads * tiles_bound;

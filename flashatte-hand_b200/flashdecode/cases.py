@@ -176,6 +176,29 @@ def materialize_e4m3(case: DecodeCase, device, seed: int = 0) -> dict:
     return t
 
 
+def materialize_fp4(case: DecodeCase, device, seed: int = 0) -> dict:
+    """materialize() with a 4-bit block-scaled K/V cache: the N(0, 1) K and V
+    are appended to it row by row (append_kv_slots) with per-KV-head scales in
+    [1/512, 1/256); q stays case.dtype.  Adds k_scale, v_scale, k_block_scale,
+    v_block_scale.  CUDA devices only."""
+    from .ops import append_kv_slots
+    t = materialize(case, device, seed=seed)
+    dev = torch.device(device)
+    g = torch.Generator().manual_seed(seed + 2)
+    t["k_scale"] = ((1.0 + torch.rand(case.Hkv, generator=g)) / 512.0).to(dev)
+    t["v_scale"] = ((1.0 + torch.rand(case.Hkv, generator=g)) / 512.0).to(dev)
+    shape = (case.num_blocks, case.page, case.Hkv, case.D // 2)
+    blocks = (case.num_blocks, case.Hkv, case.page, case.D // 16)
+    k, v = (t[n].flatten(0, 1) for n in ("k_cache", "v_cache"))
+    for n in ("k", "v"):
+        t[n + "_cache"] = torch.zeros(shape, dtype=torch.uint8, device=dev).view(torch.float4_e2m1fn_x2)
+        t[n + "_block_scale"] = torch.zeros(blocks, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+    append_kv_slots(k, v, t["k_cache"], t["v_cache"], torch.arange(k.shape[0], device=dev),
+                    k_scale=t["k_scale"], v_scale=t["v_scale"], k_block_scale=t["k_block_scale"],
+                    v_block_scale=t["v_block_scale"])
+    return t
+
+
 def lpt_partition(seqlens, world: int) -> list[list[int]]:
     """Longest-processing-time-first assignment of sequences to `world` shards."""
     order = sorted(range(len(seqlens)), key=lambda b: (-int(seqlens[b]), b))

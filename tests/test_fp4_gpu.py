@@ -297,6 +297,96 @@ def test_plan_graph_streams_and_workspace():
     assert flashdecode.device_status() == 0
 
 
+def test_captured_append_and_decode():
+    """The fused append captured with its decode: replays write the rows in
+    the bound buffers and attend them; lengths advance between replays."""
+    seqlens = [0, 30, 700]
+    t = make(seqlens, 8, 2, page=16, seed=13, extra_len=6)
+    d = on_gpu(t)
+    kn, vn = (torch.zeros((3, 1, 2, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    plan = flashdecode.DecodePlan(d["q"], d["k"], d["v"], d["lens"], d["bt"], return_softmax_lse=True, k=kn, v=vn,
+                                  k_scale=d["ks"], v_scale=d["vs"], k_block_scale=d["kb"], v_block_scale=d["vb"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan()
+    g = torch.Generator().manual_seed(1)
+    for step in range(6):
+        new = [torch.randn((3, 1, 2, 128), generator=g).bfloat16() for _ in range(2)]
+        kn.copy_(new[0])
+        vn.copy_(new[1])
+        graph.replay()
+        torch.cuda.synchronize()
+        for n, x in zip("kv", new):
+            codes, blocks = quantize_fp4(x, t[n + "s"])
+            for b, L in enumerate(seqlens):
+                pg, row = int(t["bt"][b, (L + step) // 16]), (L + step) % 16
+                t[n][pg, row] = codes[b, 0]
+                t[n + "b"][pg, :, row] = blocks[b, 0]
+        check(plan.out, plan.lse, reference(t, lens=t["lens"] + step + 1))
+        d["lens"] += 1
+    assert flashdecode.device_status() == 0
+
+
+def test_two_streams_at_once():
+    """Calls on two streams overlap, each with its stream's scratch."""
+    ts = [make([6000, 40, 3000], 32, 8, seed=s) for s in (1, 2)]
+    ds = [on_gpu(t) for t in ts]
+    want = [call(d) for d in ds]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ds]
+    for _ in range(5):
+        got = []
+        for d, st in zip(ds, streams):
+            with torch.cuda.stream(st):
+                got.append(call(d))
+        torch.cuda.synchronize()
+        for (o, l), (wo, wl) in zip(got, want):
+            assert torch.equal(o, wo) and torch.equal(l, wl)
+    for t, (o, l) in zip(ts, want):
+        check(o, l, reference(t))
+
+
+def test_offsets_beyond_32_bits():
+    """A pool of more than 4 GiB of codes: the pages in use lie at its ends."""
+    page, Hkv, D, nb = 256, 8, 128, 40000
+    L = [600, 500]
+    ids = torch.tensor([[nb - 1, 0, nb - 2], [nb - 3, 39000, -1]], dtype=torch.int32)
+    g = torch.Generator().manual_seed(2)
+    t = dict(q=torch.randn((2, 1, 32, D), generator=g).bfloat16(), lens=torch.tensor(L, dtype=torch.int32),
+             ks=torch.full((Hkv,), 1 / 256), vs=torch.full((Hkv,), 1 / 300))
+    d = {n: x.cuda() for n, x in t.items()}
+    d["bt"] = ids.cuda()
+    for n in ("k", "v"):
+        d[n] = torch.zeros((nb, page, Hkv, D // 2), dtype=torch.uint8, device="cuda").view(FP4)
+        d[n + "b"] = torch.zeros((nb, Hkv, page, D // 16), dtype=torch.uint8, device="cuda").view(E4M3)
+    rows = [torch.randn((sum(L), Hkv, D), generator=g).bfloat16() for _ in range(2)]
+    pos = torch.cat([torch.arange(n) for n in L])
+    owner = torch.cat([torch.full((n,), b) for b, n in enumerate(L)])
+    slots = ids[owner, pos // page].long() * page + pos % page
+    flashdecode.append_kv_slots(rows[0].cuda(), rows[1].cuda(), d["k"], d["v"], slots.cuda(), k_scale=d["ks"],
+                                v_scale=d["vs"], k_block_scale=d["kb"], v_block_scale=d["vb"])
+    out, lse = call(d)
+    torch.cuda.synchronize()
+    t["bt"] = torch.arange(2)[:, None]     # the reference: one page a request
+    for n, x in zip("kv", rows):
+        wide = torch.zeros((2, max(L), Hkv, D), dtype=torch.bfloat16)
+        wide[owner, pos] = x
+        t[n], blocks = quantize_fp4(wide, t[n + "s"])
+        t[n + "b"] = blocks.permute(0, 2, 1, 3).contiguous()
+    check(out, lse, reference(t))
+    assert flashdecode.device_status() == 0
+
+
+def test_workload_materialised_through_the_append():
+    c = cases.custom_case("m", torch.bfloat16, [40, 300, 7], 8, 2, page=16, seed=3)
+    t = cases.materialize_fp4(c, "cuda", seed=3)
+    t16 = cases.materialize(c, "cuda", seed=3)
+    for n in ("k", "v"):
+        codes, blocks = quantize_fp4(t16[n + "_cache"], t[n + "_scale"])
+        assert torch.equal(t[n + "_cache"].view(torch.uint8).cpu(), codes)
+        assert torch.equal(t[n + "_block_scale"].view(torch.uint8).cpu(), blocks.permute(0, 2, 1, 3))
+
+
 def test_serving_steps_together():
     """Prompts arrive, get pages and slots, are appended and attended; then
     decode steps with growing lengths; one request leaves and its pages go to
