@@ -355,7 +355,7 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
       batch_size * seqlen_q * num_heads > INT32_MAX || block_table_stride > INT32_MAX ||
       (k_new != nullptr && batch_size * seqlen_new > INT32_MAX))
     return report_error(FD_ERR_UNSUPPORTED, "size exceeds 32-bit index range");
-  if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(k_block_scale, 16) ||
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(k_block_scale, 16) ||
       !aligned(v_block_scale, 16) || !aligned(k_new, 16) || !aligned(v_new, 16))
     return report_error(FD_ERR_UNSUPPORTED, "e2m1 cache: tensors must be 16-byte aligned");
   int dev = 0;
@@ -388,7 +388,9 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
     return report_error(FD_ERR_WORKSPACE, "workspace not 256-byte aligned");
   }
 
-  const int64_t kv_max = block_table_stride * page_block_size;
+  // (a length counts up to 2^29 - 1 tokens, as the kernel clamps it)
+  const int64_t rows_max = block_table_stride * page_block_size;
+  const int64_t kv_max = rows_max < 0x1fffffff ? rows_max : 0x1fffffff;
   const int64_t len_bound = max_seqlen_k > 0 && max_seqlen_k < kv_max ? max_seqlen_k : kv_max;
   // the schedule's tiles are kTileTokens / heads tokens of `heads` heads
   const int64_t tiles_bound = (len_bound * heads + fd::kTileTokens - 1) / fd::kTileTokens;

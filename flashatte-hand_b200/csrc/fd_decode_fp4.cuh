@@ -140,6 +140,9 @@ __device__ __forceinline__ const uint8_t* plus_multiple(const uint8_t* p, uint32
   return reinterpret_cast<const uint8_t*>(d);
 }
 
+// 0xFF at the bytes of w that are NaN in e4m3
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
+
 // Read from shared memory here and now: not hoisted, not kept in registers.
 __device__ __forceinline__ int volatile_at(const int* p) { return *reinterpret_cast<const volatile int*>(p); }
 __device__ __forceinline__ int4 volatile_at(const int4* p) {
@@ -178,15 +181,28 @@ template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, ui
   }
 }
 
-// N consecutive values, rounded once, in 16-byte stores where they fill them.
+template <typename O> __device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
+  if constexpr (std::is_same<O, __half>::value) {
+    return pack_half2(lo, hi);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// N consecutive values, rounded once, in 16-byte stores.
 template <typename O, int N> __device__ __forceinline__ void store_row(O* dst, const float (&x)[N]) {
   if constexpr (sizeof(O) == 4) {
 #pragma unroll
     for (int i = 0; i < N; i += 4)
       *reinterpret_cast<float4*>(dst + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
   } else {
+    static_assert(N % 8 == 0, "whole 16-byte stores");
 #pragma unroll
-    for (int i = 0; i < N; ++i) dst[i] = fp4_out<O>(x[i]);
+    for (int i = 0; i < N; i += 8)
+      *reinterpret_cast<uint4*>(dst + i) =
+          make_uint4(pack_out<O>(x[i], x[i + 1]), pack_out<O>(x[i + 2], x[i + 3]), pack_out<O>(x[i + 4], x[i + 5]),
+                     pack_out<O>(x[i + 6], x[i + 7]));
   }
 }
 
@@ -638,6 +654,43 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
               if (t0 + mt * 16 + tau + 8 >= seen) s[mt][nt][e + 2] = neg_inf;
             }
           }
+        if constexpr (MULTI) {
+          // A NaN block scale of V (0 * NaN is NaN) must not reach the rows
+          // that do not see its token: it is taken out of the stage, and put
+          // into O's block of the rows that do see it.
+          uint32_t* sb = reinterpret_cast<uint32_t*>(ring + at + 2 * G::kTileBytes + G::kTileScales + lane * SB);
+          bool any = false;
+#pragma unroll
+          for (int i = 0; i < SB / 4; ++i) any = any || nan_bytes(sb[i]) != 0;
+          unsigned tokens = __ballot_sync(0xffffffffu, any);
+          if (tokens != 0) {
+#pragma unroll 1
+            for (; tokens != 0; tokens &= tokens - 1) {
+              const int u = __ffs(tokens) - 1;
+              const uint8_t* row = st + 2 * G::kTileBytes + G::kTileScales + u * SB + r * (D / 8) / 16;
+#pragma unroll
+              for (int j = 0; j < (D + 127) / 128; ++j) {  // the lane's blocks, of MT / that many tiles each
+                constexpr int kPer = MT / ((D + 127) / 128);
+                if (nan_bytes(row[j]) == 0) continue;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const int seen =
+                        len + (p.causal ? (base + nt * 8 + 2 * c + e) / p.group - (p.seqlen_q - 1) : 0);
+                    if (t0 + u >= seen) continue;
+#pragma unroll
+                    for (int i = j * kPer; i < (j + 1) * kPer; ++i)
+                      acc[i][nt][e] = acc[i][nt][e + 2] = __int_as_float(0x7fffffff);
+                  }
+              }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < SB / 4; ++i) sb[i] &= ~nan_bytes(sb[i]);
+            __syncwarp();
+          }
+        }
       }
       // The reference of the exponents need not be the maximum: it is raised
       // (and O, l rescaled) only when a logit exceeds it by more than 8, so

@@ -64,6 +64,14 @@ def _require_cuda(*tensors: torch.Tensor) -> None:
             raise ValueError("flashdecode runs on CUDA tensors only (no CPU path)")
 
 
+def _require_device(index: int, *tensors) -> None:
+    """Every tensor of a call (None: not given) lies on one device: a kernel
+    that followed a pointer of another one would fault."""
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError("the tensors of a call must lie on one device")
+
+
 def run_kernel(q, k_cache_paged, v_cache_paged, output, cache_seqlens, block_table, batch_size,
                seqlen_k, seqlen_q, num_heads, num_heads_k, headdim, page_block_size, num_blocks,
                causal) -> None:
@@ -87,9 +95,13 @@ def device_status() -> int:
 
 
 def workspace_size(batch_size: int, num_heads: int, num_heads_k: int, headdim: int = 128,
-                   seqlen_q: int = 1) -> int:
-    return int(load_library().fd_decode_workspace_size_mq(batch_size, seqlen_q, num_heads,
-                                                          num_heads_k, headdim))
+                   seqlen_q: int = 1, kv_dtype: torch.dtype | None = None) -> int:
+    """Bytes of workspace that flash_decode needs (kv_dtype: that of the
+    caches, to be given for float4_e2m1fn_x2)."""
+    lib = load_library()
+    size = lib.fd_decode_workspace_size_fp4 if kv_dtype == torch.float4_e2m1fn_x2 \
+        else lib.fd_decode_workspace_size_mq
+    return int(size(batch_size, seqlen_q, num_heads, num_heads_k, headdim))
 
 
 def flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -203,6 +215,8 @@ def _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, ret
     if kv4:
         if k is not None:
             _check_new_kv(k, v, k_cache, B, q.dtype)
+        _require_device(q.get_device(), k_cache, v_cache, k_block_scale, v_block_scale, k_scale, v_scale,
+                        k, v, out, lse, cache_seqlens, block_table, workspace)
         args = (_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_block_scale), _ptr(v_block_scale),
                 _ptr(k_scale), _ptr(v_scale), _ptr(k), _ptr(v), 0 if k is None else k.shape[1],
                 _ptr(out), _ptr(lse), _ptr(cache_seqlens), _ptr(block_table),
@@ -348,6 +362,8 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         _check_new_kv(k, v, k_cache, B, k.dtype)
         if cache_seqlens.shape != (B,) or not cache_seqlens.is_contiguous():
             raise ValueError("cache_seqlens must be a contiguous [B] tensor")
+        _require_device(k.get_device(), v, k_cache, v_cache, k_block_scale, v_block_scale, k_scale,
+                        v_scale, cache_seqlens, block_table)
         with torch.cuda.device(k.device):
             status = lib.fd_append_kv_paged_fp4(
                 _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(k_block_scale),
@@ -426,6 +442,8 @@ def append_kv_slots(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
                       or (T > 1 and x.stride(0) < Hkv * D)):
             raise ValueError(f"the heads of a token of {name} must be contiguous")
     row = Hkv * D
+    _require_device(k_cache.get_device(), v_cache, slot_map, k, v, k_scale, v_scale, k_block_scale,
+                    v_block_scale)
     with _on_device(k_cache.device):
         check(lib.fd_append_kv_slots(
             _ptr(k), k.stride(0) if T > 1 else row, _ptr(v), v.stride(0) if T > 1 else row,
@@ -458,6 +476,8 @@ def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_map: torch.Tens
                 or not x.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {out_dtype} {(T, Hkv, D)} CUDA tensor")
         outs.append(x)
+    _require_device(k_cache.get_device(), v_cache, slot_map, k_scale, v_scale, k_block_scale,
+                    v_block_scale, *outs)
     with _on_device(k_cache.device):
         check(lib.fd_gather_kv_slots(
             _ptr(k_cache), _ptr(v_cache), _ptr(k_block_scale), _ptr(v_block_scale), _ptr(k_scale),
@@ -528,6 +548,8 @@ def assign_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, new_len
         seqlens_out = torch.empty((B,), dtype=torch.int32, device=dev)
     else:
         _check_int32("seqlens_out", seqlens_out, (B,))
+    _require_device(block_table.get_device(), cache_seqlens, new_lens, free_pages, free_count, slot_map,
+                    cu_new_lens, seqlens_out)
     with _on_device(dev):
         check(lib.fd_assign_pages(
             block_table.data_ptr(), block_table.shape[1], cache_seqlens.data_ptr(),
@@ -549,6 +571,7 @@ def release_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, keep_l
     B = _check_pool(block_table, free_pages, free_count)
     _check_int32("cache_seqlens", cache_seqlens, (B,))
     _check_int32("keep_lens", keep_lens, (B,))
+    _require_device(block_table.get_device(), cache_seqlens, keep_lens, free_pages, free_count)
     with _on_device(block_table.device):
         check(lib.fd_release_pages(
             block_table.data_ptr(), block_table.shape[1], cache_seqlens.data_ptr(),

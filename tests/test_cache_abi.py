@@ -119,3 +119,27 @@ def test_python_calls_refuse_cpu_tensors():
 
 def test_status_string(lib):
     assert lib.fd_error_string(7) == b"not enough pages or slots for the step"
+
+
+@pytest.mark.parametrize("kw", [dict(out=P + 2), dict(odt=FP32, out=P + 4)])
+def test_decode_fp4_output_alignment(lib, kw):
+    assert lib.fd_decode_paged_fp4(*decode_args(**kw)) == UNSUPPORTED
+
+
+def test_tensors_of_several_devices_are_refused():
+    class OnDevice:
+        def __init__(self, index):
+            self.index = index
+
+        def get_device(self):
+            return self.index
+
+    from flashdecode import ops
+    ops._require_device(1, OnDevice(1), None, OnDevice(1))
+    with pytest.raises(ValueError, match="one device"):
+        ops._require_device(0, OnDevice(0), None, OnDevice(1))
+
+
+def test_workspace_size_by_cache_type(lib):
+    import torch
+    assert flashdecode.workspace_size(2, 8, 2, 96, kv_dtype=torch.float4_e2m1fn_x2) == 0   # not a head dim it has

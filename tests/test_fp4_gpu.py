@@ -204,6 +204,36 @@ def test_nan_and_infinity_travel_only_in_their_rows():
     assert nan[0, 0, :4, 16:32].all() and not nan[0, 0, :4, 32:].any() and not nan[0, 0, 4:].any()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (6, 1)])
+def test_nan_scales_stay_behind_the_causal_mask(D, Hq, Hkv):
+    """A speculated token with NaN block scales (of K, of V) reaches the rows
+    that see it, as the formula has it, and no row before it."""
+    sq, seqlens, first_bad = 4, [4, 63, 130, 2], {0: 3, 1: 62, 2: 128}
+    t = make(seqlens, Hq, Hkv, D=D, page=16, sq=sq, seed=D)
+    clean = {n: x.clone() for n, x in t.items()}
+    for b, at in first_bad.items():
+        pg, row = int(t["bt"][b, at // 16]), at % 16
+        t["vb"][pg, 0, row, 1] = 0xFF                 # dims 16 .. 31 of KV head 0
+        if b == 2:
+            t["kb"][pg, 0, row + 1, 0] = 0x7F         # and all dims from the next token on
+    out, lse = call(on_gpu(t), causal=True)
+    torch.cuda.synchronize()
+    ref = reference(clean, causal=True)
+    nan = torch.isnan(out.cpu())
+    want = torch.zeros_like(nan)
+    G = Hq // Hkv
+    for b, at in first_bad.items():
+        for i in range(sq):
+            seen = seqlens[b] - (sq - 1 - i)
+            want[b, i, :G, 16:32] = seen > at
+            if b == 2 and seen > at + 1:
+                want[b, i, :G] = True
+    assert torch.equal(nan, want)
+    lse = torch.where(torch.isnan(lse.cpu()), ref[1].float(), lse.cpu())
+    check(torch.where(nan, ref[0].to(out.dtype), out.cpu()), lse, ref)
+
+
 def test_bad_pages_read_as_zeros():
     for bad in (-1, 10 ** 6):
         t = make([500, 100], 8, 2, page=16, seed=8)
