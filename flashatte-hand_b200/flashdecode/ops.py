@@ -64,9 +64,12 @@ def _require_cuda(*tensors: torch.Tensor) -> None:
             raise ValueError("flashdecode runs on CUDA tensors only (no CPU path)")
 
 
-def _require_device(index: int, *tensors) -> None:
-    """Every tensor of a call (None: not given) lies on one device: a kernel
-    that followed a pointer of another one would fault."""
+def _require_device(first, *tensors) -> None:
+    """Every tensor of a call (None: not given) lies on one CUDA device: a
+    kernel that followed a pointer of another one would fault."""
+    index = first.get_device()
+    if index < 0:
+        raise ValueError("flashdecode runs on CUDA tensors only (no CPU path)")
     for t in tensors:
         if t is not None and t.get_device() != index:
             raise ValueError("the tensors of a call must lie on one device")
@@ -215,7 +218,7 @@ def _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, ret
     if kv4:
         if k is not None:
             _check_new_kv(k, v, k_cache, B, q.dtype)
-        _require_device(q.get_device(), k_cache, v_cache, k_block_scale, v_block_scale, k_scale, v_scale,
+        _require_device(q, k_cache, v_cache, k_block_scale, v_block_scale, k_scale, v_scale,
                         k, v, out, lse, cache_seqlens, block_table, workspace)
         args = (_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_block_scale), _ptr(v_block_scale),
                 _ptr(k_scale), _ptr(v_scale), _ptr(k), _ptr(v), 0 if k is None else k.shape[1],
@@ -302,16 +305,16 @@ def _check_block_scales(k_block_scale, v_block_scale, k_cache: torch.Tensor) -> 
         if k_block_scale is not None or v_block_scale is not None:
             raise ValueError("k_block_scale / v_block_scale apply to float4_e2m1fn_x2 caches only")
         return
-    if k_cache.dim() != 4 or k_cache.shape[3] % 8 != 0:
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[3] % 8 != 0:
         raise ValueError("a float4_e2m1fn_x2 cache is [num_blocks, page, Hkv, D / 2] with D a "
                          "multiple of 16")
-    num_blocks, page, Hkv, half = k_cache.shape
+    num_blocks, page, Hkv, half = shape
     want = (num_blocks, Hkv, page, half // 8)
     for name, sc in (("k_block_scale", k_block_scale), ("v_block_scale", v_block_scale)):
         if sc is None:
             raise ValueError(f"{name} is required with a float4_e2m1fn_x2 cache")
-        _require_cuda(sc)
-        if sc.dtype != torch.float8_e4m3fn or tuple(sc.shape) != want or not sc.is_contiguous():
+        if sc.dtype != torch.float8_e4m3fn or sc.shape != want or not sc.is_contiguous():
             raise ValueError(f"{name} must be a contiguous float8_e4m3fn {want} tensor")
 
 
@@ -362,7 +365,7 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         _check_new_kv(k, v, k_cache, B, k.dtype)
         if cache_seqlens.shape != (B,) or not cache_seqlens.is_contiguous():
             raise ValueError("cache_seqlens must be a contiguous [B] tensor")
-        _require_device(k.get_device(), v, k_cache, v_cache, k_block_scale, v_block_scale, k_scale,
+        _require_device(k, v, k_cache, v_cache, k_block_scale, v_block_scale, k_scale,
                         v_scale, cache_seqlens, block_table)
         with torch.cuda.device(k.device):
             status = lib.fd_append_kv_paged_fp4(
@@ -394,26 +397,25 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
 
 
 def _check_slot_cache(k_cache, v_cache, slot_map, k_scale, v_scale, k_block_scale, v_block_scale):
-    """Checks that append_kv_slots and gather_kv share; returns (T, page,
-    Hkv, D, num_blocks) of the call."""
-    _require_cuda(k_cache, v_cache, slot_map)
-    if k_cache.dtype not in _CACHE_DTYPES or v_cache.dtype != k_cache.dtype or k_cache.dim() != 4 \
-            or v_cache.shape != k_cache.shape:
+    """Checks that append_kv_slots and gather_kv share, but for the device of
+    the tensors; returns (T, page, Hkv, D, num_blocks) of the call."""
+    dtype, shape = k_cache.dtype, k_cache.shape
+    if dtype not in _CACHE_DTYPES or v_cache.dtype != dtype or len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("k_cache/v_cache must be bf16, fp16, float8_e4m3fn or float4_e2m1fn_x2 "
                          "[num_blocks, page, Hkv, D] tensors with equal shapes")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("caches must be contiguous")
-    if slot_map.dtype != torch.int64 or slot_map.dim() != 1 or not slot_map.is_contiguous():
+    slots = slot_map.shape
+    if slot_map.dtype != torch.int64 or len(slots) != 1 or not slot_map.is_contiguous():
         raise ValueError("slot_map must be a contiguous int64 [T] tensor")
-    num_blocks, page, Hkv, D = k_cache.shape
-    if k_cache.dtype in _DTYPES:
+    num_blocks, page, Hkv, D = shape
+    if dtype in _DTYPES:
         if k_scale is not None or v_scale is not None:
             raise ValueError("k_scale / v_scale apply to float8_e4m3fn and float4_e2m1fn_x2 caches only")
     else:
         _check_scales(k_scale, v_scale, Hkv)
     _check_block_scales(k_block_scale, v_block_scale, k_cache)
-    return (slot_map.shape[0], page, Hkv, 2 * D if k_cache.dtype == torch.float4_e2m1fn_x2 else D,
-            num_blocks)
+    return slots[0], page, Hkv, 2 * D if dtype == torch.float4_e2m1fn_x2 else D, num_blocks
 
 
 def append_kv_slots(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -428,28 +430,30 @@ def append_kv_slots(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     is of any kind flash_decode reads, and quantised ones take their scales.
     The slots should be distinct."""
     lib = load_library()
+    _require_device(k_cache, v_cache, slot_map, k, v, k_scale, v_scale, k_block_scale, v_block_scale)
     T, page, Hkv, D, num_blocks = _check_slot_cache(k_cache, v_cache, slot_map, k_scale, v_scale,
                                                     k_block_scale, v_block_scale)
-    _require_cuda(k, v)
-    if k.dtype not in _DTYPES or v.dtype != k.dtype:
+    src, dst = _DTYPES.get(k.dtype), _CACHE_DTYPES[k_cache.dtype]
+    if src is None or v.dtype != k.dtype:
         raise ValueError("k / v must be bf16 or fp16")
-    if k_cache.dtype in _DTYPES and k.dtype != k_cache.dtype:
+    if k_cache.dtype in _DTYPES and src != dst:
         raise ValueError(f"k / v must be {k_cache.dtype}")
-    for name, x in (("k", k), ("v", v)):
-        if tuple(x.shape) != (T, Hkv, D):
-            raise ValueError(f"{name} must be [T, Hkv, D] = {(T, Hkv, D)}, got {tuple(x.shape)}")
-        if T > 0 and ((D > 1 and x.stride(2) != 1) or (Hkv > 1 and x.stride(1) != D)
-                      or (T > 1 and x.stride(0) < Hkv * D)):
-            raise ValueError(f"the heads of a token of {name} must be contiguous")
+    want = (T, Hkv, D)
     row = Hkv * D
-    _require_device(k_cache.get_device(), v_cache, slot_map, k, v, k_scale, v_scale, k_block_scale,
-                    v_block_scale)
-    with _on_device(k_cache.device):
+    token = []
+    for name, x in (("k", k), ("v", v)):
+        if x.shape != want:
+            raise ValueError(f"{name} must be [T, Hkv, D] = {want}, got {tuple(x.shape)}")
+        st, sh, sd = x.stride()
+        if T > 0 and ((D > 1 and sd != 1) or (Hkv > 1 and sh != D) or (T > 1 and st < row)):
+            raise ValueError(f"the heads of a token of {name} must be contiguous")
+        token.append(st if T > 1 else row)
+    dev = k_cache.device
+    with _on_device(dev):
         check(lib.fd_append_kv_slots(
-            _ptr(k), k.stride(0) if T > 1 else row, _ptr(v), v.stride(0) if T > 1 else row,
-            _ptr(k_cache), _ptr(v_cache), _ptr(k_block_scale), _ptr(v_block_scale), _ptr(k_scale),
-            _ptr(v_scale), _ptr(slot_map), T, Hkv, D, page, num_blocks, _DTYPES[k.dtype],
-            _CACHE_DTYPES[k_cache.dtype], _stream_handle(stream, k_cache.device)))
+            k.data_ptr(), token[0], v.data_ptr(), token[1], k_cache.data_ptr(), v_cache.data_ptr(),
+            _ptr(k_block_scale), _ptr(v_block_scale), _ptr(k_scale), _ptr(v_scale), slot_map.data_ptr(),
+            T, Hkv, D, page, num_blocks, src, dst, _stream_handle(stream, dev)))
 
 
 def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_map: torch.Tensor,
@@ -461,49 +465,49 @@ def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_map: torch.Tens
     out_dtype (default: the cache's type, bf16 for quantised caches), zeros at
     negative slots.  The inverse of append_kv_slots."""
     lib = load_library()
+    _require_device(k_cache, v_cache, slot_map, k_scale, v_scale, k_block_scale, v_block_scale, k_out, v_out)
     T, page, Hkv, D, num_blocks = _check_slot_cache(k_cache, v_cache, slot_map, k_scale, v_scale,
                                                     k_block_scale, v_block_scale)
     if out_dtype is None:
         out_dtype = k_out.dtype if k_out is not None else \
             k_cache.dtype if k_cache.dtype in _DTYPES else torch.bfloat16
-    if out_dtype not in _OUT_DTYPES:
+    odt = _OUT_DTYPES.get(out_dtype)
+    if odt is None:
         raise ValueError("out_dtype must be bf16, fp16 or fp32")
-    outs = []
+    dev = k_cache.device
+    want = (T, Hkv, D)
     for name, x in (("k_out", k_out), ("v_out", v_out)):
-        if x is None:
-            x = torch.empty((T, Hkv, D), dtype=out_dtype, device=k_cache.device)
-        elif not x.is_cuda or x.dtype != out_dtype or tuple(x.shape) != (T, Hkv, D) \
-                or not x.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous {out_dtype} {(T, Hkv, D)} CUDA tensor")
-        outs.append(x)
-    _require_device(k_cache.get_device(), v_cache, slot_map, k_scale, v_scale, k_block_scale,
-                    v_block_scale, *outs)
-    with _on_device(k_cache.device):
+        if x is not None and (x.dtype != out_dtype or x.shape != want or not x.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous {out_dtype} {want} CUDA tensor")
+    if k_out is None:
+        k_out = torch.empty(T, Hkv, D, dtype=out_dtype, device=dev)
+    if v_out is None:
+        v_out = torch.empty_like(k_out)
+    with _on_device(dev):
         check(lib.fd_gather_kv_slots(
-            _ptr(k_cache), _ptr(v_cache), _ptr(k_block_scale), _ptr(v_block_scale), _ptr(k_scale),
-            _ptr(v_scale), _ptr(slot_map), T, _ptr(outs[0]), _ptr(outs[1]), Hkv, D, page, num_blocks,
-            _CACHE_DTYPES[k_cache.dtype], _OUT_DTYPES[out_dtype],
-            _stream_handle(stream, k_cache.device)))
-    return outs[0], outs[1]
+            k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_block_scale), _ptr(v_block_scale),
+            _ptr(k_scale), _ptr(v_scale), slot_map.data_ptr(), T, k_out.data_ptr(), v_out.data_ptr(),
+            Hkv, D, page, num_blocks, _CACHE_DTYPES[k_cache.dtype], odt, _stream_handle(stream, dev)))
+    return k_out, v_out
 
 
 def _check_int32(name: str, t: torch.Tensor, shape) -> None:
-    if not t.is_cuda:
-        raise ValueError("flashdecode runs on CUDA tensors only (no CPU path)")
     if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}")
 
 
-def _check_pool(block_table, free_pages, free_count) -> int:
-    """Checks that assign_pages and release_pages share; returns B."""
-    if block_table.dim() != 2:
+def _check_pool(block_table, free_pages, free_count) -> tuple[int, int, int]:
+    """Checks that assign_pages and release_pages share; returns (B, width of
+    the table, pages of the pool)."""
+    table, pool = block_table.shape, free_pages.shape
+    if len(table) != 2:
         raise ValueError("block_table must be [B, max_blocks]")
-    if free_pages.dim() != 1:
+    if len(pool) != 1:
         raise ValueError("free_pages must be [num_blocks]")
-    _check_int32("block_table", block_table, block_table.shape)
-    _check_int32("free_pages", free_pages, free_pages.shape)
+    _check_int32("block_table", block_table, table)
+    _check_int32("free_pages", free_pages, pool)
     _check_int32("free_count", free_count, (2,))
-    return block_table.shape[0]
+    return table[0], table[1], pool[0]
 
 
 def assign_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, new_lens: torch.Tensor,
@@ -529,33 +533,35 @@ def assign_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, new_len
     reports FD_ERR_NO_PAGES; requests are served in order.
     """
     lib = load_library()
-    B = _check_pool(block_table, free_pages, free_count)
+    _require_device(block_table, cache_seqlens, new_lens, free_pages, free_count, slot_map, cu_new_lens,
+                    seqlens_out)
+    B, width, num_blocks = _check_pool(block_table, free_pages, free_count)
     _check_int32("cache_seqlens", cache_seqlens, (B,))
     _check_int32("new_lens", new_lens, (B,))
     dev = block_table.device
     if slot_map is None:
         if num_slots is None:
             raise ValueError("give slot_map or num_slots")
-        slot_map = torch.empty((int(num_slots),), dtype=torch.int64, device=dev)
-    elif not slot_map.is_cuda or slot_map.dtype != torch.int64 or slot_map.dim() != 1 \
-            or not slot_map.is_contiguous():
-        raise ValueError("slot_map must be a contiguous int64 [num_slots] CUDA tensor")
+        num_slots = int(num_slots)
+        slot_map = torch.empty(num_slots, dtype=torch.int64, device=dev)
+    else:
+        slots = slot_map.shape
+        if slot_map.dtype != torch.int64 or len(slots) != 1 or not slot_map.is_contiguous():
+            raise ValueError("slot_map must be a contiguous int64 [num_slots] CUDA tensor")
+        num_slots = slots[0]
     if cu_new_lens is None:
-        cu_new_lens = torch.empty((B + 1,), dtype=torch.int32, device=dev)
+        cu_new_lens = new_lens.new_empty(B + 1)
     else:
         _check_int32("cu_new_lens", cu_new_lens, (B + 1,))
     if seqlens_out is None:
-        seqlens_out = torch.empty((B,), dtype=torch.int32, device=dev)
+        seqlens_out = torch.empty_like(cache_seqlens)
     else:
         _check_int32("seqlens_out", seqlens_out, (B,))
-    _require_device(block_table.get_device(), cache_seqlens, new_lens, free_pages, free_count, slot_map,
-                    cu_new_lens, seqlens_out)
     with _on_device(dev):
         check(lib.fd_assign_pages(
-            block_table.data_ptr(), block_table.shape[1], cache_seqlens.data_ptr(),
-            new_lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), B,
-            int(page_block_size), free_pages.shape[0], seqlens_out.data_ptr(),
-            cu_new_lens.data_ptr(), slot_map.data_ptr(), slot_map.shape[0],
+            block_table.data_ptr(), width, cache_seqlens.data_ptr(), new_lens.data_ptr(),
+            free_pages.data_ptr(), free_count.data_ptr(), B, int(page_block_size), num_blocks,
+            seqlens_out.data_ptr(), cu_new_lens.data_ptr(), slot_map.data_ptr(), num_slots,
             _stream_handle(stream, dev)))
     return slot_map, cu_new_lens, seqlens_out
 
@@ -568,15 +574,16 @@ def release_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, keep_l
     become -1; the lengths are not changed.  Releasing what the last
     assign_pages took leaves the stack as it was."""
     lib = load_library()
-    B = _check_pool(block_table, free_pages, free_count)
+    _require_device(block_table, cache_seqlens, keep_lens, free_pages, free_count)
+    B, width, num_blocks = _check_pool(block_table, free_pages, free_count)
     _check_int32("cache_seqlens", cache_seqlens, (B,))
     _check_int32("keep_lens", keep_lens, (B,))
-    _require_device(block_table.get_device(), cache_seqlens, keep_lens, free_pages, free_count)
-    with _on_device(block_table.device):
+    dev = block_table.device
+    with _on_device(dev):
         check(lib.fd_release_pages(
-            block_table.data_ptr(), block_table.shape[1], cache_seqlens.data_ptr(),
-            keep_lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), B,
-            int(page_block_size), free_pages.shape[0], _stream_handle(stream, block_table.device)))
+            block_table.data_ptr(), width, cache_seqlens.data_ptr(), keep_lens.data_ptr(),
+            free_pages.data_ptr(), free_count.data_ptr(), B, int(page_block_size), num_blocks,
+            _stream_handle(stream, dev)))
 
 
 def combine_lse(part_o: torch.Tensor, part_lse: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,

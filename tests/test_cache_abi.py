@@ -135,9 +135,11 @@ def test_tensors_of_several_devices_are_refused():
             return self.index
 
     from flashdecode import ops
-    ops._require_device(1, OnDevice(1), None, OnDevice(1))
+    ops._require_device(OnDevice(1), OnDevice(1), None, OnDevice(1))
     with pytest.raises(ValueError, match="one device"):
-        ops._require_device(0, OnDevice(0), None, OnDevice(1))
+        ops._require_device(OnDevice(0), OnDevice(0), None, OnDevice(1))
+    with pytest.raises(ValueError, match="CUDA tensors only"):
+        ops._require_device(OnDevice(-1), OnDevice(-1))
 
 
 def test_workspace_size_by_cache_type(lib):
