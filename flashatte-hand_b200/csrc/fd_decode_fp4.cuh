@@ -101,10 +101,22 @@ template <int D, int NT> struct Fp4Geo {
   static_assert(kStageBytes % 16 == 0 && kOffMisc % 16 == 0 && kJoinWarp % 16 == 0, "alignment");
 };
 
-// 16 bytes from global to shared memory past L1; the bytes behind `valid` are
-// written as zeros.
-__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, int valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+// 16 bytes from global to shared memory past L1, or zeros where `any` is 0.
+__device__ __forceinline__ void copy16_or_zeros(uint32_t dst, const uint8_t* src, int any) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %2, 0;\n\tcp.async.cg.shared.global [%0], [%1], 16, p;\n\t}" ::"r"(dst),
+      "l"(src), "r"(any)
+      : "memory");
+}
+// Two such copies where `any` is not 0, nothing otherwise.
+__device__ __forceinline__ void copy16x2_if(uint32_t dst0, const uint8_t* src0, uint32_t dst1, const uint8_t* src1,
+                                            int any) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %4, 0;\n\t"
+      "@p cp.async.cg.shared.global [%0], [%1], 16;\n\t"
+      "@p cp.async.cg.shared.global [%2], [%3], 16;\n\t}" ::"r"(dst0),
+      "l"(src0), "r"(dst1), "l"(src1), "r"(any)
+      : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() {
@@ -140,8 +152,28 @@ __device__ __forceinline__ const uint8_t* plus_multiple(const uint8_t* p, uint32
   return reinterpret_cast<const uint8_t*>(d);
 }
 
+__device__ __forceinline__ uint32_t low_twice(uint32_t v) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tmov.b32 %0, {lo, lo};\n\t}" : "=r"(d) : "r"(v));
+  return d;
+}
+__device__ __forceinline__ uint32_t high_twice(uint32_t v) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tmov.b32 %0, {hi, hi};\n\t}" : "=r"(d) : "r"(v));
+  return d;
+}
+__device__ __forceinline__ uint32_t times16(uint32_t v) {
+  uint32_t d;
+  asm("mad.lo.u32 %0, %1, 16, 0;" : "=r"(d) : "r"(v));
+  return d;
+}
+
 // 0xFF at the bytes of w that are NaN in e4m3
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
+
+// Keeps a value of the lane in its register: not computed again in the loop.
+__device__ __forceinline__ void keep(int& v) { asm volatile("" : "+r"(v)); }
+__device__ __forceinline__ void keep(uint32_t& v) { asm volatile("" : "+r"(v)); }
 
 // Read from shared memory here and now: not hoisted, not kept in registers.
 __device__ __forceinline__ int volatile_at(const int* p) { return *reinterpret_cast<const volatile int*>(p); }
@@ -324,12 +356,12 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   // ------------------------------------------------------------ loads
   // The cursor of the loads, a ring ahead of the multiplication: pc_left
   // tiles of the segment entered last (seg_ring[seg_w - 1]) are left, the
-  // next, its pc_k-th, at token pc_tok.  offs[2 i + g] are the byte offsets
+  // next is its pc_k-th.  offs[2 i + g] are the byte offsets
   // (codes; block scales) of tokens 16 g .. of the warp's stage 16 n + i of
   // the segment, plus 16, the bytes that a lane copies from there - or 0 and
   // so no bytes where there is no page; next_* the page id and row (-1: no
   // tokens) of the same entry of batch n + 1.
-  int pc_left = 0, pc_tok = 0, pc_end = 0, pc_k = 0, next_id = 0, next_row = -1, seg_w = 0;
+  int pc_left = 0, pc_end = 0, pc_k = 0, next_id = 0, next_row = -1, seg_w = 0;
   // A copy instruction moves 16 bytes a lane: half the lanes rows of K, half
   // of V, so that a lane needs one pointer; kCopies of them are 16 tokens.
   constexpr int kChunks = RB / 16;          // 16-byte chunks of a row of codes
@@ -339,12 +371,21 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   const int lr = (lane & 15) / kChunks, lc = lane % kChunks;
   const uint8_t* code_src = (lane < 16 ? p.k_cache : p.v_cache) + lr * row_bytes + lc * 16 - 16;
   const uint32_t copy_step = kRowsPer * static_cast<uint32_t>(row_bytes);
-  const uint32_t code_dst = smem_u32(ring) + (lane < 16 ? 0 : G::kTileBytes) + lr * RB;
+  // ring places of the lane's row in the first copies; the swizzle of copy i
+  // is that of copy i % kDstVariants
+  constexpr int kDstVariants = RB == 128 ? 4 : 2;
+  uint32_t code_dst[kDstVariants];
+#pragma unroll
+  for (int i = 0; i < kDstVariants; ++i) {
+    code_dst[i] = smem_u32(ring) + (lane < 16 ? 0 : G::kTileBytes) + lr * RB +
+                  swizzled<RB>(i * kRowsPer + lr, lc) * 16;
+    keep(code_dst[i]);
+  }
   // block scales: kScaleChunks 16-byte chunks of K, then of V (in two
-  // instructions at D = 256); a chunk's group of 16 tokens and first token
+  // instructions at D = 256); sg: the chunk's group of 16 tokens
   constexpr int kScaleChunks = G::kTileScales / 16;  // 8, 16 or 32
   constexpr int kScaleCopies = 2 * kScaleChunks > 32 ? 2 : 1;
-  const int sx = lane % kScaleChunks, sg = sx / (kScaleChunks / 2), s_first = sx * 16 / SB;
+  const int sx = lane % kScaleChunks, sg = sx / (kScaleChunks / 2);
   const uint8_t* scale_src =
       (kScaleCopies == 1 && lane >= kScaleChunks ? p.v_block : p.k_block) + (sx % (kScaleChunks / 2)) * 16 - 16;
   const uint32_t scale_dst = smem_u32(ring) + 2 * G::kTileBytes + lane * 16;
@@ -391,7 +432,6 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     ++seg_w;
     pc_left = g.ntiles;
     pc_end = g.seqlen / HW;
-    pc_tok = g.tile0 * step + tw * kSubTokens;
     pc_k = 0;
     fetch_ids(0);
     turn_batch(0);
@@ -404,23 +444,17 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       const int valid = static_cast<int>(off) & 16;
       const uint8_t* src = code_src + off;
 #pragma unroll
-      for (int i = 0; i < kCopies; ++i)
-        copy16(code_dst + at + (g * 16 + i * kRowsPer) * RB + swizzled<RB>(i * kRowsPer + lr, lc) * 16,
-               plus_multiple(src, copy_step, i), valid);
+      for (int i = 0; i < kCopies; i += 2)
+        copy16x2_if(code_dst[i % kDstVariants] + at + (g * 16 + i * kRowsPer) * RB, plus_multiple(src, copy_step, i),
+                    code_dst[(i + 1) % kDstVariants] + at + (g * 16 + (i + 1) * kRowsPer) * RB,
+                    plus_multiple(src, copy_step, i + 1), valid);
     }
-    // The block scales of tokens behind the sequence's end hold whatever
-    // memory held, NaN too, and 0 * NaN would reach O: they are written as
-    // zeros.
     if (2 * kScaleChunks >= 32 || lane < 2 * kScaleChunks) {
       const int64_t off = o2[sg].y;
-      int valid = static_cast<int>(off) & 16;
-      if (pc_tok + kSubTokens > pc_end) {
-        const int left = (pc_end - pc_tok - s_first) * SB;
-        valid = left <= 0 ? 0 : (left < valid ? left : valid);
-      }
+      const int any = static_cast<int>(off) & 16;
       const uint8_t* src = scale_src + off;
-      copy16(scale_dst + at, src, valid);
-      if constexpr (kScaleCopies == 2) copy16(scale_dst + at + G::kTileScales, src + (p.v_block - p.k_block), valid);
+      copy16_or_zeros(scale_dst + at, src, any);
+      if constexpr (kScaleCopies == 2) copy16_or_zeros(scale_dst + at + G::kTileScales, src + (p.v_block - p.k_block), any);
     }
   };
   {
@@ -450,9 +484,10 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     v_at[0] = tx * RB + swizzled<RB>(tx, r >> 2) * 16 + (r & 3) * 4;
     v_at[1] = ty * RB + swizzled<RB>(ty, r >> 2) * 16 + (r & 3) * 4;
   }
-  const int ks_at = 2 * G::kTileBytes + tau * SB + c * (D / 64);
-  const int vs_at[2] = {2 * G::kTileBytes + G::kTileScales + tx * SB + r * (D / 8) / 16,
+  int ks_at = 2 * G::kTileBytes + tau * SB + c * (D / 64);
+  int vs_at[2] = {2 * G::kTileBytes + G::kTileScales + tx * SB + r * (D / 8) / 16,
                         2 * G::kTileBytes + G::kTileScales + ty * SB + r * (D / 8) / 16};
+  keep(k_at), keep(k_at2), keep(v_at[0]), keep(v_at[1]), keep(ks_at), keep(vs_at[0]), keep(vs_at[1]);
 
   for (int seg_r = 0; seg_r < seg_w; ++seg_r) {
     int ntiles, t0, seqlen;
@@ -625,7 +660,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const uint32_t pair = kf[mt][half][blk / 2];
-            const uint32_t f = __byte_perm(pair, pair, blk & 1 ? 0x3232 : 0x1010);
+            const uint32_t f = blk & 1 ? high_twice(pair) : low_twice(pair);
             e2m1x8_to_half2x4(kw[mt][half][wi], h[half]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) h[half][j] = hmul2_bits(h[half][j], f);
@@ -654,11 +689,18 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
               if (t0 + mt * 16 + tau + 8 >= seen) s[mt][nt][e + 2] = neg_inf;
             }
           }
+        // Block scales of V must not be NaN where P is 0.  Behind the sequence's
+        // end they are what memory held: cleared.
+        uint32_t* sb = reinterpret_cast<uint32_t*>(ring + at + 2 * G::kTileBytes + G::kTileScales + lane * SB);
+        if (t0 + lane >= len) {
+#pragma unroll
+          for (int i = 0; i < SB / 4; ++i) sb[i] = 0;
+        }
+        __syncwarp();
         if constexpr (MULTI) {
-          // A NaN block scale of V (0 * NaN is NaN) must not reach the rows
-          // that do not see its token: it is taken out of the stage, and put
-          // into O's block of the rows that do see it.
-          uint32_t* sb = reinterpret_cast<uint32_t*>(ring + at + 2 * G::kTileBytes + G::kTileScales + lane * SB);
+          // A NaN of the sequence must not reach the rows that do not see its
+          // token: it is taken out of the stage, and put into O's block of the
+          // rows that do see it.
           bool any = false;
 #pragma unroll
           for (int i = 0; i < SB / 4; ++i) any = any || nan_bytes(sb[i]) != 0;
@@ -769,9 +811,9 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
           const uint32_t f0 = e4m3x2_to_half2(w0), f1 = e4m3x2_to_half2(w1);
           // even codes of both tokens in one word, odd codes in another
           uint32_t e0[4], o0[4], e1[4], o1[4];
-          e2m1x8_to_half2x4((v[0][wi] & 0x0F0F0F0Fu) | ((v[1][wi] << 4) & 0xF0F0F0F0u), e0);
+          e2m1x8_to_half2x4((v[0][wi] & 0x0F0F0F0Fu) | (times16(v[1][wi]) & 0xF0F0F0F0u), e0);
           e2m1x8_to_half2x4(((v[0][wi] >> 4) & 0x0F0F0F0Fu) | (v[1][wi] & 0xF0F0F0F0u), o0);
-          e2m1x8_to_half2x4((v[2][wi] & 0x0F0F0F0Fu) | ((v[3][wi] << 4) & 0xF0F0F0F0u), e1);
+          e2m1x8_to_half2x4((v[2][wi] & 0x0F0F0F0Fu) | (times16(v[3][wi]) & 0xF0F0F0F0u), e1);
           e2m1x8_to_half2x4(((v[2][wi] >> 4) & 0x0F0F0F0Fu) | (v[3][wi] & 0xF0F0F0F0u), o1);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -790,7 +832,6 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       if (more) {
         copy_stage(o2, at);
         o2 += 2;
-        pc_tok += step;
       }
       copy_commit();  // one group a stage, empty ones too, so that the count of groups stays fixed
       at = at == (G::kStages - 1) * G::kStageBytes ? 0 : at + G::kStageBytes;
