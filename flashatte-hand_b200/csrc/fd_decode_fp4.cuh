@@ -72,6 +72,7 @@ namespace {
 constexpr int kFp4Threads = 128;
 constexpr int kFp4Warps = kFp4Threads / 32;
 constexpr int kSubTokens = 32;  // tokens of a stage
+constexpr int kOffEntries = 34; // 16 stages' offsets, and a stage of none
 constexpr int kSegRing = 8;     // segments that the loads may be ahead
 static_assert(kTileTokens == kFp4Warps * kSubTokens, "a schedule tile is a stage of each warp");
 
@@ -89,8 +90,8 @@ template <int D, int NT> struct Fp4Geo {
   static constexpr int kJoinWarp = kRows * kRowPad * 4 + kRows * 2 * 4;  // O, then maximum and sum of each row
   // the ring; what a warp's lanes share of its loads (page offsets of 16
   // stages, segments ahead); the join; lengths
-  static constexpr int kOffOffs = kFp4Warps * kStages * kStageBytes;     // [warps][32] code and scale offsets
-  static constexpr int kOffSegs = kOffOffs + kFp4Warps * 32 * 16;        // [warps][kSegRing]
+  static constexpr int kOffOffs = kFp4Warps * kStages * kStageBytes;     // [warps][kOffEntries] code and scale offsets
+  static constexpr int kOffSegs = kOffOffs + kFp4Warps * kOffEntries * 16;        // [warps][kSegRing]
   static constexpr int kOffJoin = kOffSegs + kFp4Warps * kSegRing * 32;  // [kFp4Warps - 1]
   static constexpr int kOffMisc = kOffJoin + (kFp4Warps - 1) * kJoinWarp;
   static constexpr int kOffPrefix = kOffMisc + 32;
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   const int r = lane >> 2, c = lane & 3;
 
   uint8_t* ring = smem + warp * G::kStages * G::kStageBytes;
-  longlong2* offs = reinterpret_cast<longlong2*>(smem + G::kOffOffs) + warp * 32;
+  longlong2* offs = reinterpret_cast<longlong2*>(smem + G::kOffOffs) + warp * kOffEntries;
   int4* seg_ring = reinterpret_cast<int4*>(smem + G::kOffSegs) + warp * kSegRing * 2;
   unsigned long long* launch_epoch = reinterpret_cast<unsigned long long*>(smem + G::kOffMisc);
   volatile int* last_flag = reinterpret_cast<volatile int*>(smem + G::kOffMisc + 8);  // [2]
@@ -457,6 +458,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       if constexpr (kScaleCopies == 2) copy16_or_zeros(scale_dst + at + G::kTileScales, src + (p.v_block - p.k_block), any);
     }
   };
+  if (lane < 2) offs[32 + lane] = make_longlong2(0, 0);
   {
     const Schedule sched = schedule();
     Segment g;
@@ -611,7 +613,8 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
         const int turn = 16 - (pc_k & 15), calm = pc_left < turn ? pc_left : turn;
         n = n < calm ? n : calm;
       }
-      const longlong2* o2 = offs + (pc_k & 15) * 2;
+      const longlong2* o2 = offs + (more ? (pc_k & 15) * 2 : 32);
+      const int o2_step = more ? 2 : 0;
 #pragma unroll 1
       for (const int stop = k + n; k < stop; ++k) {
       if (k >= 0) {
@@ -674,7 +677,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       }
 
       // ---- softmax over the warp's 32 tokens (log2 domain)
-      if (t0 + kSubTokens > all_seen) {  // some row does not see some token
+      if (__any_sync(0xffffffffu, t0 + kSubTokens > all_seen)) {  // some row does not see some token
         const int len = volatile_at(entry(seg_r) + 1).x / HW, base = MULTI ? place().row_base : 0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -829,10 +832,8 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       }
       // ---- refill the stage
       __syncwarp();  // every lane has read it
-      if (more) {
-        copy_stage(o2, at);
-        o2 += 2;
-      }
+      copy_stage(o2, at);
+      o2 += o2_step;
       copy_commit();  // one group a stage, empty ones too, so that the count of groups stays fixed
       at = at == (G::kStages - 1) * G::kStageBytes ? 0 : at + G::kStageBytes;
       }
