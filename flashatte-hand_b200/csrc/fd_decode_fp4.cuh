@@ -203,11 +203,6 @@ template <> __device__ __forceinline__ float2 pair_to_float2<__half>(uint32_t w)
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-template <typename O> __device__ __forceinline__ O fp4_out(float x);
-template <> __device__ __forceinline__ float fp4_out<float>(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 fp4_out<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <> __device__ __forceinline__ __half fp4_out<__half>(float x) { return __float2half_rn(x); }
-
 // N words (1, 2, 4 or 8) from shared memory in the widest loads.
 template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
   if constexpr (N == 1) {
@@ -244,6 +239,29 @@ template <typename O, int N> __device__ __forceinline__ void store_row(O* dst, c
       *reinterpret_cast<uint4*>(dst + i) =
           make_uint4(pack_out<O>(x[i], x[i + 1]), pack_out<O>(x[i + 2], x[i + 3]), pack_out<O>(x[i + 4], x[i + 5]),
                      pack_out<O>(x[i + 6], x[i + 7]));
+  }
+}
+
+// N = 2 or 4 consecutive values, as wide as they are: partials past L1, and
+// the output, rounded once.
+template <int N> __device__ __forceinline__ void load_vec(const float* src, float (&x)[N]) {
+  if constexpr (N == 4) {
+    const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
+    x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+  } else {
+    static_assert(N == 2, "2 or 4 values");
+    const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
+    x[0] = y.x; x[1] = y.y;
+  }
+}
+template <typename O, int N> __device__ __forceinline__ void store_vec(O* dst, const float (&x)[N]) {
+  if constexpr (sizeof(O) == 4) {
+    if constexpr (N == 4) *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+    else *reinterpret_cast<float2*>(dst) = make_float2(x[0], x[1]);
+  } else {
+    if constexpr (N == 4)
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_out<O>(x[0], x[1]), pack_out<O>(x[2], x[3]));
+    else *reinterpret_cast<uint32_t*>(dst) = pack_out<O>(x[0], x[1]);
   }
 }
 
@@ -978,19 +996,21 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       }
       last = __shfl_sync(0xffffffffu, last, 0);
     }
-    // with more rows than one round takes, the head's other warps take a share
-    const int ways = nrows > kAt ? TW : 1;
-    if (ways > 1) {
+    // With more rows or partials than one round takes, the head's other warps
+    // take a share: of the rows, or else of the partials.
+    const int row_ways = nrows > kAt ? TW : 1;
+    const int part_ways = row_ways == 1 && nseg > kAt ? TW : 1;
+    if (row_ways * part_ways > 1) {
       if (tw == 0 && lane == 0) last_flag[hw] = last;
       __syncthreads();
       last = last_flag[hw];
       __syncthreads();
     }
-    if (!last) continue;  // (warps tw > 0 that have no share, too)
+    if (!last && part_ways == 1) continue;  // (warps tw > 0 that have no share, too)
     __threadfence();
     // The last of the pair's segments joins them: partial j of the head is
     // part (cfirst + j + pair) * HW + hw.  A round is kAt partials of kAt rows
-    // (of the warp's rows tw, tw + ways, ..), all their loads in flight: lane
+    // (of the warp's rows, partials), all their loads in flight: lane
     // kAt v + u holds the weight of partial u of row v, relative to a running
     // maximum.  Short code on purpose: it runs once, and cold instructions
     // cost more than the loads (16 partials unrolled took 2 to 10 us longer).
@@ -998,8 +1018,9 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     const int64_t lse_step = static_cast<int64_t>(HW) * rows;
     constexpr int kVec = D >= 128 ? 4 : 2, kPieces = D / (32 * kVec);
     const int lu = lane & (kAt - 1), lv = lane / kAt;
+    const int row_tw = row_ways > 1 ? tw : 0, part_tw = part_ways > 1 ? tw : 0;
 #pragma unroll 1
-    for (int row0 = tw; row0 < nrows; row0 += kAt * ways) {
+    for (int row0 = row_tw; row0 < nrows; row0 += kAt * row_ways) {
       float mm = neg_inf, den = 0.f;  // of row lv
       float o[kAt][kPieces][kVec];
 #pragma unroll
@@ -1009,28 +1030,19 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
 #pragma unroll
           for (int i = 0; i < kVec; ++i) o[v][q][i] = 0.f;
 #pragma unroll 1
-      for (int j0 = 0; j0 < nseg; j0 += kAt) {
+      for (int j0 = part_tw * kAt; last && j0 < nseg; j0 += kAt * part_ways) {
         const int64_t at_row = first * rows + row0 + j0 * lse_step;
-        const bool mine = lv < kAt && row0 + lv * ways < nrows && j0 + lu < nseg;
-        const float lj = mine ? __ldcg(p.part_lse + at_row + lv * ways + lu * lse_step) : neg_inf;
+        const bool mine = lv < kAt && row0 + lv * row_ways < nrows && j0 + lu < nseg;
+        const float lj = mine ? __ldcg(p.part_lse + at_row + lv * row_ways + lu * lse_step) : neg_inf;
         float x[kAt][kAt][kPieces][kVec];
         const float* src = p.part_o + at_row * D + lane * kVec;
 #pragma unroll
         for (int u = 0; u < kAt; ++u) {
 #pragma unroll
           for (int v = 0; v < kAt; ++v) {
-            if (j0 + u < nseg && row0 + v * ways < nrows) {
+            if (j0 + u < nseg && row0 + v * row_ways < nrows) {
 #pragma unroll
-              for (int q = 0; q < kPieces; ++q) {
-                const float* at_v = src + v * ways * D + q * 32 * kVec;
-                if constexpr (kVec == 4) {
-                  const float4 y = __ldcg(reinterpret_cast<const float4*>(at_v));
-                  x[v][u][q][0] = y.x; x[v][u][q][1] = y.y; x[v][u][q][2] = y.z; x[v][u][q][3] = y.w;
-                } else {
-                  const float2 y = __ldcg(reinterpret_cast<const float2*>(at_v));
-                  x[v][u][q][0] = y.x; x[v][u][q][1] = y.y;
-                }
-              }
+              for (int q = 0; q < kPieces; ++q) load_vec(src + v * row_ways * D + q * 32 * kVec, x[v][u][q]);
             }
           }
           src += lse_step * D;
@@ -1062,19 +1074,57 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
           }
         }
       }
+      if (part_ways > 1) {  // one round of rows: what the other warps joined goes to the first
+        float* buf = reinterpret_cast<float*>(smem + G::kOffJoin + (warp - HW) * G::kJoinWarp);
+        if (tw > 0 && last) {
+          float* ml = buf + G::kRows * G::kRowPad;
+          if (lv < kAt && lu == 0) ml[2 * lv] = mm, ml[2 * lv + 1] = den;
+#pragma unroll
+          for (int v = 0; v < kAt; ++v)
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+              for (int i = 0; i < kVec; ++i) buf[v * G::kRowPad + (q * 32 + lane) * kVec + i] = o[v][q][i];
+        }
+        __syncthreads();
+        if (tw == 0 && last) {
+#pragma unroll 1
+          for (int u = 1; u < TW; ++u) {
+            const float* from = reinterpret_cast<const float*>(smem + G::kOffJoin + (warp + (u - 1) * HW) * G::kJoinWarp);
+            const float* ml = from + G::kRows * G::kRowPad + 2 * (lv < kAt ? lv : 0);
+            const float m_new = fmaxf(mm, ml[0]);
+            const float fa = mm == m_new ? 1.f : fast_exp2(mm - m_new), fb = ml[0] == m_new ? 1.f : fast_exp2(ml[0] - m_new);
+            mm = m_new;
+            den = fmaf(den, fa, ml[1] * fb);
+#pragma unroll
+            for (int v = 0; v < kAt; ++v) {
+              const float av = __shfl_sync(0xffffffffu, fa, v * kAt), bv = __shfl_sync(0xffffffffu, fb, v * kAt);
+#pragma unroll
+              for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+                for (int i = 0; i < kVec; ++i)
+                  o[v][q][i] = fmaf(o[v][q][i], av, from[v * G::kRowPad + (q * 32 + lane) * kVec + i] * bv);
+            }
+          }
+        }
+        __syncthreads();  // the buffers are free again
+        if (tw > 0 || !last) break;
+      }
       const bool some = !(den == 0.f);
       const float inv = some ? 1.f / den : 0.f;
-      if (lv < kAt && lu == 0 && row0 + lv * ways < nrows)
-        put_lse(row0 + lv * ways, some ? mm + fast_log2(den) : neg_inf);
+      if (lv < kAt && lu == 0 && row0 + lv * row_ways < nrows)
+        put_lse(row0 + lv * row_ways, some ? mm + fast_log2(den) : neg_inf);
 #pragma unroll
       for (int v = 0; v < kAt; ++v) {
         const float iv = __shfl_sync(0xffffffffu, inv, v * kAt);
-        if (row0 + v * ways >= nrows) continue;
-        OutT* dst = out_at(row0 + v * ways) + lane * kVec;
+        if (row0 + v * row_ways >= nrows) continue;
+        OutT* dst = out_at(row0 + v * row_ways) + lane * kVec;
 #pragma unroll
-        for (int q = 0; q < kPieces; ++q)
+        for (int q = 0; q < kPieces; ++q) {
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) dst[q * 32 * kVec + i] = fp4_out<OutT>(o[v][q][i] * iv);
+          for (int i = 0; i < kVec; ++i) o[v][q][i] *= iv;
+          store_vec(dst + q * 32 * kVec, o[v][q]);
+        }
       }
     }
   }
