@@ -19,23 +19,18 @@ constexpr int kMaxDevices = 64;
 
 // Split cost model of the 4-bit cache (units and meaning as in fd_api.cu: a
 // tile, 128 tokens of one head or 64 of two, costs 8 and a bit).  A pair costs
-// its CTA about 4 us beside its tiles (query, joining, partials, arrival), four
-// tiles' time.  Charged in full it balances launches with more pairs than CTAs
-// (config 3: 142 us at 30, 131 us at 45); with fewer pairs it mostly makes the
-// ranges, which must be longer than a pair's share, too coarse (4 speculated
-// tokens of 32 sequences: 47 us at 30, 50 us at 45).
+// its CTA about 5 us beside its tiles (query, joining, partials, arrival), five
+// tiles' time.  From 45 to 60 it makes little difference; config 3 takes 126 us
+// at 30, 115 at 52 and 119 at 90, 4 speculated tokens of 32 sequences 43.6,
+// 40.6 and 41.6 us.
 constexpr int kCostTile4 = 2;
-constexpr int kCostSeg4 = 30;
-constexpr int kCostSegMany4 = 45;
-// Short launches take whole pairs where no CTA gets more than 12 tiles: eight
-// 1k-token sequences 19.8 -> 16.0 us, but config 1 (16 tiles) 19.8 -> 21.5.
+constexpr int kCostSeg4 = 52;
+// Short launches take whole pairs where no CTA gets more than 12 tiles: 64
+// sequences of up to 600 tokens 22.9 -> 22.0 us, eight 1k-token sequences alike,
+// but config 1 (16 tiles) 15.7 -> 20.5.
 constexpr int kAlignTiles4 = 12;
 int cost_tile4() { static const int v = fd::env_int("FD_COST_TILE4", kCostTile4, 0, 64); return v; }
-int cost_seg4(bool many) {
-  static const int few = fd::env_int("FD_COST_SEG4", kCostSeg4, 1, 256);
-  static const int lot = fd::env_int("FD_COST_SEG4", kCostSegMany4, 1, 256);
-  return many ? lot : few;
-}
+int cost_seg4() { static const int v = fd::env_int("FD_COST_SEG4", kCostSeg4, 1, 256); return v; }
 int align_tiles4() { static const int v = fd::env_int("FD_ALIGN_TILES4", kAlignTiles4, 0, 4096); return v; }
 
 // A partial for every (sequence, KV head, row tile), and for every KV head of
@@ -394,7 +389,7 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
   const int64_t len_bound = max_seqlen_k > 0 && max_seqlen_k < kv_max ? max_seqlen_k : kv_max;
   // the schedule's tiles are kTileTokens / heads tokens of `heads` heads
   const int64_t tiles_bound = (len_bound * heads + fd::kTileTokens - 1) / fd::kTileTokens;
-  const int lead = cost_seg4(batch_size * vheads >= grid_max);
+  const int lead = cost_seg4();
   const int64_t per_seq_cost = lead + ((kv_max * heads + fd::kTileTokens - 1) / fd::kTileTokens + 1) *
                                                  (8 + static_cast<int64_t>(cost_tile4()));
   const int64_t aligned_cost = lead + static_cast<int64_t>(align_tiles4()) * (8 + cost_tile4()) + 1;

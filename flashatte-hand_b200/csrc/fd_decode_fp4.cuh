@@ -368,13 +368,14 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     x.batch = p.batch;
     x.hkv = p.num_heads_k / HW * p.row_tiles;
     x.cm = CostModel{p.cost_tile, p.cost_seg, p.cost_floor};
+    x.behind_lead = true;
     x.align_m = volatile_at(align_word);
     x.align_cost = x.cm.max_lead() + p.align_tiles * x.cm.full() + 1;
     if (x.align_m > 0) {
       x.grid = (x.batch * x.hkv + x.align_m - 1) / x.align_m;
     } else {
-      // every range longer than the costliest tile: none inside a pair is empty
-      const int64_t g = div_u32(x.total, x.cm.max_lead() + x.cm.full() + 1);
+      // every range longer than a tile: none inside a pair is empty
+      const int64_t g = div_u32(x.total, x.cm.full() + 1);
       x.grid = static_cast<int>(g < 1 ? 1 : (g < gridDim.x ? g : gridDim.x));
     }
     return x;

@@ -114,6 +114,10 @@ struct Schedule {
   int align_m;
   int64_t align_cost;
   CostModel cm;
+  // Where tile 0 starts: at the pair's start, or behind its lead like every
+  // other.  In the second form a range that ends inside a lead leaves the whole
+  // pair to the next CTA, in the first it takes a segment of that one tile.
+  bool behind_lead = false;
 
   __device__ __forceinline__ int len_of(int b) const { return lens[b]; }
   __device__ __forceinline__ int64_t range_start(int c) const {
@@ -136,7 +140,7 @@ struct Schedule {
   }
   // start of tile j of the pair that starts at cp and has lead `lead`
   __device__ __forceinline__ int64_t tile_start(int64_t cp, int lead, int j) const {
-    return j == 0 ? cp : cp + lead + static_cast<int64_t>(j) * cm.full();
+    return j == 0 && !behind_lead ? cp : cp + lead + static_cast<int64_t>(j) * cm.full();
   }
   // Segment of `pair` from tile j0 on, cut at range end e1; false if no tile
   // of the pair at or after j0 starts before e1.  Integer work here is 32-bit
@@ -166,7 +170,7 @@ struct Schedule {
       s.nseg = 1;
       s.cfirst = -1;
     } else {
-      s.cfirst = cta_of(cp);
+      s.cfirst = cta_of(tile_start(cp, lead, 0));
       s.nseg = cta_of(tile_start(cp, lead, n - 1)) - s.cfirst + 1;
     }
     return true;
@@ -188,8 +192,8 @@ struct Schedule {
     int j0 = 0;
     if (e0 > cp) {
       const int64_t x = e0 - cp - cm.lead(len_of(lo));
-      j0 = static_cast<int>(x > 0 ? ceil_div_u32(x, cm.full()) : 1);
-      if (j0 < 1) j0 = 1;
+      j0 = static_cast<int>(x > 0 ? ceil_div_u32(x, cm.full()) : 0);
+      if (j0 < 1 && !behind_lead) j0 = 1;
     }
     if (make(pair, j0, e1, s)) return true;
     return pair + 1 < batch * hkv && make(pair + 1, 0, e1, s);
