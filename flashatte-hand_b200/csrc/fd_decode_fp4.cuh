@@ -35,24 +35,40 @@
 // and the byte of its neighbour give the pairs (t, t + 1) that the fragment
 // wants.  P^T comes from S^T by movmatrix.  The tokens of a tile are numbered
 // so that rows of both parities meet in a quarter-warp (tau below): with the
-// TMA swizzle K's and V's loads are free of bank conflicts at D = 128, 256.
+// swizzle of the rings K's and V's loads are free of bank conflicts.
 //
 // Loads.  A row of codes is D / 2 = 64 bytes at a stride of Hkv * 64: a TMA
 // box of such rows was measured to move one row in about 5 cycles of the SM
 // (4.0 TB/s in all at D = 128, 1.8 TB/s with the 32-byte rows of D = 64,
 // however many boxes were in flight, from L2 as from HBM).  So the lanes copy
-// 16 bytes each with cp.async, eight rows an instruction, past L1.
+// 16 bytes each with cp.async, eight rows an instruction, past L1: 6.5 to 6.8
+// TB/s for the loads alone.
 //
 // A CTA is four warps, and a schedule tile four 32-token stages, one a warp:
 // HW = 2 neighbouring KV heads of the same tokens (1 where their number is odd,
 // and in short launches), so that the warps together read 128-byte runs (one
-// head a CTA cost 1.27 times the DRAM traffic), times 4 / HW stages along the
-// sequence.  Each warp has a ring and a softmax state of its own,
-// and nothing in the loop waits for another warp.  The ring runs across
-// segments (a segment is the CTA's part of a sequence's heads): the next
-// one's first loads are in flight while this one is written out.  Work split
-// and the joining of segments on different CTAs are those of
+// head a CTA costs 1.27 times the DRAM traffic, 107 instead of 68 us on config
+// 2), times 4 / HW stages along the sequence.  Each warp has a ring and a
+// softmax state of its own, and nothing in the loop waits for another warp.
+// The ring runs across segments (a segment is the CTA's part of a sequence's
+// heads): the next one's first loads are in flight while this one is written
+// out.  Work split and the joining of segments on different CTAs are those of
 // fd_decode_sm100.cuh, a head of a segment at a time.
+//
+// What bounds it.  32 tokens of K and V of a head at D = 128 are 4.6 KB, 765
+// cycles of a quarter SM's share of the HBM, and 499 instructions of a warp:
+// 128 conversions of code pairs and 84 other ones on the half-rate ALU, 128
+// half-rate f16 multiplications, 32 mma, 38 loads and stores.  Two warps a
+// scheduler overlap these to 1.1 to 1.2 times the HBM's time; three (3 CTAs an
+// SM, 168 registers) were 10 to 17 % slower, with more segments for each.  So
+// the loop is written for few instructions (the half-rate ones most of all):
+// every five ALU instructions of it are a percent.
+//
+// Measured on a B200 (back-to-back launches; 6.56 TB/s is its copy rate): 64
+// sequences of 4096 tokens, 32 over 8 heads, D = 128: 68.5 us, 4.4 TB/s; two
+// of 131072: 117 us, 5.2 TB/s; the fixed part of a launch is 16 us (first data
+// after 6.5 us: schedule 1.5, first page ids 1.9, query 1.3, data 1.8; 2 to 3
+// us for a segment's end, 1.5 to 5 for a joining, the rest imbalance).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -83,9 +99,11 @@ template <int D, int NT> struct Fp4Geo {
   static constexpr int kTileScales = kSubTokens * kScaleBytes;
   static constexpr int kStageBytes = 2 * kTileBytes + 2 * kTileScales;
   static constexpr int kRows = 8 * NT;
-  // CTAs per SM, and stages that fit beside them
+  // CTAs per SM (D = 64: 50.5 us for 64 sequences of 4096 tokens, 52.6 with 2),
+  // and stages of a ring: enough for the HBM's latency; 4 at D = 128 and 5 at
+  // D = 64 were within 1 % and not better
   static constexpr int kCtas = D == 64 ? 3 : 2;
-  static constexpr int kStages = D == 64 ? 5 : D == 128 ? 4 : 2;
+  static constexpr int kStages = D == 64 ? 4 : D == 128 ? 3 : 2;
   static constexpr int kRowPad = D + 4;  // floats of a row of the join buffer
   static constexpr int kJoinWarp = kRows * kRowPad * 4 + kRows * 2 * 4;  // O, then maximum and sum of each row
   // the ring; what a warp's lanes share of its loads (page offsets of 16
@@ -153,6 +171,8 @@ __device__ __forceinline__ const uint8_t* plus_multiple(const uint8_t* p, uint32
   return reinterpret_cast<const uint8_t*>(d);
 }
 
+// (v's low half, twice), (its high half, twice): written like this the compiler
+// makes them operand selections of the multiplication, no instructions.
 __device__ __forceinline__ uint32_t low_twice(uint32_t v) {
   uint32_t d;
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tmov.b32 %0, {lo, lo};\n\t}" : "=r"(d) : "r"(v));
@@ -163,6 +183,7 @@ __device__ __forceinline__ uint32_t high_twice(uint32_t v) {
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tmov.b32 %0, {hi, hi};\n\t}" : "=r"(d) : "r"(v));
   return d;
 }
+// A shift by 4 that stays a multiplication, off the ALU.
 __device__ __forceinline__ uint32_t times16(uint32_t v) {
   uint32_t d;
   asm("mad.lo.u32 %0, %1, 16, 0;" : "=r"(d) : "r"(v));
@@ -384,11 +405,12 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   // ------------------------------------------------------------ loads
   // The cursor of the loads, a ring ahead of the multiplication: pc_left
   // tiles of the segment entered last (seg_ring[seg_w - 1]) are left, the
-  // next is its pc_k-th.  offs[2 i + g] are the byte offsets
-  // (codes; block scales) of tokens 16 g .. of the warp's stage 16 n + i of
-  // the segment, plus 16, the bytes that a lane copies from there - or 0 and
-  // so no bytes where there is no page; next_* the page id and row (-1: no
-  // tokens) of the same entry of batch n + 1.
+  // next is its pc_k-th.  offs[2 i + g] are the byte offsets (codes; block
+  // scales) of tokens 16 g .. of the warp's stage 16 n + i of the segment, plus
+  // 16, or 0 where there is no page: no codes are copied then, and zeros as
+  // scales; next_* the page id and row (-1: no tokens) of the same entry of
+  // batch n + 1.  offs[32 .. 33] are a stage of none, for the rounds after the
+  // last.
   int pc_left = 0, pc_end = 0, pc_k = 0, next_id = 0, next_row = -1, seg_w = 0;
   // A copy instruction moves 16 bytes a lane: half the lanes rows of K, half
   // of V, so that a lane needs one pointer; kCopies of them are 16 tokens.
@@ -482,7 +504,8 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       const int any = static_cast<int>(off) & 16;
       const uint8_t* src = scale_src + off;
       copy16_or_zeros(scale_dst + at, src, any);
-      if constexpr (kScaleCopies == 2) copy16_or_zeros(scale_dst + at + G::kTileScales, src + (p.v_block - p.k_block), any);
+      if constexpr (kScaleCopies == 2)
+        copy16_or_zeros(scale_dst + at + G::kTileScales, src + (p.v_block - p.k_block), any);
     }
   };
   if (lane < 2) offs[32 + lane] = make_longlong2(0, 0);
@@ -545,69 +568,69 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     uint32_t qf[NT][KS][2];
     float qfac[NT][2];  // per column of the lane (query rows 2 c, 2 c + 1 of each 8)
     {
-    const Place pl = place();
-    const int b = pl.b, kvh = pl.kvh, row_base = pl.row_base, nrows = pl.nrows;
-    const float factor = __ldg(p.k_scale + kvh) * p.scale_log2;
-    const float sign = factor > 0.f ? 1.f : (factor < 0.f ? -1.f : factor);
-    float row_inv[NT];  // 2^-k of the row's scaling
+      const Place pl = place();
+      const int b = pl.b, kvh = pl.kvh, row_base = pl.row_base, nrows = pl.nrows;
+      const float factor = __ldg(p.k_scale + kvh) * p.scale_log2;
+      const float sign = factor > 0.f ? 1.f : (factor < 0.f ? -1.f : factor);
+      float row_inv[NT];  // 2^-k of the row's scaling
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int n = nt * 8 + r;
-      row_inv[nt] = 1.f;
-      uint4 raw[D / 32];
-      if (n < nrows) {
-        const int h = row_base + n, qi = MULTI ? h / p.group : 0, g = h - qi * p.group;
-        const uint4* src = reinterpret_cast<const uint4*>(
-            static_cast<const T*>(p.q) +
-            ((static_cast<int64_t>(b) * p.seqlen_q + qi) * p.num_heads + kvh * p.group + g) * D + c * (D / 4));
+      for (int nt = 0; nt < NT; ++nt) {
+        const int n = nt * 8 + r;
+        row_inv[nt] = 1.f;
+        uint4 raw[D / 32];
+        if (n < nrows) {
+          const int h = row_base + n, qi = MULTI ? h / p.group : 0, g = h - qi * p.group;
+          const uint4* src = reinterpret_cast<const uint4*>(
+              static_cast<const T*>(p.q) +
+              ((static_cast<int64_t>(b) * p.seqlen_q + qi) * p.num_heads + kvh * p.group + g) * D + c * (D / 4));
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) raw[i] = __ldg(src + i);
-      } else {
+          for (int i = 0; i < D / 32; ++i) raw[i] = __ldg(src + i);
+        } else {
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) raw[i] = make_uint4(0, 0, 0, 0);
-      }
-      float sc = sign;
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        float mx = 0.f;
+          for (int i = 0; i < D / 32; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+        }
+        float sc = sign;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          float mx = 0.f;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = pair_to_float2<T>(x[j]);
+              mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          if (mx > 0.f && mx <= 3.4e38f) {
+            int k = 13 - (((__float_as_int(mx) >> 23) & 0xff) - 127);
+            k = k > 126 ? 126 : (k < -126 ? -126 : k);
+            sc = __int_as_float((k + 127) << 23) * sign;
+            row_inv[nt] = __int_as_float((127 - k) << 23);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
           const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float2 f = pair_to_float2<T>(x[j]);
-            mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+            uint32_t h = x[j];
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+              const float2 f = pair_to_float2<T>(x[j]);
+              h = pack_half2(f.x * sc, f.y * sc);
+            } else {
+              h = hmul2_bits(h, pack_half2(sc, sc));
+            }
+            qf[nt][2 * i + (j >> 1)][j & 1] = h;  // step s: values 4 s .. 4 s + 3 of the lane's
           }
         }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        if (mx > 0.f && mx <= 3.4e38f) {
-          int k = 13 - (((__float_as_int(mx) >> 23) & 0xff) - 127);
-          k = k > 126 ? 126 : (k < -126 ? -126 : k);
-          sc = __int_as_float((k + 127) << 23) * sign;
-          row_inv[nt] = __int_as_float((127 - k) << 23);
-        }
       }
+      const float f = factor == 0.f ? 1.f : fabsf(factor);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t h = x[j];
-          if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-            const float2 f = pair_to_float2<T>(x[j]);
-            h = pack_half2(f.x * sc, f.y * sc);
-          } else {
-            h = hmul2_bits(h, pack_half2(sc, sc));
-          }
-          qf[nt][2 * i + (j >> 1)][j & 1] = h;  // step s: values 4 s .. 4 s + 3 of the lane's
-        }
-      }
-    }
-    const float f = factor == 0.f ? 1.f : fabsf(factor);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) qfac[nt][e] = f * __shfl_sync(0xffffffffu, row_inv[nt], (2 * c + e) * 4);
+        for (int e = 0; e < 2; ++e) qfac[nt][e] = f * __shfl_sync(0xffffffffu, row_inv[nt], (2 * c + e) * 4);
     }
     const int all_seen = seqlen - ((MULTI && p.causal) ? p.seqlen_q - 1 : 0);  // keys that every row sees
 
@@ -644,225 +667,225 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       const int o2_step = more ? 2 : 0;
 #pragma unroll 1
       for (const int stop = k + n; k < stop; ++k) {
-      if (k >= 0) {
-      copy_wait<G::kStages - 1>();
-      __syncwarp();  // every lane's copies of the stage have landed
-      const uint8_t* st = ring + at;
+        if (k >= 0) {
+          copy_wait<G::kStages - 1>();
+          __syncwarp();  // every lane's copies of the stage have landed
+          const uint8_t* st = ring + at;
 
-      // ---- S^T = K . Q^T, two tiles of 16 tokens side by side
-      float s[2][NT][4];
-      uint32_t kw[2][2][KW];               // [tile][rows r, r + 8]: the lane's codes
-      uint32_t kf[2][2][(D + 127) / 128];  // and the f16 pairs of their block scales
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int row = mt * 16 + half * 8;
-          const uint8_t* sc = st + ks_at + row * SB;
-          if constexpr (D == 256) {
-            uint32_t x[4], y[4];
-            load_words<4>(st + k_at + row * RB, x);
-            load_words<4>(st + k_at2 + row * RB, y);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { kw[mt][half][i] = x[i]; kw[mt][half][4 + i] = y[i]; }
-            const uint32_t q = *reinterpret_cast<const uint32_t*>(sc);
-            kf[mt][half][0] = e4m3x2_to_half2(q);
-            kf[mt][half][1] = e4m3x2_to_half2(q >> 16);
-          } else if constexpr (D == 128) {
-            load_words<4>(st + k_at + row * RB, kw[mt][half]);
-            kf[mt][half][0] = e4m3x2_to_half2(*reinterpret_cast<const uint16_t*>(sc));
-          } else {
-            load_words<2>(st + k_at + row * RB, kw[mt][half]);
-            kf[mt][half][0] = e4m3x2_to_half2(*sc);
-          }
-        }
-      }
-#pragma unroll
-      for (int wi = 0; wi < KW; ++wi) {
-        const int blk = wi / 2;  // two words a block
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          uint32_t h[2][4];
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t pair = kf[mt][half][blk / 2];
-            const uint32_t f = blk & 1 ? high_twice(pair) : low_twice(pair);
-            e2m1x8_to_half2x4(kw[mt][half][wi], h[half]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) h[half][j] = hmul2_bits(h[half][j], f);
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(s[mt][nt], h[0][0], h[1][0], h[0][1], h[1][1], qf[nt][2 * wi][0], qf[nt][2 * wi][1]);
-            mma_f16(s[mt][nt], h[0][2], h[1][2], h[0][3], h[1][3], qf[nt][2 * wi + 1][0], qf[nt][2 * wi + 1][1]);
-          }
-        }
-      }
-
-      // ---- softmax over the warp's 32 tokens (log2 domain)
-      if (__any_sync(0xffffffffu, t0 + kSubTokens > all_seen)) {  // some row does not see some token
-        const int len = volatile_at(entry(seg_r) + 1).x / HW, base = MULTI ? place().row_base : 0;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            // causal: row (qi, g) sees the keys up to its own position
-            const int seen =
-                len + ((MULTI && p.causal) ? (base + nt * 8 + 2 * c + e) / p.group - (p.seqlen_q - 1) : 0);
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-              if (t0 + mt * 16 + tau >= seen) s[mt][nt][e] = neg_inf;
-              if (t0 + mt * 16 + tau + 8 >= seen) s[mt][nt][e + 2] = neg_inf;
-            }
-          }
-        // Block scales of V must not be NaN where P is 0.  Behind the sequence's
-        // end they are what memory held: cleared.
-        uint32_t* sb = reinterpret_cast<uint32_t*>(ring + at + 2 * G::kTileBytes + G::kTileScales + lane * SB);
-        if (t0 + lane >= len) {
-#pragma unroll
-          for (int i = 0; i < SB / 4; ++i) sb[i] = 0;
-        }
-        __syncwarp();
-        if constexpr (MULTI) {
-          // A NaN of the sequence must not reach the rows that do not see its
-          // token: it is taken out of the stage, and put into O's block of the
-          // rows that do see it.
-          bool any = false;
-#pragma unroll
-          for (int i = 0; i < SB / 4; ++i) any = any || nan_bytes(sb[i]) != 0;
-          unsigned tokens = __ballot_sync(0xffffffffu, any);
-          if (tokens != 0) {
-#pragma unroll 1
-            for (; tokens != 0; tokens &= tokens - 1) {
-              const int u = __ffs(tokens) - 1;
-              const uint8_t* row = st + 2 * G::kTileBytes + G::kTileScales + u * SB + r * (D / 8) / 16;
-#pragma unroll
-              for (int j = 0; j < (D + 127) / 128; ++j) {  // the lane's blocks, of MT / that many tiles each
-                constexpr int kPer = MT / ((D + 127) / 128);
-                if (nan_bytes(row[j]) == 0) continue;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e) {
-                    const int seen =
-                        len + (p.causal ? (base + nt * 8 + 2 * c + e) / p.group - (p.seqlen_q - 1) : 0);
-                    if (t0 + u >= seen) continue;
-#pragma unroll
-                    for (int i = j * kPer; i < (j + 1) * kPer; ++i)
-                      acc[i][nt][e] = acc[i][nt][e + 2] = __int_as_float(0x7fffffff);
-                  }
-              }
-            }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < SB / 4; ++i) sb[i] &= ~nan_bytes(sb[i]);
-            __syncwarp();
-          }
-        }
-      }
-      // The reference of the exponents need not be the maximum: it is raised
-      // (and O, l rescaled) only when a logit exceeds it by more than 8, so
-      // that P stays below 2^8, well inside f16, and most stages need no
-      // reduction over the tokens' lanes.  Rounded up, it bounds the exact
-      // products that the exponents subtract it from, however large.
-      bool above = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float mx = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
-          above = above || __fmul_ru(mx, qfac[nt][e]) - m[nt][e] > 8.f;
-        }
-      if (__any_sync(0xffffffffu, above)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float m_new = fmaxf(m[nt][e], __fmul_ru(mx, qfac[nt][e]));
-            const float alpha = m_new == m[nt][e] ? 1.f : fast_exp2(m[nt][e] - m_new);
-            m[nt][e] = m_new;
-            m_use[nt][e] = m_new == neg_inf ? 0.f : m_new;
-            l[nt][e] *= alpha;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              acc[i][nt][e] *= alpha;
-              acc[i][nt][e + 2] *= alpha;
-            }
-          }
-      }
-      uint32_t pt[2][NT][2];  // P^T fragments of each 16 tokens
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
+          // ---- S^T = K . Q^T, two tiles of 16 tokens side by side
+          float s[2][NT][4];
+          uint32_t kw[2][2][KW];               // [tile][rows r, r + 8]: the lane's codes
+          uint32_t kf[2][2][(D + 127) / 128];  // and the f16 pairs of their block scales
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
-            s[mt][nt][e] = fast_exp2(fmaf(s[mt][nt][e], qfac[nt][e], -m_use[nt][e]));
-            s[mt][nt][e + 2] = fast_exp2(fmaf(s[mt][nt][e + 2], qfac[nt][e], -m_use[nt][e]));
-          }
-          l[nt][e] += (s[0][nt][e] + s[0][nt][e + 2]) + (s[1][nt][e] + s[1][nt][e + 2]);
-        }
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          pt[mt][nt][0] = transpose8x8(pack_half2(s[mt][nt][0], s[mt][nt][1]));
-          pt[mt][nt][1] = transpose8x8(pack_half2(s[mt][nt][2], s[mt][nt][3]));
-        }
-      }
-
-      // ---- O^T += V^T . P^T
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        uint32_t v[4][VW], sc[4];  // tokens tx, ty, tx + 8, ty + 8 of the 16
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int row = ks * 16 + (u >> 1) * 8;
-          load_words<VW>(st + G::kTileBytes + v_at[u & 1] + row * RB, v[u]);
-          const uint8_t* sb = st + vs_at[u & 1] + row * SB;
-          sc[u] = D == 256 ? *reinterpret_cast<const uint16_t*>(sb) : *sb;
-        }
-#pragma unroll
-        for (int wi = 0; wi < VW; ++wi) {
-          uint32_t w0, w1;  // the block scales of the word's block, of two tokens each
-          if constexpr (D == 256) {
-            w0 = __byte_perm(sc[0], sc[1], wi < 2 ? 0x0040 : 0x0051);
-            w1 = __byte_perm(sc[2], sc[3], wi < 2 ? 0x0040 : 0x0051);
-          } else {
-            w0 = sc[0] + sc[1] * 256u;
-            w1 = sc[2] + sc[3] * 256u;
-          }
-          const uint32_t f0 = e4m3x2_to_half2(w0), f1 = e4m3x2_to_half2(w1);
-          // even codes of both tokens in one word, odd codes in another
-          uint32_t e0[4], o0[4], e1[4], o1[4];
-          e2m1x8_to_half2x4(low_high(v[0][wi], times16(v[1][wi])), e0);
-          e2m1x8_to_half2x4(low_high(v[0][wi] >> 4, v[1][wi]), o0);
-          e2m1x8_to_half2x4(low_high(v[2][wi], times16(v[3][wi])), e1);
-          e2m1x8_to_half2x4(low_high(v[2][wi] >> 4, v[3][wi]), o1);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t a0 = hmul2_bits(e0[j], f0), a1 = hmul2_bits(o0[j], f0);
-            const uint32_t a2 = hmul2_bits(e1[j], f1), a3 = hmul2_bits(o1[j], f1);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma_f16(acc[wi * 4 + j][nt], a0, a1, a2, a3, pt[ks][nt][0], pt[ks][nt][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int row = mt * 16 + half * 8;
+              const uint8_t* sc = st + ks_at + row * SB;
+              if constexpr (D == 256) {
+                uint32_t x[4], y[4];
+                load_words<4>(st + k_at + row * RB, x);
+                load_words<4>(st + k_at2 + row * RB, y);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { kw[mt][half][i] = x[i]; kw[mt][half][4 + i] = y[i]; }
+                const uint32_t q = *reinterpret_cast<const uint32_t*>(sc);
+                kf[mt][half][0] = e4m3x2_to_half2(q);
+                kf[mt][half][1] = e4m3x2_to_half2(q >> 16);
+              } else if constexpr (D == 128) {
+                load_words<4>(st + k_at + row * RB, kw[mt][half]);
+                kf[mt][half][0] = e4m3x2_to_half2(*reinterpret_cast<const uint16_t*>(sc));
+              } else {
+                load_words<2>(st + k_at + row * RB, kw[mt][half]);
+                kf[mt][half][0] = e4m3x2_to_half2(*sc);
+              }
+            }
           }
+#pragma unroll
+          for (int wi = 0; wi < KW; ++wi) {
+            const int blk = wi / 2;  // two words a block
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+              uint32_t h[2][4];
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const uint32_t pair = kf[mt][half][blk / 2];
+                const uint32_t f = blk & 1 ? high_twice(pair) : low_twice(pair);
+                e2m1x8_to_half2x4(kw[mt][half][wi], h[half]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[half][j] = hmul2_bits(h[half][j], f);
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_f16(s[mt][nt], h[0][0], h[1][0], h[0][1], h[1][1], qf[nt][2 * wi][0], qf[nt][2 * wi][1]);
+                mma_f16(s[mt][nt], h[0][2], h[1][2], h[0][3], h[1][3], qf[nt][2 * wi + 1][0], qf[nt][2 * wi + 1][1]);
+              }
+            }
+          }
+
+          // ---- softmax over the warp's 32 tokens (log2 domain)
+          if (__any_sync(0xffffffffu, t0 + kSubTokens > all_seen)) {  // some row does not see some token
+            const int len = volatile_at(entry(seg_r) + 1).x / HW, base = MULTI ? place().row_base : 0;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                // causal: row (qi, g) sees the keys up to its own position
+                const int seen =
+                    len + ((MULTI && p.causal) ? (base + nt * 8 + 2 * c + e) / p.group - (p.seqlen_q - 1) : 0);
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt) {
+                  if (t0 + mt * 16 + tau >= seen) s[mt][nt][e] = neg_inf;
+                  if (t0 + mt * 16 + tau + 8 >= seen) s[mt][nt][e + 2] = neg_inf;
+                }
+              }
+            // Block scales of V must not be NaN where P is 0.  Behind the sequence's
+            // end they are what memory held: cleared.
+            uint32_t* sb = reinterpret_cast<uint32_t*>(ring + at + 2 * G::kTileBytes + G::kTileScales + lane * SB);
+            if (t0 + lane >= len) {
+#pragma unroll
+              for (int i = 0; i < SB / 4; ++i) sb[i] = 0;
+            }
+            __syncwarp();
+            if constexpr (MULTI) {
+              // A NaN of the sequence must not reach the rows that do not see its
+              // token: it is taken out of the stage, and put into O's block of the
+              // rows that do see it.
+              bool any = false;
+#pragma unroll
+              for (int i = 0; i < SB / 4; ++i) any = any || nan_bytes(sb[i]) != 0;
+              unsigned tokens = __ballot_sync(0xffffffffu, any);
+              if (tokens != 0) {
+#pragma unroll 1
+                for (; tokens != 0; tokens &= tokens - 1) {
+                  const int u = __ffs(tokens) - 1;
+                  const uint8_t* row = st + 2 * G::kTileBytes + G::kTileScales + u * SB + r * (D / 8) / 16;
+#pragma unroll
+                  for (int j = 0; j < (D + 127) / 128; ++j) {  // the lane's blocks, of MT / that many tiles each
+                    constexpr int kPer = MT / ((D + 127) / 128);
+                    if (nan_bytes(row[j]) == 0) continue;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                      for (int e = 0; e < 2; ++e) {
+                        const int seen =
+                            len + (p.causal ? (base + nt * 8 + 2 * c + e) / p.group - (p.seqlen_q - 1) : 0);
+                        if (t0 + u >= seen) continue;
+#pragma unroll
+                        for (int i = j * kPer; i < (j + 1) * kPer; ++i)
+                          acc[i][nt][e] = acc[i][nt][e + 2] = __int_as_float(0x7fffffff);
+                      }
+                  }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < SB / 4; ++i) sb[i] &= ~nan_bytes(sb[i]);
+                __syncwarp();
+              }
+            }
+          }
+          // The reference of the exponents need not be the maximum: it is raised
+          // (and O, l rescaled) only when a logit exceeds it by more than 8, so
+          // that P stays below 2^8, well inside f16, and most stages need no
+          // reduction over the tokens' lanes.  Rounded up, it bounds the exact
+          // products that the exponents subtract it from, however large.
+          bool above = false;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float mx = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+              above = above || __fmul_ru(mx, qfac[nt][e]) - m[nt][e] > 8.f;
+            }
+          if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float mx = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float m_new = fmaxf(m[nt][e], __fmul_ru(mx, qfac[nt][e]));
+                const float alpha = m_new == m[nt][e] ? 1.f : fast_exp2(m[nt][e] - m_new);
+                m[nt][e] = m_new;
+                m_use[nt][e] = m_new == neg_inf ? 0.f : m_new;
+                l[nt][e] *= alpha;
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                  acc[i][nt][e] *= alpha;
+                  acc[i][nt][e + 2] *= alpha;
+                }
+              }
+          }
+          uint32_t pt[2][NT][2];  // P^T fragments of each 16 tokens
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt) {
+                s[mt][nt][e] = fast_exp2(fmaf(s[mt][nt][e], qfac[nt][e], -m_use[nt][e]));
+                s[mt][nt][e + 2] = fast_exp2(fmaf(s[mt][nt][e + 2], qfac[nt][e], -m_use[nt][e]));
+              }
+              l[nt][e] += (s[0][nt][e] + s[0][nt][e + 2]) + (s[1][nt][e] + s[1][nt][e + 2]);
+            }
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+              pt[mt][nt][0] = transpose8x8(pack_half2(s[mt][nt][0], s[mt][nt][1]));
+              pt[mt][nt][1] = transpose8x8(pack_half2(s[mt][nt][2], s[mt][nt][3]));
+            }
+          }
+
+          // ---- O^T += V^T . P^T
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            uint32_t v[4][VW], sc[4];  // tokens tx, ty, tx + 8, ty + 8 of the 16
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int row = ks * 16 + (u >> 1) * 8;
+              load_words<VW>(st + G::kTileBytes + v_at[u & 1] + row * RB, v[u]);
+              const uint8_t* sb = st + vs_at[u & 1] + row * SB;
+              sc[u] = D == 256 ? *reinterpret_cast<const uint16_t*>(sb) : *sb;
+            }
+#pragma unroll
+            for (int wi = 0; wi < VW; ++wi) {
+              uint32_t w0, w1;  // the block scales of the word's block, of two tokens each
+              if constexpr (D == 256) {
+                w0 = __byte_perm(sc[0], sc[1], wi < 2 ? 0x0040 : 0x0051);
+                w1 = __byte_perm(sc[2], sc[3], wi < 2 ? 0x0040 : 0x0051);
+              } else {
+                w0 = sc[0] + sc[1] * 256u;
+                w1 = sc[2] + sc[3] * 256u;
+              }
+              const uint32_t f0 = e4m3x2_to_half2(w0), f1 = e4m3x2_to_half2(w1);
+              // even codes of both tokens in one word, odd codes in another
+              uint32_t e0[4], o0[4], e1[4], o1[4];
+              e2m1x8_to_half2x4(low_high(v[0][wi], times16(v[1][wi])), e0);
+              e2m1x8_to_half2x4(low_high(v[0][wi] >> 4, v[1][wi]), o0);
+              e2m1x8_to_half2x4(low_high(v[2][wi], times16(v[3][wi])), e1);
+              e2m1x8_to_half2x4(low_high(v[2][wi] >> 4, v[3][wi]), o1);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t a0 = hmul2_bits(e0[j], f0), a1 = hmul2_bits(o0[j], f0);
+                const uint32_t a2 = hmul2_bits(e1[j], f1), a3 = hmul2_bits(o1[j], f1);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                  mma_f16(acc[wi * 4 + j][nt], a0, a1, a2, a3, pt[ks][nt][0], pt[ks][nt][1]);
+              }
+            }
+          }
+          t0 += step;
         }
-      }
-      t0 += step;
-      }
-      // ---- refill the stage
-      __syncwarp();  // every lane has read it
-      copy_stage(o2, at);
-      o2 += o2_step;
-      copy_commit();  // one group a stage, empty ones too, so that the count of groups stays fixed
-      at = at == (G::kStages - 1) * G::kStageBytes ? 0 : at + G::kStageBytes;
+        // ---- refill the stage
+        __syncwarp();  // every lane has read it
+        copy_stage(o2, at);
+        o2 += o2_step;
+        copy_commit();  // one group a stage, empty ones too, so that the count of groups stays fixed
+        at = at == (G::kStages - 1) * G::kStageBytes ? 0 : at + G::kStageBytes;
       }
       if (more) {
         pc_k += n;
@@ -1091,10 +1114,12 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
         if (tw == 0 && last) {
 #pragma unroll 1
           for (int u = 1; u < TW; ++u) {
-            const float* from = reinterpret_cast<const float*>(smem + G::kOffJoin + (warp + (u - 1) * HW) * G::kJoinWarp);
+            const float* from =
+                reinterpret_cast<const float*>(smem + G::kOffJoin + (warp + (u - 1) * HW) * G::kJoinWarp);
             const float* ml = from + G::kRows * G::kRowPad + 2 * (lv < kAt ? lv : 0);
             const float m_new = fmaxf(mm, ml[0]);
-            const float fa = mm == m_new ? 1.f : fast_exp2(mm - m_new), fb = ml[0] == m_new ? 1.f : fast_exp2(ml[0] - m_new);
+            const float fa = mm == m_new ? 1.f : fast_exp2(mm - m_new);
+            const float fb = ml[0] == m_new ? 1.f : fast_exp2(ml[0] - m_new);
             mm = m_new;
             den = fmaf(den, fa, ml[1] * fb);
 #pragma unroll

