@@ -4,20 +4,22 @@
 // A slot is page * page_size + row.  The append takes rows [T, Hkv, D] (any
 // token stride, e.g. a slice of a fused projection) and stores row t at slot
 // slot_map[t] of a 16-bit, e4m3 or 4-bit block-scaled cache; the gather is
-// its inverse and returns the values the cache stands for.  Both are single
-// passes bound by HBM: one thread handles 16 consecutive values of K and of V
-// (two 16-byte loads each), which is one scale block of the 4-bit format, so
+// its inverse and returns the values the cache stands for.  Slots below zero
+// are padding (skipped by the append, zeros from the gather); a slot past the
+// pool is skipped the same way and reported (FD_ERR_BAD_PAGE).
+//
+// Both are single passes: one thread handles 16 consecutive values of K and of
+// V (two 16-byte loads each), which is one scale block of the 4-bit format, so
 // a block's largest magnitude never leaves its thread.  A CTA takes several
 // rows, so that what depends on the unit alone (head, scales) is read once.
+//
 // Measured on a B200 (copy rate 6.56 TB/s): 59k tokens of 8 heads of 128
 // values in bf16 into the 4-bit cache 62.7 us, 4.9 TB/s of bytes read and
 // written; the quantising bounds it (schedulers issue in 74 % of the cycles,
-// half of that on the half-rate ALU).  Back 66.5 us, 5.2 TB/s, bound by the
-// latency of slot, codes and store (two rows at a time: 80 registers, 81 us; six
-// CTAs an SM: spilled, 112 us).  16-bit rows 9.0 us for 50 MB, 5.6 TB/s; a decode step's rows 3 us, a
-// launch.  Slots below zero are
-// padding (skipped by the append, zeros from the gather); a slot past the
-// pool is skipped the same way and reported (FD_ERR_BAD_PAGE).
+// the half-rate ALU works in 56 %).  Back 66.5 us, 5.2 TB/s, bound by the
+// latency of slot, codes and store (two rows at a time: 80 registers, 81 us;
+// six CTAs an SM: spilled, 112 us).  16-bit rows 9.0 us for 50 MB, 5.6 TB/s; a
+// decode step's rows 3 us, a launch.
 #include <cuda_runtime.h>
 
 #include <cstdint>

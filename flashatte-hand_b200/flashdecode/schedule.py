@@ -1,4 +1,4 @@
-"""Host-side model of the device scheduler in csrc/fd_decode_sm100.cu.
+"""Host-side model of the device scheduler in csrc/fd_schedule.cuh.
 
 The kernel decides its split on the device from cache_seqlens; this module
 computes the same partition on the host so tests can check its invariants
@@ -31,6 +31,12 @@ DEFAULT_FLOOR = 40
 E4M3_TILE_FIXED = 8
 E4M3_SEG = 48
 E4M3_FLOOR = 0
+# 4-bit caches (behind_lead; lengths times two where two KV heads are read
+# together, halving the heads)
+E2M1_TILE_FIXED = 2
+E2M1_SEG = 52
+E2M1_FLOOR = 0
+E2M1_ALIGN_TILES = 12
 # pair-aligned split: one whole pair per CTA when B * Hkv <= grid and no
 # sequence has more than this many tiles
 DEFAULT_ALIGN_TILES = 16
@@ -78,13 +84,17 @@ def pair_cost(length: int, tile_fixed: int = DEFAULT_TILE_FIXED, seg: int = DEFA
 
 def segments(seqlens, hkv: int, grid: int, max_len: int | None = None,
              tile_fixed: int = DEFAULT_TILE_FIXED, seg: int = DEFAULT_SEG,
-             align_tiles: int = 0, floor: int = DEFAULT_FLOOR) -> list[Segment]:
+             align_tiles: int = 0, floor: int = DEFAULT_FLOOR,
+             behind_lead: bool = False) -> list[Segment]:
     """All segments of all CTAs, in CTA order then work order (kernel's split).
 
     align_tiles > 0: with m = ceil(B * Hkv / grid) pairs per CTA, when no
     sequence has more than align_tiles // m tiles, every pair costs the same
     (max lead + align_tiles full tiles + 1) and CTA c takes exactly the whole
-    pairs [m c, m (c + 1))."""
+    pairs [m c, m (c + 1)).
+
+    behind_lead: a pair's first tile too starts behind its lead, so that a
+    range ending inside a lead leaves the whole pair to the next CTA."""
     lens = [min(max(0, int(L)), max_len) if max_len is not None else max(0, int(L)) for L in seqlens]
     full = FULL_TILE + tile_fixed
     npairs = len(lens) * hkv
@@ -97,7 +107,7 @@ def segments(seqlens, hkv: int, grid: int, max_len: int | None = None,
     for L in lens:
         prefix.append(prefix[-1] + (k_aligned if aligned else pair_cost(L, tile_fixed, seg, floor)))
     total = hkv * prefix[-1]
-    grid = -(-npairs // m) if aligned else max(1, min(grid, total // (max_lead + full + 1)))
+    grid = -(-npairs // m) if aligned else max(1, min(grid, total // ((0 if behind_lead else max_lead) + full + 1)))
 
     def range_start(c):
         if aligned:
@@ -112,7 +122,7 @@ def segments(seqlens, hkv: int, grid: int, max_len: int | None = None,
         return hkv * prefix[b] + kvh * (prefix[b + 1] - prefix[b])
 
     def tile_start(cp, ld, j):
-        return cp if j == 0 else cp + ld + j * full
+        return cp if j == 0 and not behind_lead else cp + ld + j * full
 
     def make(c, pair, j0, e1):
         b, kvh = divmod(pair, hkv)
@@ -124,7 +134,7 @@ def segments(seqlens, hkv: int, grid: int, max_len: int | None = None,
         x = e1 - cp - ld
         jmax = -(-x // full) - 1 if x > 0 else 0
         jmax = min(jmax, n - 1)
-        c0 = cta_of(cp)
+        c0 = cta_of(tile_start(cp, ld, 0))
         return Segment(c, b, kvh, pair, j0, jmax - j0 + 1, cta_of(tile_start(cp, ld, n - 1)) - c0 + 1, c0)
 
     out: list[Segment] = []
@@ -144,7 +154,7 @@ def segments(seqlens, hkv: int, grid: int, max_len: int | None = None,
         j0 = 0
         if e0 > cp:
             x = e0 - cp - leads[lo]
-            j0 = max(1, -(-x // full)) if x > 0 else 1
+            j0 = max(0 if behind_lead else 1, -(-x // full)) if x > 0 else (0 if behind_lead else 1)
         s = make(c, pair, j0, e1)
         if s is None and pair + 1 < npairs:
             s = make(c, pair + 1, 0, e1)

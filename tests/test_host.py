@@ -235,3 +235,32 @@ def test_cost_defaults_match_the_host_library():
                    "kDefaultCostFloor": schedule.DEFAULT_FLOOR, "kDefaultCostFloor8": schedule.E4M3_FLOOR}
     align = re.search(r"constexpr int kDefaultAlignTiles = (\d+);", src)
     assert int(align.group(1)) == schedule.DEFAULT_ALIGN_TILES
+
+
+@pytest.mark.parametrize("seg", [1, schedule.E2M1_SEG, 256])
+@pytest.mark.parametrize("grid", [1, 7, 148, 296])
+@pytest.mark.parametrize("seed", range(6))
+def test_behind_lead_schedule_covers_every_tile_once(seed, grid, seg):
+    """The 4-bit cache's split: every tile once, a pair's segments on
+    consecutive CTAs, slots unique."""
+    g = torch.Generator().manual_seed(seed)
+    B, hkv = [(1, 1), (2, 4), (64, 4), (128, 4), (33, 2), (5, 7)][seed]
+    hi = [300000, 524288, 8192, 65536, 700, 9000][seed]
+    lens = (torch.rand(B, generator=g) ** 3 * hi).long().tolist()
+    for align in (0, schedule.E2M1_ALIGN_TILES):
+        segs = schedule.segments(lens, hkv, grid, tile_fixed=schedule.E2M1_TILE_FIXED, seg=seg,
+                                 floor=schedule.E2M1_FLOOR, align_tiles=align, behind_lead=True)
+        tiles = [(s.pair, t) for s in segs for t in range(s.tile0, s.tile0 + s.ntiles)]
+        assert sorted(tiles) == [(b * hkv + h, t) for b, L in enumerate(lens) for h in range(hkv)
+                                 for t in range(schedule.tiles_of(L))]
+        slots = [s.slot for s in segs if s.nseg > 1]
+        assert len(slots) == len(set(slots)) and all(0 <= x < grid + B * hkv for x in slots)
+        by_pair = {}
+        for s in segs:
+            by_pair.setdefault(s.pair, []).append(s)
+        for ss in by_pair.values():
+            if ss[0].nseg == 1:
+                assert len(ss) == 1
+                continue
+            assert [s.cta for s in ss] == list(range(ss[0].cfirst, ss[0].cfirst + ss[0].nseg))
+            assert all((s.nseg, s.cfirst) == (ss[0].nseg, ss[0].cfirst) for s in ss)
