@@ -59,16 +59,18 @@
 // cycles of a quarter SM's share of the HBM, and 499 instructions of a warp:
 // 128 conversions of code pairs and 84 other ones on the half-rate ALU, 128
 // half-rate f16 multiplications, 32 mma, 38 loads and stores.  Two warps a
-// scheduler overlap these to 1.1 to 1.2 times the HBM's time; three (3 CTAs an
-// SM, 168 registers) were 10 to 17 % slower, with more segments for each.  So
+// scheduler overlap these to 831 cycles (840 with the loads from HBM: 6.2
+// TB/s); three (3 CTAs an SM, 168 registers) were 10 to 17 % slower, with more
+// segments for each.  So
 // the loop is written for few instructions (the half-rate ones most of all):
 // every five ALU instructions of it are a percent.
 //
 // Measured on a B200 (back-to-back launches; 6.56 TB/s is its copy rate): 64
 // sequences of 4096 tokens, 32 over 8 heads, D = 128: 68.5 us, 4.4 TB/s; two
-// of 131072: 117 us, 5.2 TB/s; the fixed part of a launch is 16 us (first data
+// of 262144: 117 us, 5.2 TB/s; the fixed part of a launch is 20 us (first data
 // after 6.5 us: schedule 1.5, first page ids 1.9, query 1.3, data 1.8; 2 to 3
-// us for a segment's end, 1.5 to 5 for a joining, the rest imbalance).
+// us for a segment's end, 1.5 to 5 for a joining, the rest ramps and
+// imbalance).
 #pragma once
 
 #include <cuda_bf16.h>
