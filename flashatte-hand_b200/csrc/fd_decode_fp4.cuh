@@ -61,9 +61,8 @@
 // half-rate f16 multiplications, 32 mma, 38 loads and stores.  Two warps a
 // scheduler overlap these to 831 cycles (840 with the loads from HBM: 6.2
 // TB/s); three (3 CTAs an SM, 168 registers) were 10 to 17 % slower, with more
-// segments for each.  So
-// the loop is written for few instructions (the half-rate ones most of all):
-// every five ALU instructions of it are a percent.
+// segments for each.  So the loop is written for few instructions (the
+// half-rate ones most of all): every five ALU instructions of it are a percent.
 //
 // Measured on a B200 (back-to-back launches; 6.56 TB/s is its copy rate): 64
 // sequences of 4096 tokens, 32 over 8 heads, D = 128: 68.5 us, 4.4 TB/s; two
@@ -544,12 +543,14 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   keep(k_at), keep(k_at2), keep(v_at[0]), keep(v_at[1]), keep(ks_at), keep(vs_at[0]), keep(vs_at[1]);
 
   for (int seg_r = 0; seg_r < seg_w; ++seg_r) {
-    int ntiles, t0, seqlen;
+    int ntiles, k_mask;  // from stage k_mask on some row does not see some token
     {
       const Segment g = segment_of(seg_r);
       ntiles = g.ntiles;
-      t0 = g.tile0 * step + tw * kSubTokens;
-      seqlen = g.seqlen / HW;
+      // t0 + kSubTokens > the keys that every row sees, for t0 = t + k * step
+      const int t = g.tile0 * step + tw * kSubTokens;
+      const int all_seen = g.seqlen / HW - ((MULTI && p.causal) ? p.seqlen_q - 1 : 0);
+      k_mask = ((all_seen - kSubTokens - t) >> (HW == 2 ? 6 : 7)) + 1;
     }
     // sequence, KV head, first query row of the pass and its rows
     struct Place {
@@ -634,11 +635,9 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
 #pragma unroll
         for (int e = 0; e < 2; ++e) qfac[nt][e] = f * __shfl_sync(0xffffffffu, row_inv[nt], (2 * c + e) * 4);
     }
-    const int all_seen = seqlen - ((MULTI && p.causal) ? p.seqlen_q - 1 : 0);  // keys that every row sees
 
     float acc[MT][NT][4];
     float m[NT][2], l[NT][2];
-    float m_use[NT][2];  // m, or 0 while no key was seen (then every P is 0)
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -647,8 +646,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
         for (int e = 0; e < 4; ++e) acc[i][nt][e] = 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = neg_inf;
-      m_use[nt][0] = m_use[nt][1] = 0.f;
+      m[nt][0] = m[nt][1] = -3e38f;  // below any logit; while no key was seen every P is 0
       l[nt][0] = l[nt][1] = 0.f;
     }
 
@@ -729,7 +727,8 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
           }
 
           // ---- softmax over the warp's 32 tokens (log2 domain)
-          if (__any_sync(0xffffffffu, t0 + kSubTokens > all_seen)) {  // some row does not see some token
+          if (__any_sync(0xffffffffu, k >= k_mask)) {
+            const int t0 = (volatile_at(entry(seg_r)).z + k) * step + tw * kSubTokens;
             const int len = volatile_at(entry(seg_r) + 1).x / HW, base = MULTI ? place().row_base : 0;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -814,7 +813,6 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
                 const float m_new = fmaxf(m[nt][e], __fmul_ru(mx, qfac[nt][e]));
                 const float alpha = m_new == m[nt][e] ? 1.f : fast_exp2(m[nt][e] - m_new);
                 m[nt][e] = m_new;
-                m_use[nt][e] = m_new == neg_inf ? 0.f : m_new;
                 l[nt][e] *= alpha;
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
@@ -830,8 +828,8 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
               for (int mt = 0; mt < 2; ++mt) {
-                s[mt][nt][e] = fast_exp2(fmaf(s[mt][nt][e], qfac[nt][e], -m_use[nt][e]));
-                s[mt][nt][e + 2] = fast_exp2(fmaf(s[mt][nt][e + 2], qfac[nt][e], -m_use[nt][e]));
+                s[mt][nt][e] = fast_exp2(fmaf(s[mt][nt][e], qfac[nt][e], -m[nt][e]));
+                s[mt][nt][e + 2] = fast_exp2(fmaf(s[mt][nt][e + 2], qfac[nt][e], -m[nt][e]));
               }
               l[nt][e] += (s[0][nt][e] + s[0][nt][e + 2]) + (s[1][nt][e] + s[1][nt][e + 2]);
             }
@@ -880,7 +878,6 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
               }
             }
           }
-          t0 += step;
         }
         // ---- refill the stage
         __syncwarp();  // every lane has read it
@@ -943,7 +940,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
             for (int e = 0; e < 2; ++e) {
               const int row = nt * 8 + 2 * c + e;
               const float mo = ml[row * 2], mm = fmaxf(m[nt][e], mo);
-              // equal references (both -inf too) weigh 1, so that NaN sums stay
+              // equal references weigh 1, so that NaN sums stay
               const float fa = m[nt][e] == mm ? 1.f : fast_exp2(m[nt][e] - mm);
               const float fb = mo == mm ? 1.f : fast_exp2(mo - mm);
               m[nt][e] = mm;
