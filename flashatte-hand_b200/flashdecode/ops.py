@@ -25,6 +25,7 @@ from ._lib import (FD_DTYPE_BF16, FD_DTYPE_E2M1, FD_DTYPE_E4M3, FD_DTYPE_FP16, F
 _DTYPES = {torch.bfloat16: FD_DTYPE_BF16, torch.float16: FD_DTYPE_FP16}
 _CACHE_DTYPES = {torch.bfloat16: FD_DTYPE_BF16, torch.float16: FD_DTYPE_FP16,
                  torch.float8_e4m3fn: FD_DTYPE_E4M3, torch.float4_e2m1fn_x2: FD_DTYPE_E2M1}
+_INT32 = torch.int32
 _OUT_DTYPES = {torch.bfloat16: FD_DTYPE_BF16, torch.float16: FD_DTYPE_FP16, torch.float32: FD_DTYPE_FP32}
 
 
@@ -56,6 +57,18 @@ def _on_device(dev: torch.device):
     if dev.index is None or dev.index == _current_device():
         return _NO_SWITCH
     return torch.cuda.device(dev)
+
+
+def _launch(fn, dev: torch.device, stream, args) -> None:
+    """fn(*args, stream handle) with `dev` current; raises on a bad status."""
+    handle = _stream_handle(stream, dev)
+    if dev.index == _current_device():
+        status = fn(*args, handle)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, handle)
+    if status:
+        check(status)
 
 
 def _require_cuda(*tensors: torch.Tensor) -> None:
@@ -449,11 +462,10 @@ def append_kv_slots(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
             raise ValueError(f"the heads of a token of {name} must be contiguous")
         token.append(st if T > 1 else row)
     dev = k_cache.device
-    with _on_device(dev):
-        check(lib.fd_append_kv_slots(
-            k.data_ptr(), token[0], v.data_ptr(), token[1], k_cache.data_ptr(), v_cache.data_ptr(),
-            _ptr(k_block_scale), _ptr(v_block_scale), _ptr(k_scale), _ptr(v_scale), slot_map.data_ptr(),
-            T, Hkv, D, page, num_blocks, src, dst, _stream_handle(stream, dev)))
+    _launch(lib.fd_append_kv_slots, dev, stream, (
+        k.data_ptr(), token[0], v.data_ptr(), token[1], k_cache.data_ptr(), v_cache.data_ptr(),
+        _ptr(k_block_scale), _ptr(v_block_scale), _ptr(k_scale), _ptr(v_scale), slot_map.data_ptr(),
+        T, Hkv, D, page, num_blocks, src, dst))
 
 
 def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_map: torch.Tensor,
@@ -483,16 +495,15 @@ def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_map: torch.Tens
         k_out = torch.empty(T, Hkv, D, dtype=out_dtype, device=dev)
     if v_out is None:
         v_out = torch.empty_like(k_out)
-    with _on_device(dev):
-        check(lib.fd_gather_kv_slots(
-            k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_block_scale), _ptr(v_block_scale),
-            _ptr(k_scale), _ptr(v_scale), slot_map.data_ptr(), T, k_out.data_ptr(), v_out.data_ptr(),
-            Hkv, D, page, num_blocks, _CACHE_DTYPES[k_cache.dtype], odt, _stream_handle(stream, dev)))
+    _launch(lib.fd_gather_kv_slots, dev, stream, (
+        k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_block_scale), _ptr(v_block_scale),
+        _ptr(k_scale), _ptr(v_scale), slot_map.data_ptr(), T, k_out.data_ptr(), v_out.data_ptr(),
+        Hkv, D, page, num_blocks, _CACHE_DTYPES[k_cache.dtype], odt))
     return k_out, v_out
 
 
 def _check_int32(name: str, t: torch.Tensor, shape) -> None:
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+    if t.dtype is not _INT32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}")
 
 
@@ -557,12 +568,10 @@ def assign_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, new_len
         seqlens_out = torch.empty_like(cache_seqlens)
     else:
         _check_int32("seqlens_out", seqlens_out, (B,))
-    with _on_device(dev):
-        check(lib.fd_assign_pages(
-            block_table.data_ptr(), width, cache_seqlens.data_ptr(), new_lens.data_ptr(),
-            free_pages.data_ptr(), free_count.data_ptr(), B, int(page_block_size), num_blocks,
-            seqlens_out.data_ptr(), cu_new_lens.data_ptr(), slot_map.data_ptr(), num_slots,
-            _stream_handle(stream, dev)))
+    _launch(lib.fd_assign_pages, dev, stream, (
+        block_table.data_ptr(), width, cache_seqlens.data_ptr(), new_lens.data_ptr(),
+        free_pages.data_ptr(), free_count.data_ptr(), B, int(page_block_size), num_blocks,
+        seqlens_out.data_ptr(), cu_new_lens.data_ptr(), slot_map.data_ptr(), num_slots))
     return slot_map, cu_new_lens, seqlens_out
 
 
@@ -579,11 +588,9 @@ def release_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, keep_l
     _check_int32("cache_seqlens", cache_seqlens, (B,))
     _check_int32("keep_lens", keep_lens, (B,))
     dev = block_table.device
-    with _on_device(dev):
-        check(lib.fd_release_pages(
-            block_table.data_ptr(), width, cache_seqlens.data_ptr(), keep_lens.data_ptr(),
-            free_pages.data_ptr(), free_count.data_ptr(), B, int(page_block_size), num_blocks,
-            _stream_handle(stream, dev)))
+    _launch(lib.fd_release_pages, dev, stream, (
+        block_table.data_ptr(), width, cache_seqlens.data_ptr(), keep_lens.data_ptr(),
+        free_pages.data_ptr(), free_count.data_ptr(), B, int(page_block_size), num_blocks))
 
 
 def combine_lse(part_o: torch.Tensor, part_lse: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,
