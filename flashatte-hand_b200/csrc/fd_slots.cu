@@ -18,7 +18,8 @@
 // written; the quantising bounds it (schedulers issue in 74 % of the cycles,
 // the half-rate ALU works in 56 %).  Back 66.5 us, 5.2 TB/s, bound by the
 // latency of slot, codes and store (two rows at a time: 80 registers, 81 us;
-// six CTAs an SM: spilled, 112 us).  16-bit rows 9.0 us for 50 MB, 5.6 TB/s; a
+// six CTAs an SM: spilled, 112 us; lanes exchanging halves for whole-sector
+// stores: 64 registers, 72 us).  16-bit rows 9.0 us for 50 MB, 5.6 TB/s; a
 // decode step's rows 3 us, a launch.
 #include <cuda_runtime.h>
 
