@@ -498,3 +498,32 @@ def test_refusals():
         t16 = cases.materialize(c16, "cuda")
         flashdecode.flash_decode(t16["q"], t16["k_cache"], t16["v_cache"], t16["cache_seqlens"],
                                  t16["block_table"], k_block_scale=d["kb"])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("out_dtype", [None, torch.float32])
+@pytest.mark.parametrize("Hq,Hkv,sq", [(16, 1, 1), (8, 2, 1), (6, 3, 1), (8, 2, 3), (24, 2, 2)])
+def test_many_partials_of_a_pair(D, out_dtype, Hq, Hkv, sq):
+    """One long sequence over all CTAs, at every head dim: rows and partials
+    shared by the warps of the joining, rows of more than one pass."""
+    t = make([30000, 5], Hq, Hkv, D=D, page=64, sq=sq, seed=D + Hq, dtype=torch.float16)
+    out, lse = call(on_gpu(t), causal=sq > 1, out_dtype=out_dtype)
+    torch.cuda.synchronize()
+    check(out, lse, reference(t, causal=sq > 1))
+
+
+@pytest.mark.parametrize("D,Hq,Hkv", [(128, 8, 2), (64, 6, 3), (256, 2, 1)])
+def test_many_query_tokens(D, Hq, Hkv):
+    """A prompt's worth of causal query tokens: many passes over the rows, most
+    of them of rows that do not see the last keys, or any."""
+    t = make([70, 33, 900, 0], Hq, Hkv, D=D, page=16, sq=70, seed=D)
+    out, lse = call(on_gpu(t), causal=True)
+    torch.cuda.synchronize()
+    check(out, lse, reference(t, causal=True))
+
+
+def test_workspace_size_of_the_cache_type():
+    lib = flashdecode.load_library()
+    assert flashdecode.workspace_size(4, 32, 8, 128, 2, kv_dtype=FP4) == \
+        lib.fd_decode_workspace_size_fp4(4, 2, 32, 8, 128) > 0
+    assert flashdecode.workspace_size(4, 32, 8) == lib.fd_decode_workspace_size_mq(4, 1, 32, 8, 128)
