@@ -239,7 +239,9 @@ int fd_append_kv_paged_fp8(const void* k_new, const void* v_new, void* k_cache, 
  * append as in fd_decode_paged_fp8 (k_new / v_new 16-bit rows of q's type
  * [B, seqlen_new, Hkv, headdim], or NULL for both).  Supported: headdim 64,
  * 128 or 256, any number of query rows, page a multiple of 16, 16-byte aligned
- * q, new rows, caches and block scales (FD_ERR_UNSUPPORTED otherwise).  Workspace: at least
+ * q, out, new rows, caches and block scales (FD_ERR_UNSUPPORTED otherwise).
+ * Rows of the cache behind a sequence's length are never used, and a NaN of a
+ * token reaches the query rows that see it only.  Workspace: at least
  * fd_decode_workspace_size_fp4(...) bytes, 256-byte aligned and zero-filled
  * before its first use, or NULL (as for fd_decode_paged).
  * Replaces: nothing in the reference (its caches are bf16, best :1186-1211).
