@@ -350,8 +350,8 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
       batch_size * seqlen_q * num_heads > INT32_MAX || block_table_stride > INT32_MAX ||
       (k_new != nullptr && batch_size * seqlen_new > INT32_MAX))
     return report_error(FD_ERR_UNSUPPORTED, "size exceeds 32-bit index range");
-  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(k_block_scale, 16) ||
-      !aligned(v_block_scale, 16) || !aligned(k_new, 16) || !aligned(v_new, 16))
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) ||
+      !aligned(k_block_scale, 16) || !aligned(v_block_scale, 16) || !aligned(k_new, 16) || !aligned(v_new, 16))
     return report_error(FD_ERR_UNSUPPORTED, "e2m1 cache: tensors must be 16-byte aligned");
   int dev = 0;
   int* status = nullptr;
@@ -441,7 +441,6 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
     p.err = status;
     p.cost_tile = cost_tile4();
     p.cost_seg = lead;
-    p.cost_floor = 0;
     p.align_tiles = align_tiles4();
     p.pdl = fd::pdl_enabled() ? 1 : 0;
     const int64_t work = nb * vheads * tiles_bound;

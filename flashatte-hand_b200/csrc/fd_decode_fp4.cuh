@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
 
   // ------------------------------------------------------------ prologue
   if (tid == 0) pdl_launch_dependents();
-  const CostModel cm{p.cost_tile, p.cost_seg, p.cost_floor};
+  const CostModel cm{p.cost_tile, p.cost_seg, 0};
   pdl_wait_prerequisites();
   unsigned long long epoch_ld = 0;
   if (tid == 0) epoch_ld = *reinterpret_cast<volatile unsigned long long*>(p.epoch_word);
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     x.total = static_cast<int64_t>(p.num_heads_k / HW * p.row_tiles) * volatile_at(prefix + p.batch);
     x.batch = p.batch;
     x.hkv = p.num_heads_k / HW * p.row_tiles;
-    x.cm = CostModel{p.cost_tile, p.cost_seg, p.cost_floor};
+    x.cm = CostModel{p.cost_tile, p.cost_seg, 0};
     x.behind_lead = true;
     x.align_m = volatile_at(align_word);
     x.align_cost = x.cm.max_lead() + p.align_tiles * x.cm.full() + 1;

@@ -172,7 +172,7 @@ struct Fp4DecodeParams {
   unsigned long long* tickets;   // arrival counters of (pair, head), as DecodeParams::tickets
   unsigned long long* epoch_word;
   int* err;
-  int cost_tile, cost_seg, cost_floor;
+  int cost_tile, cost_seg;
   int align_tiles;               // short launches: most tiles of a CTA (0: never)
   int pdl;
 };
