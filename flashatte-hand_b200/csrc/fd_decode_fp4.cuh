@@ -17,8 +17,14 @@
 // of the logits and of O.  The query is f16 after scaling each row by a power
 // of two that brings its largest magnitude to [2^13, 2^14): exact for fp16
 // rows (not scaled) and for the bf16 values down to 2^-28 of the row's
-// largest (smaller ones keep an absolute error of 2^-39 of it).  P is rounded
-// to f16 (11 bits; values below 2^-14 of a row's largest keep 2^-25 of it).
+// largest (smaller ones keep an absolute error of 2^-39 of it).  P enters
+// as two f16 parts, the rounded value and the rounded rest: 2^-24 of each, and
+// 2^-32 of the row's largest below that, so that fp32 outputs are worth their
+// bits, as over the 16-bit caches.  Up to four query rows the parts lie side by
+// side in a tile's 8 columns (FOLD), beyond that each is multiplied with V.
+// One part alone (2^-11 of each weight): 64 sequences of 4096 tokens with 4
+// rows 67.6 us instead of 70.1 (76.5 unfolded), config 3 with 8 rows 114
+// instead of 131, 16 rows of 4 speculated tokens 40.8 instead of 45.8.
 //
 // Why mma.sync and not tcgen05: the dequantised tiles would have to be
 // written to shared memory (2 bytes a value) and read back by the tensor
@@ -91,6 +97,9 @@ constexpr int kFp4Warps = kFp4Threads / 32;
 constexpr int kSubTokens = 32;  // tokens of a stage
 constexpr int kOffEntries = 34; // 16 stages' offsets, and a stage of none
 constexpr int kSegRing = 8;     // segments that the loads may be ahead
+// P is 2^kLift where its logit is the reference's largest, and its reference
+// is raised when one is 2^kRaise: in f16's range with room at both ends.
+constexpr int kLift = 7, kRaise = 15;
 static_assert(kTileTokens == kFp4Warps * kSubTokens, "a schedule tile is a stage of each warp");
 
 template <int D, int NT> struct Fp4Geo {
@@ -161,6 +170,17 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// (lo, hi) + f * h, with f an f16 number, rounded to f16.  For h = pack_half2(lo,
+// hi) and f = -1: what that rounding left of both, exactly before its own.
+constexpr uint16_t kMinusOne = 0xBC00;
+__device__ __forceinline__ uint32_t pack_rest2(float lo, float hi, uint32_t h, uint16_t f) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+      "fma.rn.f32.f16 %0, a, %3, %0;\n\tfma.rn.f32.f16 %1, b, %3, %1;\n\t}"
+      : "+f"(lo), "+f"(hi)
+      : "r"(h), "h"(f));
+  return pack_half2(lo, hi);
 }
 
 // p + n * step in one instruction of the FMA pipe (a 64-bit addition is two of
@@ -296,7 +316,9 @@ template <int RB> __device__ __forceinline__ int swizzled(int row, int chunk) {
   else return chunk ^ (row & 7);
 }
 
-template <typename T, typename OutT, int D, int NT, bool MULTI>
+// MULTI: several query tokens, or a causal mask.  FOLD: at most four query rows;
+// the second halves of the 8 columns hold them again, for P's second part.
+template <typename T, typename OutT, int D, int NT, bool MULTI, bool FOLD>
 __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
     decode_fp4_kernel(const __grid_constant__ Fp4DecodeParams p) {
   using G = Fp4Geo<D, NT>;
@@ -305,9 +327,13 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   constexpr int VW = D / 64;        // words of V a lane takes from a token
   constexpr int MT = D / 16;        // 16-dim tiles of O^T
   constexpr int KS = D / 16;        // 16-dim steps of S^T
+  constexpr int kParts = FOLD ? 1 : 2;  // products of V with parts of P
+  static_assert(!FOLD || NT == 1, "four rows, twice");
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int r = lane >> 2, c = lane & 3;
+  // the query row of the pass in column 2 c + e of tile nt
+  auto row_of = [&](int nt, int e) { return FOLD ? (2 * c + e) & 3 : nt * 8 + 2 * c + e; };
 
   uint8_t* ring = smem + warp * G::kStages * G::kStageBytes;
   longlong2* offs = reinterpret_cast<longlong2*>(smem + G::kOffOffs) + warp * kOffEntries;
@@ -578,7 +604,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       float row_inv[NT];  // 2^-k of the row's scaling
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int n = nt * 8 + r;
+        const int n = FOLD ? r & 3 : nt * 8 + r;
         row_inv[nt] = 1.f;
         uint4 raw[D / 32];
         if (n < nrows) {
@@ -736,7 +762,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
               for (int e = 0; e < 2; ++e) {
                 // causal: row (qi, g) sees the keys up to its own position
                 const int seen =
-                    len + ((MULTI && p.causal) ? (base + nt * 8 + 2 * c + e) / p.group - (p.seqlen_q - 1) : 0);
+                    len + ((MULTI && p.causal) ? (base + row_of(nt, e)) / p.group - (p.seqlen_q - 1) : 0);
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
                   if (t0 + mt * 16 + tau >= seen) s[mt][nt][e] = neg_inf;
@@ -773,7 +799,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
 #pragma unroll
                       for (int e = 0; e < 2; ++e) {
                         const int seen =
-                            len + (p.causal ? (base + nt * 8 + 2 * c + e) / p.group - (p.seqlen_q - 1) : 0);
+                            len + (p.causal ? (base + row_of(nt, e)) / p.group - (p.seqlen_q - 1) : 0);
                         if (t0 + u >= seen) continue;
 #pragma unroll
                         for (int i = j * kPer; i < (j + 1) * kPer; ++i)
@@ -788,18 +814,18 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
               }
             }
           }
-          // The reference of the exponents need not be the maximum: it is raised
-          // (and O, l rescaled) only when a logit exceeds it by more than 8, so
-          // that P stays below 2^8, well inside f16, and most stages need no
-          // reduction over the tokens' lanes.  Rounded up, it bounds the exact
-          // products that the exponents subtract it from, however large.
+          // The reference of the exponents need not be the maximum less kLift: it
+          // is raised (and O, l rescaled) only when a logit exceeds it by more than
+          // kRaise, so that P stays inside f16 and most stages need no reduction
+          // over the tokens' lanes.  The product rounded up bounds the exact ones
+          // that the exponents subtract the reference from, however large.
           bool above = false;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const float mx = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
-              above = above || __fmul_ru(mx, qfac[nt][e]) - m[nt][e] > 8.f;
+              above = above || __fmul_ru(mx, qfac[nt][e]) - m[nt][e] > kRaise;
             }
           if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
@@ -810,7 +836,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                const float m_new = fmaxf(m[nt][e], __fmul_ru(mx, qfac[nt][e]));
+                const float m_new = fmaxf(m[nt][e], __fmul_ru(mx, qfac[nt][e]) - kLift);
                 const float alpha = m_new == m[nt][e] ? 1.f : fast_exp2(m[nt][e] - m_new);
                 m[nt][e] = m_new;
                 l[nt][e] *= alpha;
@@ -821,7 +847,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
                 }
               }
           }
-          uint32_t pt[2][NT][2];  // P^T fragments of each 16 tokens
+          uint32_t pt[2][NT][kParts][2];  // P^T fragments of each 16 tokens
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -835,8 +861,17 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
             }
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
-              pt[mt][nt][0] = transpose8x8(pack_half2(s[mt][nt][0], s[mt][nt][1]));
-              pt[mt][nt][1] = transpose8x8(pack_half2(s[mt][nt][2], s[mt][nt][3]));
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const float x = s[mt][nt][2 * half], y = s[mt][nt][2 * half + 1];
+                const uint32_t h = pack_half2(x, y);
+                if constexpr (FOLD) {  // the first part in columns 0 .. 3, the second in 4 .. 7
+                  pt[mt][nt][0][half] = transpose8x8(pack_rest2(x, y, h, c < 2 ? 0 : kMinusOne));
+                } else {
+                  pt[mt][nt][0][half] = transpose8x8(h);
+                  pt[mt][nt][1][half] = transpose8x8(pack_rest2(x, y, h, kMinusOne));
+                }
+              }
             }
           }
 
@@ -874,7 +909,9 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
                 const uint32_t a2 = hmul2_bits(e1[j], f1), a3 = hmul2_bits(o1[j], f1);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
-                  mma_f16(acc[wi * 4 + j][nt], a0, a1, a2, a3, pt[ks][nt][0], pt[ks][nt][1]);
+#pragma unroll
+                  for (int part = kParts - 1; part >= 0; --part)
+                    mma_f16(acc[wi * 4 + j][nt], a0, a1, a2, a3, pt[ks][nt][part][0], pt[ks][nt][part][1]);
               }
             }
           }
@@ -908,6 +945,12 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
         l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
         l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
       }
+    if constexpr (FOLD) {  // the sums of both parts, in columns 0 .. 3
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][0][e] += __shfl_xor_sync(0xffffffffu, acc[i][0][e], 2);
+    }
     if (TW > 1) {
       // Lane (r, c) holds dims r * D / 8 + 2 i (entries e) and + 2 i + 1
       // (entries e + 2) of rows 2 c + e.
@@ -989,7 +1032,8 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
           if (row >= nrows) continue;
           const bool some = !(l[nt][e] == 0.f);  // a row that saw a key (NaN stays NaN)
           const float inv = some ? vs / l[nt][e] : 0.f;
-          const float lse2 = some ? m[nt][e] + fast_log2(l[nt][e]) : neg_inf;
+          // (the lift is taken out of both, so that the logarithm is of a small number)
+          const float lse2 = some ? (m[nt][e] + kLift) + fast_log2(l[nt][e] * (1.f / (1 << kLift))) : neg_inf;
           float o[D / 8];
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
@@ -1165,10 +1209,10 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
   }
 }
 
-template <typename T, typename OutT, int D, int NT, bool MULTI>
+template <typename T, typename OutT, int D, int NT, bool MULTI, bool FOLD>
 cudaError_t launch_fp4_typed(const Fp4DecodeParams& p, int grid, cudaStream_t stream) {
   using G = Fp4Geo<D, NT>;
-  auto kern = decode_fp4_kernel<T, OutT, D, NT, MULTI>;
+  auto kern = decode_fp4_kernel<T, OutT, D, NT, MULTI, FOLD>;
   static unsigned long long configured = 0;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1192,27 +1236,27 @@ cudaError_t launch_fp4_typed(const Fp4DecodeParams& p, int grid, cudaStream_t st
   return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-template <typename T, typename OutT>
-cudaError_t launch_fp4(const Fp4DecodeParams& p, int head_dim, int grid,
-                       cudaStream_t stream) {
+template <typename T, typename OutT, int D>
+cudaError_t launch_fp4_dim(const Fp4DecodeParams& p, int grid, cudaStream_t stream) {
   const bool multi = p.seqlen_q > 1 || p.causal;
-  const bool two = p.rows == 16;
+  if (p.qrows <= 4)
+    return multi ? launch_fp4_typed<T, OutT, D, 1, true, true>(p, grid, stream)
+                 : launch_fp4_typed<T, OutT, D, 1, false, true>(p, grid, stream);
+  if constexpr (D < 256) {
+    if (p.rows == 16)
+      return multi ? launch_fp4_typed<T, OutT, D, 2, true, false>(p, grid, stream)
+                   : launch_fp4_typed<T, OutT, D, 2, false, false>(p, grid, stream);
+  }
+  return multi ? launch_fp4_typed<T, OutT, D, 1, true, false>(p, grid, stream)
+               : launch_fp4_typed<T, OutT, D, 1, false, false>(p, grid, stream);
+}
+
+template <typename T, typename OutT>
+cudaError_t launch_fp4(const Fp4DecodeParams& p, int head_dim, int grid, cudaStream_t stream) {
   switch (head_dim) {
-    case 64:
-      if (two)
-        return multi ? launch_fp4_typed<T, OutT, 64, 2, true>(p, grid, stream)
-                     : launch_fp4_typed<T, OutT, 64, 2, false>(p, grid, stream);
-      return multi ? launch_fp4_typed<T, OutT, 64, 1, true>(p, grid, stream)
-                   : launch_fp4_typed<T, OutT, 64, 1, false>(p, grid, stream);
-    case 128:
-      if (two)
-        return multi ? launch_fp4_typed<T, OutT, 128, 2, true>(p, grid, stream)
-                     : launch_fp4_typed<T, OutT, 128, 2, false>(p, grid, stream);
-      return multi ? launch_fp4_typed<T, OutT, 128, 1, true>(p, grid, stream)
-                   : launch_fp4_typed<T, OutT, 128, 1, false>(p, grid, stream);
-    default:
-      return multi ? launch_fp4_typed<T, OutT, 256, 1, true>(p, grid, stream)
-                   : launch_fp4_typed<T, OutT, 256, 1, false>(p, grid, stream);
+    case 64: return launch_fp4_dim<T, OutT, 64>(p, grid, stream);
+    case 128: return launch_fp4_dim<T, OutT, 128>(p, grid, stream);
+    default: return launch_fp4_dim<T, OutT, 256>(p, grid, stream);
   }
 }
 

@@ -527,3 +527,21 @@ def test_workspace_size_of_the_cache_type():
     assert flashdecode.workspace_size(4, 32, 8, 128, 2, kv_dtype=FP4) == \
         lib.fd_decode_workspace_size_fp4(4, 2, 32, 8, 128) > 0
     assert flashdecode.workspace_size(4, 32, 8) == lib.fd_decode_workspace_size_mq(4, 1, 32, 8, 128)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq,Hkv,sq", [(8, 2, 1), (16, 1, 1), (6, 3, 3)])
+def test_fp32_outputs_are_worth_their_bits(D, dtype, Hq, Hkv, sq):
+    """The weights enter the product with V in two f16 parts: 2^-24 of each
+    weight, and 2^-32 of the row's largest.  Small queries keep E below 2^-17,
+    and up to 160 tokens are at most 8 products a warp, each adding 16 tokens in
+    the accumulator (17 roundings of 2^-24 at most: 2^-17 in all); with exp2, the
+    division and the joining below 2^-18 the rest is 2^-16 of A.  One f16 part
+    alone is off by up to 2^-12."""
+    t = make([2, 3, 4, 5, 8, 17, 40, 160], Hq, Hkv, D=D, page=16, sq=sq, dtype=dtype, seed=D + sq, q_std=1 / 32)
+    out, _ = call(on_gpu(t), out_dtype=torch.float32, causal=sq > 1)
+    O, _, A, E, W = reference(t, causal=sq > 1)          # W: L 2^-25 max|v|
+    tol = (2 * E.permute(0, 2, 1)[..., None] + 2.0 ** -16) * A + 2.0 ** -7 * W + 2.0 ** -24 * O.abs()
+    err = (out.cpu().double() - O).abs()
+    assert bool((err <= tol).all()), float((err / tol.clamp(min=1e-300)).max())
