@@ -1133,7 +1133,8 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
 #pragma unroll
           for (int u = 0; u < kAt; ++u) {
             const float wu = __shfl_sync(0xffffffffu, w, v * kAt + u);
-            if (wu == 0.f) continue;
+            // not read above; one whose weight is 0 counts, for its NaNs
+            if (j0 + u >= nseg || row0 + v * row_ways >= nrows) continue;
 #pragma unroll
             for (int q = 0; q < kPieces; ++q)
 #pragma unroll

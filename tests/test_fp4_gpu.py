@@ -545,3 +545,25 @@ def test_fp32_outputs_are_worth_their_bits(D, dtype, Hq, Hkv, sq):
     tol = (2 * E.permute(0, 2, 1)[..., None] + 2.0 ** -16) * A + 2.0 ** -7 * W + 2.0 ** -24 * O.abs()
     err = (out.cpu().double() - O).abs()
     assert bool((err <= tol).all()), float((err / tol.clamp(min=1e-300)).max())
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (3, 1), (16, 1)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_nan_of_a_partial_without_weight(D, Hq, Hkv):
+    """Block scales of V that are NaN at tokens of no weight, around one that
+    takes all of it: 0 * NaN is NaN, wherever the sequence is cut."""
+    L, peak = 30000, 15000
+    t = make([L], Hq, Hkv, D=D, page=16, seed=D)
+    t["q"][:] = 8.0
+    pg, row = int(t["bt"][0, peak // 16]), peak % 16
+    t["k"][pg, row] = 0x77           # every code 6, every block scale 448
+    t["kb"][pg, :, row] = 0x7E
+    at = [peak + s * n * 90 for n in range(1, 1 + D // 32) for s in (-1, 1)]   # one token a block
+    for block, tok in enumerate(at):
+        t["vb"][int(t["bt"][0, tok // 16]), 0, tok % 16, block] = 0x7F
+    out, lse = call(on_gpu(t))
+    assert torch.isfinite(lse).all()
+    nan = torch.isnan(out.cpu())
+    want = torch.zeros_like(nan)
+    want[0, 0, :Hq // Hkv] = True
+    assert torch.equal(nan, want), int(nan.sum())
