@@ -659,7 +659,12 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) qfac[nt][e] = f * __shfl_sync(0xffffffffu, row_inv[nt], (2 * c + e) * 4);
+        for (int e = 0; e < 2; ++e) {
+          // not 0, whose product with a masked key's -infinity is NaN (the
+          // smallest normal number does not change logits that are 0 to 2^-90)
+          const float x = f * __shfl_sync(0xffffffffu, row_inv[nt], (2 * c + e) * 4);
+          qfac[nt][e] = x < 1.17549435e-38f ? 1.17549435e-38f : x;
+        }
     }
 
     float acc[MT][NT][4];

@@ -567,3 +567,14 @@ def test_nan_of_a_partial_without_weight(D, Hq, Hkv):
     want = torch.zeros_like(nan)
     want[0, 0, :Hq // Hkv] = True
     assert torch.equal(nan, want), int(nan.sum())
+
+
+def test_logit_factors_below_the_smallest_number():
+    """Rows near bf16's smallest numbers times tiny head scales: the factor of
+    the scaled products is below fp32's range, the logits are 0 to any
+    precision, and the masked keys of the last tile stay masked."""
+    t = make([300, 45, 1, 129, 0], 8, 2, page=16, seed=4)
+    t["q"] = (t["q"].float() * 4e-38).bfloat16()
+    t["ks"][:] = 1e-12
+    out, lse = call(on_gpu(t))
+    check(out, lse, reference(t))
