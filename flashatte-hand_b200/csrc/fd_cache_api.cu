@@ -367,7 +367,7 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
   const int64_t row_tiles = (qrows + rows - 1) / rows;
   // neighbouring KV heads of a token are read together where their count allows
   const int heads = num_heads_k % 2 == 0 ? 2 : 1;
-  const int64_t vheads = num_heads_k / heads * row_tiles;
+  const int64_t head_sets = num_heads_k / heads;
   const int grid_max = fd::fp4_max_grid(D, rows, sms);
   const int64_t nb_max = batch_size < fd::kMaxBatchPerLaunch ? batch_size : fd::kMaxBatchPerLaunch;
   const fd::WorkspaceLayout wl = fp4_workspace(nb_max, num_heads_k, qrows, rows, grid_max, D);
@@ -392,9 +392,18 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
   const int lead = cost_seg4();
   const int64_t per_seq_cost = lead + ((kv_max * heads + fd::kTileTokens - 1) / fd::kTileTokens + 1) *
                                                  (8 + static_cast<int64_t>(cost_tile4()));
-  const int64_t aligned_cost = lead + static_cast<int64_t>(align_tiles4()) * (8 + cost_tile4()) + 1;
-  const int64_t per_launch = fd::seqs_per_launch(per_seq_cost, aligned_cost, num_heads_k * row_tiles, grid_max);
-  if (per_launch == 0) return report_error(FD_ERR_UNSUPPORTED, "sequence too long");
+  // (whole pairs are taken a head at a time: `heads` as many)
+  const int64_t aligned_cost = heads * (lead + static_cast<int64_t>(align_tiles4()) * (8 + cost_tile4()) + 1);
+  int64_t tiles_per_launch = row_tiles;
+  int64_t per_launch = fd::seqs_per_launch(per_seq_cost, aligned_cost, head_sets * row_tiles, grid_max);
+  if (per_launch == 0) {  // not one sequence's rows: as many of its row tiles as fit, a launch each
+    tiles_per_launch = fd::seqs_per_launch(per_seq_cost, aligned_cost, head_sets, grid_max);
+    if (tiles_per_launch > row_tiles) tiles_per_launch = row_tiles;
+    per_launch = 1;
+  }
+  if (tiles_per_launch == 0)
+    return report_error(FD_ERR_UNSUPPORTED, "a block table of %lld tokens is too wide for %lld KV heads",
+                        (long long)rows_max, (long long)num_heads_k);
 
   int len_add = 0;
   if (k_new != nullptr) {  // everything the attention would refuse has been checked
@@ -407,46 +416,50 @@ int fd_decode_paged_fp4(const void* q, void* k_cache, void* v_cache, void* k_blo
   const int64_t es = 2, oes = out_dtype == FD_DTYPE_FP32 ? 4 : 2;
   for (int64_t b0 = 0; b0 < batch_size; b0 += per_launch) {
     const int64_t nb = batch_size - b0 < per_launch ? batch_size - b0 : per_launch;
-    fd::Fp4DecodeParams p{};
-    p.q = static_cast<const uint8_t*>(q) + b0 * seqlen_q * num_heads * headdim * es;
-    p.k_cache = static_cast<const uint8_t*>(k_cache);
-    p.v_cache = static_cast<const uint8_t*>(v_cache);
-    p.k_block = static_cast<const uint8_t*>(k_block_scale);
-    p.v_block = static_cast<const uint8_t*>(v_block_scale);
-    p.out = static_cast<uint8_t*>(out) + b0 * seqlen_q * num_heads * headdim * oes;
-    p.lse = lse != nullptr ? lse + b0 * num_heads * seqlen_q : nullptr;
-    p.k_scale = k_scale;
-    p.v_scale = v_scale;
-    p.seqlens = cache_seqlens + b0;
-    p.block_table = block_table + b0 * block_table_stride;
-    p.bt_stride = block_table_stride;
-    p.num_blocks = num_blocks;
-    p.batch = static_cast<int>(nb);
-    p.num_heads = static_cast<int>(num_heads);
-    p.num_heads_k = static_cast<int>(num_heads_k);
-    p.group = group;
-    p.page = static_cast<int>(page_block_size);
-    p.seqlen_q = static_cast<int>(seqlen_q);
-    p.causal = causal ? 1 : 0;
-    p.qrows = static_cast<int>(qrows);
-    p.row_tiles = static_cast<int>(row_tiles);
-    p.rows = rows;
-    p.heads = heads;
-    p.len_add = len_add;
-    p.scale_log2 = softmax_scale * 1.4426950408889634f;
-    p.tickets = reinterpret_cast<unsigned long long*>(ws + wl.tickets_off);
-    p.part_lse = reinterpret_cast<float*>(ws + wl.lse_off);
-    p.part_o = reinterpret_cast<float*>(ws + wl.o_off);
-    p.epoch_word = reinterpret_cast<unsigned long long*>(ws + wl.epoch_off);
-    p.err = status;
-    p.cost_tile = cost_tile4();
-    p.cost_seg = lead;
-    p.align_tiles = align_tiles4();
-    p.pdl = fd::pdl_enabled() ? 1 : 0;
-    const int64_t work = nb * vheads * tiles_bound;
-    const int grid = static_cast<int>(work < grid_max ? work : grid_max);
-    const cudaError_t e = fd::launch_decode_fp4(p, D, q_dtype, out_dtype == FD_DTYPE_FP32, grid, cs);
-    if (e != cudaSuccess) return report_error(FD_ERR_CUDA, "e2m1 launch: %s", cudaGetErrorString(e));
+    for (int64_t t0 = 0; t0 < row_tiles; t0 += tiles_per_launch) {
+      const int64_t nt = row_tiles - t0 < tiles_per_launch ? row_tiles - t0 : tiles_per_launch;
+      fd::Fp4DecodeParams p{};
+      p.q = static_cast<const uint8_t*>(q) + b0 * seqlen_q * num_heads * headdim * es;
+      p.k_cache = static_cast<const uint8_t*>(k_cache);
+      p.v_cache = static_cast<const uint8_t*>(v_cache);
+      p.k_block = static_cast<const uint8_t*>(k_block_scale);
+      p.v_block = static_cast<const uint8_t*>(v_block_scale);
+      p.out = static_cast<uint8_t*>(out) + b0 * seqlen_q * num_heads * headdim * oes;
+      p.lse = lse != nullptr ? lse + b0 * num_heads * seqlen_q : nullptr;
+      p.k_scale = k_scale;
+      p.v_scale = v_scale;
+      p.seqlens = cache_seqlens + b0;
+      p.block_table = block_table + b0 * block_table_stride;
+      p.bt_stride = block_table_stride;
+      p.num_blocks = num_blocks;
+      p.batch = static_cast<int>(nb);
+      p.num_heads = static_cast<int>(num_heads);
+      p.num_heads_k = static_cast<int>(num_heads_k);
+      p.group = group;
+      p.page = static_cast<int>(page_block_size);
+      p.seqlen_q = static_cast<int>(seqlen_q);
+      p.causal = causal ? 1 : 0;
+      p.qrows = static_cast<int>(qrows);
+      p.row_tiles = static_cast<int>(nt);
+      p.row_tile0 = static_cast<int>(t0);
+      p.rows = rows;
+      p.heads = heads;
+      p.len_add = len_add;
+      p.scale_log2 = softmax_scale * 1.4426950408889634f;
+      p.tickets = reinterpret_cast<unsigned long long*>(ws + wl.tickets_off);
+      p.part_lse = reinterpret_cast<float*>(ws + wl.lse_off);
+      p.part_o = reinterpret_cast<float*>(ws + wl.o_off);
+      p.epoch_word = reinterpret_cast<unsigned long long*>(ws + wl.epoch_off);
+      p.err = status;
+      p.cost_tile = cost_tile4();
+      p.cost_seg = lead;
+      p.align_tiles = align_tiles4();
+      p.pdl = fd::pdl_enabled() ? 1 : 0;
+      const int64_t work = nb * head_sets * nt * tiles_bound;
+      const int grid = static_cast<int>(work < grid_max ? work : grid_max);
+      const cudaError_t e = fd::launch_decode_fp4(p, D, q_dtype, out_dtype == FD_DTYPE_FP32, grid, cs);
+      if (e != cudaSuccess) return report_error(FD_ERR_CUDA, "e2m1 launch: %s", cudaGetErrorString(e));
+    }
   }
   return fd::report_ok();
 }

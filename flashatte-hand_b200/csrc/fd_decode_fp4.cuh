@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       Place g;
       g.b = x.x;
       g.kvh = x.y / p.row_tiles * HW + hw;
-      g.row_base = (x.y % p.row_tiles) * p.rows;
+      g.row_base = (p.row_tile0 + x.y % p.row_tiles) * p.rows;
       g.nrows = p.qrows - g.row_base < G::kRows ? p.qrows - g.row_base : G::kRows;
       return g;
     };

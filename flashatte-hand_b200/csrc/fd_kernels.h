@@ -164,6 +164,7 @@ struct Fp4DecodeParams {
   int batch, num_heads, num_heads_k, group, page;
   int seqlen_q, causal, qrows;   // qrows = seqlen_q * group
   int row_tiles, rows;           // query rows are taken `rows` at a time, in row_tiles passes
+  int row_tile0;                 // from this one of a sequence on
   int heads;                     // KV heads that a CTA takes together: 2 or 1
   int len_add;
   float scale_log2;

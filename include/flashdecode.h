@@ -240,6 +240,8 @@ int fd_append_kv_paged_fp8(const void* k_new, const void* v_new, void* k_cache, 
  * [B, seqlen_new, Hkv, headdim], or NULL for both).  Supported: headdim 64,
  * 128 or 256, any number of query rows, page a multiple of 16, 16-byte aligned
  * q, out, new rows, caches and block scales (FD_ERR_UNSUPPORTED otherwise).
+ * The query rows are taken 8 or 16 at a time; a table so wide (many millions of
+ * tokens times KV heads) that not even one such pass fits a launch is refused.
  * Rows of the cache behind a sequence's length are never used, and a NaN of a
  * token reaches the query rows that see it only.  Workspace: at least
  * fd_decode_workspace_size_fp4(...) bytes, 256-byte aligned and zero-filled

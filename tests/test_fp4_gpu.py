@@ -578,3 +578,48 @@ def test_logit_factors_below_the_smallest_number():
     t["ks"][:] = 1e-12
     out, lse = call(on_gpu(t))
     check(out, lse, reference(t))
+
+
+def reference_of_many_rows(t, causal):
+    """reference() of a case whose sequences have many query tokens, all rows at
+    once; same formulas."""
+    q = t["q"].double()
+    B, sq, Hq, D = q.shape
+    nb, page, Hkv, _ = t["k"].shape
+    G, scale = Hq // Hkv, 1 / math.sqrt(D)
+    K, V = (dequantize_fp4(t[n].view(torch.uint8), t[n + "b"].view(torch.uint8), t[n + "s"]) for n in ("k", "v"))
+    out, A, W = (torch.zeros((B, sq, Hq, D), dtype=torch.float64) for _ in range(3))
+    E, lse = torch.zeros((B, Hq, sq), dtype=torch.float64), torch.full((B, Hq, sq), -math.inf, dtype=torch.float64)
+    for b, L in enumerate(t["lens"].tolist()):
+        ids = t["bt"][b, :-(-L // page)].long()
+        kb, vb = K[ids].flatten(0, 1)[:L], V[ids].flatten(0, 1)[:L]
+        seen = L - (sq - 1 - torch.arange(sq)) if causal else torch.full((sq,), L)
+        hidden = torch.arange(L)[None, :] >= seen[:, None]
+        for h in range(Hq):
+            k, v, x = kb[:, h // G], vb[:, h // G], q[b, :, h]
+            z = (x @ k.T * scale).masked_fill(hidden, -math.inf)
+            lse[b, h] = torch.logsumexp(z, -1)
+            p = torch.where(hidden, 0.0, torch.exp(z - lse[b, h].clamp(min=-1e300)[:, None]))
+            out[b, :, h], A[b, :, h] = p @ v, p @ v.abs()
+            E[b, h] = (D + 8) * 2.0 ** -24 * (x.abs() @ k.abs().T * scale).amax(-1)
+        W[b] = L * 2.0 ** -25 * vb.abs().amax()
+    return out, lse, A, E, W
+
+
+@pytest.mark.parametrize("lens,sq,Hq,Hkv,D,table_tokens,causal", [
+    ([300], 4096, 32, 8, 128, 16384, False),
+    ([300, 5], 256, 64, 8, 128, 131072, True),
+    ([300], 4096, 32, 8, 128, 131072, True),       # the passes of a sequence in several launches
+    ([40, 200, 7], 500, 14, 2, 64, 4194304, False),
+    ([130, 90], 210, 3, 1, 256, 8388608, True),
+])
+def test_many_query_tokens_under_a_wide_table(lens, sq, Hq, Hkv, D, table_tokens, causal):
+    """The bound of a launch goes by the table's width: rows that one launch
+    cannot take go to the next."""
+    t = make(lens, Hq, Hkv, D=D, page=256, sq=sq, seed=sq)
+    d = on_gpu(t)
+    d["bt"] = torch.full((len(lens), table_tokens // 256), -1, dtype=torch.int32, device="cuda")
+    d["bt"][:, :t["bt"].shape[1]] = t["bt"].cuda()
+    out, lse = call(d, causal=causal)
+    check(out, lse, reference_of_many_rows(t, causal))
+    assert flashdecode.device_status() == 0
