@@ -1062,7 +1062,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
       __syncwarp();
       if (lane == 0) {
         unsigned long long* ticket = p.tickets + static_cast<int64_t>(pair) * HW + hw;
-        last = ticket_add(ticket, *launch_epoch, nseg) ? 1 : 0;
+        last = ticket_add(ticket, pair_stamp(*launch_epoch), nseg) ? 1 : 0;
         // every segment of the pair has counted itself: clear for later launches
         if (last) *reinterpret_cast<volatile unsigned long long*>(ticket) = 0ull;
       }

@@ -879,7 +879,7 @@ __global__ void __launch_bounds__(kSm100Threads, 1)
       named_bar_sync(1, 128);
       if (d == 0) {
         int is_last = 0;
-        if (!*abort_flag) is_last = ticket_arrive(p.tickets + sg.pair, *launch_epoch, sg.nseg) ? 1 : 0;
+        if (!*abort_flag) is_last = ticket_arrive(p.tickets + sg.pair, pair_stamp(*launch_epoch), sg.nseg) ? 1 : 0;
         // Every segment of the pair has counted itself: clear the counter for
         // later launches (nothing else touches it in this one).
         if (is_last) *reinterpret_cast<volatile unsigned long long*>(p.tickets + sg.pair) = 0ull;

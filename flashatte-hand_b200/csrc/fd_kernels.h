@@ -30,7 +30,7 @@ struct DecodeParams {
   float* part_o;              // [slots, group, 128] fp32 (normalised partial O)
   float* part_lse;            // [slots, group] log2-domain partial LSE
   // [batch * num_heads_k] arrival counters of split pairs: bits [12, 64) the
-  // launch epoch, bits [0, 12) the arrivals seen in it.  The CTA that merges
+  // launch's stamp (made of its epoch), bits [0, 12) the arrivals seen under it.  The CTA that merges
   // a pair clears its counter, so a launch that completes leaves them all 0.
   unsigned long long* tickets;
   int* err;                   // the device's status word (first error a kernel met)

@@ -12,42 +12,49 @@ namespace fd {
 namespace {
 
 // Arrival counter of a split (sequence, KV head) pair, and of the grid:
-// bits [12, 64) hold the launch epoch, bits [0, 12) the arrivals seen in that
-// epoch (at most one per CTA, and a launch has at most 4095 CTAs).  Epochs run
-// 1 .. 2^52 - 1 and then start again at 1, so a counter can only be mistaken
-// for the current launch's after 2^52 - 1 launches on one workspace (centuries
-// of back-to-back calls).  Only a launch that stopped early (a bounded wait
-// ran out) leaves a counter behind: the CTA that merges a pair clears its
-// counter and the last CTA to arrive clears the grid counter, so a launch
-// that completes leaves every counter at zero.  The first arrival of a launch
-// stamps the epoch with one compare-and-swap; every arrival that sees the
+// bits [12, 64) hold the launch's stamp, bits [0, 12) the arrivals seen under
+// it (at most one per CTA, and a launch has at most 4095 CTAs).  The grid's
+// stamp is the launch epoch, which runs 1 .. 2^52 - 1 and then starts again at
+// 1.  A pair's counter lies where the partials of a launch of another shape may
+// have been, any two fp32 numbers: its stamp is 12 bits that make the word's
+// upper half a signalling NaN, which no arithmetic gives, and 40 bits of the
+// epoch.  (The epoch alone is two numbers like (1, 0) at launch 0x3F800.)  So a
+// counter can only be mistaken for the current launch's after 2^40 launches on
+// one workspace (months of back-to-back calls), and only one that a launch
+// which stopped early (a bounded wait ran out) left behind: the CTA that merges
+// a pair clears its counter and the last CTA to arrive clears the grid
+// counter, so a launch that completes leaves every counter at zero.  The first arrival of a launch
+// sets the stamp with one compare-and-swap; every arrival that sees the
 // stamp counts itself with one fetch-and-add, so the tens of CTAs sharing one
 // long sequence's pair, finishing together, do not queue on a compare-and-swap
 // loop.  Returns true for the pair's last arrival.
 constexpr int kTicketCountBits = 12;
 constexpr unsigned long long kTicketCountMask = (1ull << kTicketCountBits) - 1ull;
 constexpr unsigned long long kEpochMax = (1ull << (64 - kTicketCountBits)) - 1ull;
-__device__ __forceinline__ bool ticket_arrive(unsigned long long* t, unsigned long long epoch, int nseg) {
+__device__ __forceinline__ unsigned long long pair_stamp(unsigned long long epoch) {
+  return (0xFFAull << 40) | (epoch & ((1ull << 40) - 1ull));
+}
+__device__ __forceinline__ bool ticket_arrive(unsigned long long* t, unsigned long long stamp, int nseg) {
   unsigned long long cur = *reinterpret_cast<volatile unsigned long long*>(t);
   for (;;) {
-    if ((cur >> kTicketCountBits) == epoch) {
+    if ((cur >> kTicketCountBits) == stamp) {
       const unsigned long long old = atomicAdd(t, 1ull);
       return (old & kTicketCountMask) + 1ull == static_cast<unsigned long long>(nseg);
     }
-    const unsigned long long prev = atomicCAS(t, cur, (epoch << kTicketCountBits) | 1ull);
+    const unsigned long long prev = atomicCAS(t, cur, (stamp << kTicketCountBits) | 1ull);
     if (prev == cur) return nseg == 1;
     cur = prev;
   }
 }
 
 // The same arrival in one round trip where the counter already carries the
-// epoch (every arrival of a pair but the first): count first, look after.  A
-// counter of another epoch is only made larger, and is overwritten as above.
-__device__ __forceinline__ bool ticket_add(unsigned long long* t, unsigned long long epoch, int nseg) {
+// stamp (every arrival of a pair but the first): count first, look after.  A
+// counter of another stamp is only made larger, and is overwritten as above.
+__device__ __forceinline__ bool ticket_add(unsigned long long* t, unsigned long long stamp, int nseg) {
   const unsigned long long old = atomicAdd(t, 1ull);
-  if ((old >> kTicketCountBits) == epoch)
+  if ((old >> kTicketCountBits) == stamp)
     return (old & kTicketCountMask) + 1ull == static_cast<unsigned long long>(nseg);
-  return ticket_arrive(t, epoch, nseg);
+  return ticket_arrive(t, stamp, nseg);
 }
 
 // ---------------------------------------------------------------- schedule

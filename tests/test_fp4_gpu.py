@@ -623,3 +623,21 @@ def test_many_query_tokens_under_a_wide_table(lens, sq, Hq, Hkv, D, table_tokens
     out, lse = call(d, causal=causal)
     check(out, lse, reference_of_many_rows(t, causal))
     assert flashdecode.device_status() == 0
+
+
+def test_partials_of_another_shape_are_no_counters():
+    """The workspace's arrival counters (from byte 128; the launch epoch in the
+    first word) may hold what a launch of another shape left there as partials:
+    (x, 0), whose upper bits are the epoch and whose lower ones a count."""
+    t = make([5000, 17, 9000, 0, 300, 2049], 32, 8, seed=5)
+    d = on_gpu(t)
+    want = call(d)
+    check(*want, reference(t))
+    n = flashdecode.workspace_size(6, 32, 8, 128, kv_dtype=FP4)
+    ws = torch.zeros((n,), dtype=torch.uint8, device="cuda")
+    for x in (1.0 + 2.0 ** -23, 0.7 + 3 * 2.0 ** -24, 1e-30):
+        stale = torch.tensor([x, 0.0], dtype=torch.float32, device="cuda").repeat(6 * 8)
+        ws[:8].view(torch.int64)[0] = int(stale[0].view(torch.int32)) >> 12
+        ws[128:128 + 8 * 6 * 8].view(torch.float32).copy_(stale)
+        out, lse = call(d, workspace=ws)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])

@@ -218,3 +218,21 @@ def test_append_into_an_unallocated_page_is_reported():
     assert lib.fd_device_status() == FD_ERR_BAD_PAGE
     assert torch.equal(t["k_cache"].cpu(), kc_ref) and torch.equal(t["v_cache"].cpu(), vc_ref)
     assert lib.fd_device_status() == 0
+
+
+def test_partials_of_another_shape_are_no_counters():
+    """The counters of a large batch lie where a smaller one's partials were:
+    the bits of two fp32 numbers.  (x, 0) with the launch's epoch in x's upper
+    bits and a count in its lower ones must not pass for arrivals."""
+    c, t = _split_case()
+    n = flashdecode.workspace_size(c.B, c.Hq, c.Hkv)
+    ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    tick = ws[TICKETS_OFF:TICKETS_OFF + 8 * c.B * c.Hkv]
+    ref_o, ref_l = oracle(t, c)
+    for x in (1.0 + 2.0 ** -23, 0.7 + 3 * 2.0 ** -24, 1e-30):
+        stale = torch.tensor([x, 0.0], dtype=torch.float32, device="cuda").repeat(c.B * c.Hkv)
+        ws[:8].view(torch.int64)[0] = int(stale[0].view(torch.int32)) >> 12
+        tick.view(torch.float32).copy_(stale)
+        out, lse = run(t, c, workspace=ws)
+        torch.cuda.synchronize()
+        check(out, lse, ref_o, ref_l, f"stale {x}")
