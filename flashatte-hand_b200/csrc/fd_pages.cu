@@ -380,34 +380,45 @@ __global__ void __launch_bounds__(kReleaseThreads) release_pages_kernel(const Re
   }
 }
 
-// Dynamic shared memory above the default limit has to be allowed once per device.
-template <typename K>
-cudaError_t allow_smem(K kernel, size_t bytes) {
-  return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                  static_cast<int>(bytes))
-                           : cudaSuccess;
+constexpr size_t assign_smem(int batch) { return (3 * static_cast<size_t>(batch) + 2) * sizeof(int); }
+constexpr size_t release_smem(int batch) { return (2 * static_cast<size_t>(batch) + 1) * sizeof(int); }
+
+// Shared memory above the default limit (static and dynamic together) has to be
+// allowed, once per device: what the largest call takes, so that no call lowers
+// the limit under another thread's.
+cudaError_t allow_smem(const void* kernel, size_t most, unsigned long long* allowed) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if ((__atomic_load_n(allowed, __ATOMIC_ACQUIRE) & bit) != 0) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+  if (e == cudaSuccess) __atomic_fetch_or(allowed, bit, __ATOMIC_RELEASE);
+  return e;
 }
 
 }  // namespace
 
 cudaError_t launch_assign_pages(const AssignPagesParams& p, int sms, cudaStream_t stream) {
-  const size_t smem = (3 * static_cast<size_t>(p.batch) + 2) * sizeof(int);
-  cudaError_t e = allow_smem(assign_pages_kernel, smem);
+  static unsigned long long allowed = 0;
+  const cudaError_t e =
+      allow_smem(reinterpret_cast<const void*>(assign_pages_kernel), assign_smem(kMaxPagedRequests), &allowed);
   if (e != cudaSuccess) return e;
   int64_t grid = (p.num_slots + 4 * kPagesThreads - 1) / (4 * kPagesThreads);
   grid = grid < 1 ? 1 : (grid < 2 * sms ? grid : 2 * sms);
-  assign_pages_kernel<<<static_cast<unsigned>(grid), kPagesThreads, smem, stream>>>(p);
+  assign_pages_kernel<<<static_cast<unsigned>(grid), kPagesThreads, assign_smem(p.batch), stream>>>(p);
   return cudaGetLastError();
 }
 
 cudaError_t launch_release_pages(const ReleasePagesParams& p, int sms, cudaStream_t stream) {
-  const size_t smem = (2 * static_cast<size_t>(p.batch) + 1) * sizeof(int);
-  cudaError_t e = allow_smem(release_pages_kernel, smem);
+  static unsigned long long allowed = 0;
+  const cudaError_t e =
+      allow_smem(reinterpret_cast<const void*>(release_pages_kernel), release_smem(kMaxPagedRequests), &allowed);
   if (e != cudaSuccess) return e;
   // a CTA for every 8 pages of a thread that the table could hold
   const int64_t most = (p.batch * p.bt_stride + 8 * kReleaseThreads - 1) / (8 * kReleaseThreads);
   const unsigned grid = static_cast<unsigned>(most < sms ? most : sms);
-  release_pages_kernel<<<grid, kReleaseThreads, smem, stream>>>(p);
+  release_pages_kernel<<<grid, kReleaseThreads, release_smem(p.batch), stream>>>(p);
   return cudaGetLastError();
 }
 

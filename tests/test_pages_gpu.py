@@ -1,5 +1,9 @@
 """Block tables and slot maps on the GPU against plain loops: all whole
 numbers, compared exactly."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -205,3 +209,36 @@ def test_refusals():
     with pytest.raises(ValueError):
         flashdecode.release_pages(s["table"], s["lens"], s["lens"].long(), s["pool"], s["count"], 16)
     assert s["count"].tolist() == [5, 0]
+
+
+REQUESTS_AROUND_48_KB = """
+import sys
+import torch
+sys.path[:0] = [{root!r}, {root!r} + "/flashatte-hand_b200"]
+import flashdecode
+i32 = dict(dtype=torch.int32, device="cuda")
+for what, B in {calls}:
+    table, lens = torch.arange(B, **i32)[:, None].contiguous(), torch.ones(B, **i32)
+    pool, count = torch.zeros(B, **i32), torch.zeros(2, **i32)
+    if what == "assign":
+        slots, cu, after = flashdecode.assign_pages(table, lens, lens, pool, count, 16, num_slots=B)
+        assert torch.equal(slots, torch.arange(B, device="cuda") * 16 + 1) and bool((after == 2).all())
+    else:
+        flashdecode.release_pages(table, lens, torch.zeros_like(lens), pool, count, 16)
+        assert count.tolist() == [B, 0] and bool((table == -1).all())
+        assert torch.equal(pool, torch.arange(B, **i32).flip(0))
+"""
+
+
+@pytest.mark.parametrize("calls", [
+    [("assign", b) for b in (4083, 4084, 4085, 4095, 4096, 8192, 1)],
+    [("release", b) for b in (6110, 6111, 6112, 6143, 6144, 8192, 1)],
+])
+def test_requests_around_the_default_limit_of_shared_memory(calls):
+    """12 B + 8 and 8 B + 4 bytes of dynamic shared memory, which with the
+    kernels' static arrays pass 48 KB a little before the dynamic part does; in
+    a process of its own, in which no larger call came before."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", REQUESTS_AROUND_48_KB.format(root=root, calls=calls)],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
