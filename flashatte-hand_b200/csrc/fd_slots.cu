@@ -95,10 +95,12 @@ __device__ __forceinline__ Place place_of_row(const SlotParams& p, int64_t r, bo
 // x / d, correctly rounded, for r = 1 / d correctly rounded and nothing near
 // the ends of the range: one Newton correction of x r with the exact
 // remainder (Markstein's theorem).  Rounding to e2m1 then sees the tie cases
-// exactly, which a plain product with the reciprocal would miss.
+// exactly, which a plain product with the reciprocal would miss.  The remainder
+// is taken with its sign turned: +0 for x = +0 and -0 alike, so that -0 keeps
+// its sign (x - q d would add +0 to it).
 __device__ __forceinline__ float divide(float x, float d, float r) {
   const float q = x * r;
-  return fmaf(fmaf(-q, d, x), r, q);
+  return fmaf(-fmaf(q, d, -x), r, q);
 }
 
 __device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {

@@ -277,3 +277,22 @@ def test_dense_append_matches_the_slot_append(page):
     slots = torch.where(pos // page < 1, short.long() * page + pos % page, -1)
     check("fp4", c, kw, before, k.flatten(0, 1), v.flatten(0, 1), slots.flatten())
     assert flashdecode.device_status() == 0
+
+
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+def test_zeros_keep_their_sign_among_other_values(src):
+    c, kw = make_cache("fp4", 4, 16, 2, 64, src)
+    g = torch.Generator().manual_seed(0)
+    k, v = (torch.randn((20, 2, 64), generator=g) for _ in range(2))
+    for x in (k, v):
+        x[torch.rand(x.shape, generator=g) < 0.3] = -0.0
+        x[torch.rand(x.shape, generator=g) < 0.2] = 0.0
+    k, v = k.to(src).cuda(), v.to(src).cuda()
+    slots = torch.randperm(64, generator=g)[:20].cuda()
+    before = clone(c)
+    flashdecode.append_kv_slots(k, v, c["k"], c["v"], slots, **kw)
+    torch.cuda.synchronize()
+    check("fp4", c, kw, before, k, v, slots)
+    val, _ = flashdecode.gather_kv(c["k"], c["v"], slots, out_dtype=torch.float32, **kw)
+    zero = k == 0
+    assert torch.equal(torch.signbit(val)[zero], torch.signbit(k)[zero])
