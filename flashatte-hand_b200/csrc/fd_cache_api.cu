@@ -101,6 +101,7 @@ int append_rows(fd::SlotParams p, int src_dtype, int cache_dtype, cudaStream_t s
                         "quantised append: head dim must be a multiple of 16, rows and caches "
                         "16-byte aligned");
   if (p.rows > INT32_MAX) return report_error(FD_ERR_UNSUPPORTED, "size exceeds 32-bit index range");
+  if (p.sms <= 0) return report_error(FD_ERR_CUDA, "cannot query SM count");
   const cudaError_t e = wide ? fd::launch_append_slots(p, src_dtype, cache_dtype, stream)
                              : fd::launch_append_slots_narrow(p, stream);
   if (e != cudaSuccess) return report_error(FD_ERR_CUDA, "append launch: %s", cudaGetErrorString(e));
@@ -173,6 +174,7 @@ int fd_gather_kv_slots(const void* k_cache, const void* v_cache, const void* k_b
                                  const_cast<void*>(k_block_scale), const_cast<void*>(v_block_scale),
                                  k_scale, v_scale, num_heads_k, headdim, page_block_size, num_blocks,
                                  dev, status);
+  if (p.sms <= 0) return report_error(FD_ERR_CUDA, "cannot query SM count");
   p.k_out = k_out;
   p.v_out = v_out;
   p.slot_map = slot_map;

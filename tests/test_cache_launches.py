@@ -69,3 +69,12 @@ def test_launches_cover_every_row(host, B, sq, Hq, Hkv, D, page, width, launches
 def test_a_table_too_wide_for_one_pass_is_refused(host):
     status, lines = host(148, "decode", 1, 1, 512, 512, 128, 256, 1 << 21)
     assert status == 2 and "too wide" in lines[0]
+
+
+@pytest.mark.parametrize("call", ["append", "append_paged", "gather"])
+def test_no_count_of_the_sms_is_an_error(host, call):
+    """The launchers divide by it."""
+    status, lines = host(0, call)
+    assert status == 4 and lines == ["cannot query SM count"]
+    status, lines = host(148, call)
+    assert status == 0 and lines[0].endswith("sms 148")
