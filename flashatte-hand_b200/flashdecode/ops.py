@@ -23,8 +23,13 @@ from ._lib import (FD_DTYPE_BF16, FD_DTYPE_E2M1, FD_DTYPE_E4M3, FD_DTYPE_FP16, F
                    FlashDecodeError, check, load_library)
 
 _DTYPES = {torch.bfloat16: FD_DTYPE_BF16, torch.float16: FD_DTYPE_FP16}
+# the codes' type of 4-bit caches, where torch has it: calls over other caches
+# do not need it
+_FP4 = getattr(torch, "float4_e2m1fn_x2", None)
 _CACHE_DTYPES = {torch.bfloat16: FD_DTYPE_BF16, torch.float16: FD_DTYPE_FP16,
-                 torch.float8_e4m3fn: FD_DTYPE_E4M3, torch.float4_e2m1fn_x2: FD_DTYPE_E2M1}
+                 torch.float8_e4m3fn: FD_DTYPE_E4M3}
+if _FP4 is not None:
+    _CACHE_DTYPES[_FP4] = FD_DTYPE_E2M1
 _INT32 = torch.int32
 _OUT_DTYPES = {torch.bfloat16: FD_DTYPE_BF16, torch.float16: FD_DTYPE_FP16, torch.float32: FD_DTYPE_FP32}
 
@@ -115,7 +120,7 @@ def workspace_size(batch_size: int, num_heads: int, num_heads_k: int, headdim: i
     """Bytes of workspace that flash_decode needs (kv_dtype: that of the
     caches, to be given for float4_e2m1fn_x2)."""
     lib = load_library()
-    size = lib.fd_decode_workspace_size_fp4 if kv_dtype == torch.float4_e2m1fn_x2 \
+    size = lib.fd_decode_workspace_size_fp4 if kv_dtype is not None and kv_dtype == _FP4 \
         else lib.fd_decode_workspace_size_mq
     return int(size(batch_size, seqlen_q, num_heads, num_heads_k, headdim))
 
@@ -187,7 +192,7 @@ def _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, ret
     if q.dim() != 4:
         raise ValueError(f"q must be [B, seqlen_q, Hq, D], got {tuple(q.shape)}")
     kv8 = k_cache.dtype == torch.float8_e4m3fn
-    kv4 = k_cache.dtype == torch.float4_e2m1fn_x2
+    kv4 = k_cache.dtype == _FP4
     if q.dtype not in _DTYPES or v_cache.dtype != k_cache.dtype \
             or not (kv8 or kv4 or k_cache.dtype == q.dtype):
         raise ValueError("q, k_cache, v_cache must share dtype bf16 or fp16 (or e4m3 or e2m1 caches)")
@@ -314,7 +319,7 @@ def _check_scales(k_scale, v_scale, Hkv: int) -> None:
 
 def _check_block_scales(k_block_scale, v_block_scale, k_cache: torch.Tensor) -> None:
     """Block scales are given exactly with a 4-bit cache, in its shape."""
-    if k_cache.dtype != torch.float4_e2m1fn_x2:
+    if k_cache.dtype != _FP4:
         if k_block_scale is not None or v_block_scale is not None:
             raise ValueError("k_block_scale / v_block_scale apply to float4_e2m1fn_x2 caches only")
         return
@@ -336,7 +341,7 @@ def _check_new_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, B: in
     _require_cuda(k, v)
     if k.dim() != 4 or tuple(v.shape) != tuple(k.shape):
         raise ValueError("k and v must both be [B, seqlen_new, Hkv, D]")
-    D = k_cache.shape[3] * (2 if k_cache.dtype == torch.float4_e2m1fn_x2 else 1)
+    D = k_cache.shape[3] * (2 if k_cache.dtype == _FP4 else 1)
     if k.shape[0] != B or k.shape[2] != k_cache.shape[2] or k.shape[3] != D:
         raise ValueError("k / v shape does not match the batch and cache heads")
     want = k_cache.dtype if new_dtype is None else new_dtype
@@ -371,7 +376,7 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     num_blocks, page, Hkv, D = k_cache.shape
     _check_block_scales(k_block_scale, v_block_scale, k_cache)
     st = stream if stream is not None else torch.cuda.current_stream(k.device)
-    if k_cache.dtype == torch.float4_e2m1fn_x2:
+    if k_cache.dtype == _FP4:
         _check_scales(k_scale, v_scale, Hkv)
         if k.dtype not in _DTYPES:
             raise ValueError("k / v must be bf16 or fp16")
@@ -428,7 +433,7 @@ def _check_slot_cache(k_cache, v_cache, slot_map, k_scale, v_scale, k_block_scal
     else:
         _check_scales(k_scale, v_scale, Hkv)
     _check_block_scales(k_block_scale, v_block_scale, k_cache)
-    return slots[0], page, Hkv, 2 * D if dtype == torch.float4_e2m1fn_x2 else D, num_blocks
+    return slots[0], page, Hkv, 2 * D if dtype == _FP4 else D, num_blocks
 
 
 def append_kv_slots(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,

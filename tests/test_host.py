@@ -1,11 +1,16 @@
 """CPU checks of the host-side logic: workload layouts and the split scheduler
 model (the same partition the kernel computes on the device)."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
 
 from flashdecode import cases, schedule
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def test_config2_matches_baseline_sizes():
@@ -264,3 +269,29 @@ def test_behind_lead_schedule_covers_every_tile_once(seed, grid, seg):
                 continue
             assert [s.cta for s in ss] == list(range(ss[0].cfirst, ss[0].cfirst + ss[0].nseg))
             assert all((s.nseg, s.cfirst) == (ss[0].nseg, ss[0].cfirst) for s in ss)
+
+
+def test_a_torch_without_the_4_bit_type():
+    """Calls over 16-bit and e4m3 caches, which need none, work without it."""
+    code = """
+import sys, torch
+del torch.float4_e2m1fn_x2
+sys.path[:0] = sys.argv[1:]
+import flashdecode
+from flashdecode import ops
+ops._require_cuda = lambda *t: None
+flashdecode.workspace_size(2, 8, 2)
+i32 = dict(dtype=torch.int32)
+q = torch.zeros((1, 1, 8, 128), dtype=torch.bfloat16)
+new = torch.zeros((1, 1, 2, 128), dtype=torch.bfloat16)
+lens, table, sc = torch.ones(1, **i32), torch.zeros((1, 1), **i32), torch.ones(2)
+for dtype, scales in ((torch.bfloat16, (None, None)), (torch.float8_e4m3fn, (sc, sc))):
+    c = torch.zeros((1, 16, 2, 128), dtype=torch.bfloat16).to(dtype)
+    for k in (None, new):
+        call = ops._prepare(q, c, c, lens, table, None, False, None, None, None, None, None, False, k, k, *scales)
+        assert call.out.shape == q.shape
+    assert ops._check_slot_cache(c, c, torch.zeros(3, dtype=torch.int64), *scales, None, None) == (3, 16, 2, 128, 1)
+"""
+    r = subprocess.run([sys.executable, "-c", code, ROOT, os.path.join(ROOT, "flashatte-hand_b200")],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
