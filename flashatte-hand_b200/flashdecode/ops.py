@@ -76,6 +76,19 @@ def _launch(fn, dev: torch.device, stream, args) -> None:
         check(status)
 
 
+def _new(shape, dtype: torch.dtype, dev: torch.device, stream=None) -> torch.Tensor:
+    """An output tensor.  One that a kernel on `stream` writes is allocated
+    there: a block of the current stream's pool may still be read by work
+    queued on that stream for its last owner.  The current stream, where the
+    caller may use and drop it, is recorded."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=dev)
+    t.record_stream(torch.cuda.current_stream(dev))
+    return t
+
+
 def _require_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if not t.is_cuda:
@@ -166,7 +179,7 @@ def flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     """
     call = _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale,
                     return_softmax_lse, out, out_dtype, max_seqlen_k, workspace, lse, causal, k, v,
-                    k_scale, v_scale, k_block_scale, v_block_scale)
+                    k_scale, v_scale, k_block_scale, v_block_scale, stream)
     with _on_device(q.device):
         check(call.fn(*call.args, _stream_handle(stream, q.device)))
     return (call.out, call.lse) if call.return_lse else call.out
@@ -184,9 +197,10 @@ class _Call:
 
 def _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, return_softmax_lse,
              out, out_dtype, max_seqlen_k, workspace, lse, causal, k, v, k_scale, v_scale,
-             k_block_scale=None, v_block_scale=None) -> _Call:
+             k_block_scale=None, v_block_scale=None, stream=None) -> _Call:
     """Check the arguments of flash_decode, allocate the outputs it was not
-    given and bind the C entry point that serves them."""
+    given (for a kernel on `stream`) and bind the C entry point that serves
+    them."""
     lib = load_library()
     _require_cuda(q, k_cache, v_cache, cache_seqlens, block_table)
     if q.dim() != 4:
@@ -216,7 +230,7 @@ def _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, ret
     scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
     odt = q.dtype if out_dtype is None else out_dtype
     if out is None:
-        out = torch.empty((B, sq, Hq, D), dtype=odt, device=q.device)
+        out = _new((B, sq, Hq, D), odt, q.device, stream)
     elif out.dtype != odt or tuple(out.shape) != (B, sq, Hq, D) or not out.is_contiguous():
         raise ValueError("out has the wrong shape, dtype or layout")
     lse_shape = (B, Hq) if sq == 1 else (B, Hq, sq)
@@ -225,7 +239,7 @@ def _prepare(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, ret
             raise ValueError(f"lse must be a contiguous fp32 {lse_shape} tensor")
         return_softmax_lse = True
     elif return_softmax_lse:
-        lse = torch.empty(lse_shape, dtype=torch.float32, device=q.device)
+        lse = _new(lse_shape, torch.float32, q.device, stream)
     ws_ptr, ws_bytes = None, 0
     if workspace is not None:
         ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
@@ -497,9 +511,9 @@ def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_map: torch.Tens
         if x is not None and (x.dtype != out_dtype or x.shape != want or not x.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous {out_dtype} {want} CUDA tensor")
     if k_out is None:
-        k_out = torch.empty(T, Hkv, D, dtype=out_dtype, device=dev)
+        k_out = _new(want, out_dtype, dev, stream)
     if v_out is None:
-        v_out = torch.empty_like(k_out)
+        v_out = _new(want, out_dtype, dev, stream)
     _launch(lib.fd_gather_kv_slots, dev, stream, (
         k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_block_scale), _ptr(v_block_scale),
         _ptr(k_scale), _ptr(v_scale), slot_map.data_ptr(), T, k_out.data_ptr(), v_out.data_ptr(),
@@ -559,18 +573,18 @@ def assign_pages(block_table: torch.Tensor, cache_seqlens: torch.Tensor, new_len
         if num_slots is None:
             raise ValueError("give slot_map or num_slots")
         num_slots = int(num_slots)
-        slot_map = torch.empty(num_slots, dtype=torch.int64, device=dev)
+        slot_map = _new(num_slots, torch.int64, dev, stream)
     else:
         slots = slot_map.shape
         if slot_map.dtype != torch.int64 or len(slots) != 1 or not slot_map.is_contiguous():
             raise ValueError("slot_map must be a contiguous int64 [num_slots] CUDA tensor")
         num_slots = slots[0]
     if cu_new_lens is None:
-        cu_new_lens = new_lens.new_empty(B + 1)
+        cu_new_lens = _new(B + 1, _INT32, dev, stream)
     else:
         _check_int32("cu_new_lens", cu_new_lens, (B + 1,))
     if seqlens_out is None:
-        seqlens_out = torch.empty_like(cache_seqlens)
+        seqlens_out = _new(B, _INT32, dev, stream)
     else:
         _check_int32("seqlens_out", seqlens_out, (B,))
     _launch(lib.fd_assign_pages, dev, stream, (
@@ -612,13 +626,14 @@ def combine_lse(part_o: torch.Tensor, part_lse: torch.Tensor, out_dtype: torch.d
     if part_o.dtype != torch.float32 or part_lse.dtype != torch.float32:
         raise ValueError("partials must be fp32")
     n, rows, D = part_o.shape
-    if part_o.stride()[1:] != (D, 1):
-        part_o = part_o.contiguous()
-    if part_lse.stride(1) != 1:
-        part_lse = part_lse.contiguous()
-    out = torch.empty((rows, D), dtype=out_dtype, device=part_o.device)
-    lse = torch.empty((rows,), dtype=torch.float32, device=part_o.device) if return_lse else None
     st = stream if stream is not None else torch.cuda.current_stream(part_o.device)
+    with torch.cuda.stream(st):  # copies are read by the kernel on this stream
+        if part_o.stride()[1:] != (D, 1):
+            part_o = part_o.contiguous()
+        if part_lse.stride(1) != 1:
+            part_lse = part_lse.contiguous()
+    out = _new((rows, D), out_dtype, part_o.device, stream)
+    lse = _new((rows,), torch.float32, part_o.device, stream) if return_lse else None
     with torch.cuda.device(part_o.device):
         status = lib.fd_combine_lse(_ptr(part_o), part_o.stride(0), _ptr(part_lse), part_lse.stride(0),
                                     n, rows, D, _ptr(out), _OUT_DTYPES[out_dtype], _ptr(lse),
