@@ -641,3 +641,70 @@ def test_partials_of_another_shape_are_no_counters():
         ws[128:128 + 8 * 6 * 8].view(torch.float32).copy_(stale)
         out, lse = call(d, workspace=ws)
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+def test_whole_step_captured():
+    """Pages, slots, append, decode over the new lengths, the step's rows read
+    back, and the release of what is not kept: one graph on fixed buffers,
+    replayed with other lengths, rows, queries and numbers of tokens kept."""
+    page, B, Hq, Hkv, D, room, sq = 16, 4, 8, 2, 128, 70, 1
+    t = make([0] * B, Hq, Hkv, page=page, seed=21, pool_extra=60)
+    d = on_gpu(t)
+    nb = d["k"].shape[0]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table, lens, after = torch.full((B, 12), -1, **i32), torch.zeros(B, **i32), torch.zeros(B, **i32)
+    new, keep, cu = torch.zeros(B, **i32), torch.zeros(B, **i32), torch.zeros(B + 1, **i32)
+    pool, count = torch.arange(nb, **i32), torch.tensor([nb, 0], **i32)
+    slots = torch.zeros(room, dtype=torch.int64, device="cuda")
+    k, v = (torch.zeros((room, Hkv, D), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    back = [torch.zeros((room, Hkv, D), device="cuda") for _ in range(2)]
+    kw = dict(k_scale=d["ks"], v_scale=d["vs"], k_block_scale=d["kb"], v_block_scale=d["vb"])
+    q = torch.zeros((B, sq, Hq, D), dtype=torch.bfloat16, device="cuda")
+    plan = flashdecode.DecodePlan(q, d["k"], d["v"], after, table, return_softmax_lse=True, **kw)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        flashdecode.assign_pages(table, lens, new, pool, count, page, slot_map=slots, cu_new_lens=cu,
+                                 seqlens_out=after)
+        flashdecode.append_kv_slots(k, v, d["k"], d["v"], slots, **kw)
+        plan()
+        flashdecode.gather_kv(d["k"], d["v"], slots, out_dtype=torch.float32, k_out=back[0], v_out=back[1], **kw)
+        flashdecode.release_pages(table, after, keep, pool, count, page)
+        lens.copy_(keep)
+    g = torch.Generator().manual_seed(3)
+    held = [[[], []] for _ in range(B)]
+    for step, (add, kept) in enumerate([([30, 0, 5, 16], [30, 0, 5, 16]), ([1, 1, 1, 1], [1, 1, 1, 1]),
+                                        ([4, 4, 4, 4], [4, 1, 0, 3]), ([4, 20, 4, 4], [0, 20, 2, 4]),
+                                        ([1, 1, 40, 1], [1, None, 40, 1]), ([1, 60, 1, 1], [1, 60, 1, 1])]):
+        x = [torch.randn((room, Hkv, D), generator=g).bfloat16() for _ in range(2)]
+        qs = torch.randn(q.shape, generator=g).bfloat16()
+        before = [len(h[0]) for h in held]
+        stay = [0 if n is None else m + n for m, n in zip(before, kept)]       # None: the request leaves
+        for dst, src in ((k, x[0]), (v, x[1]), (q, qs), (new, torch.tensor(add, dtype=torch.int32)),
+                         (keep, torch.tensor(stay, dtype=torch.int32))):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert cu.tolist() == [sum(add[:b]) for b in range(B + 1)]
+        for b in range(B):
+            for i in range(2):
+                held[b][i] += list(x[i][int(cu[b]):int(cu[b + 1])])
+        L = [len(h[0]) for h in held]
+        assert after.tolist() == L
+        ref = dict(q=qs, lens=torch.tensor(L), bt=torch.arange(B)[:, None], ks=t["ks"], vs=t["vs"])
+        for i, name in enumerate("kv"):
+            rows = torch.zeros((B, max(L), Hkv, D), dtype=torch.bfloat16)
+            for b in range(B):
+                for j, row in enumerate(held[b][i]):
+                    rows[b, j] = row
+            ref[name], blocks = quantize_fp4(rows, t[name + "s"])
+            ref[name + "b"] = blocks.permute(0, 2, 1, 3).contiguous()
+            codes, blocks = quantize_fp4(x[i], t[name + "s"])
+            want = dequantize_fp4(codes[:, None], blocks[:, None].transpose(1, 2), t[name + "s"], torch.float32)[:, 0]
+            want[sum(add):] = 0                                                # slots -1
+            assert torch.equal(back[i].cpu(), want)
+        check(plan.out, plan.lse, reference(ref))
+        for b in range(B):
+            held[b] = [h[:stay[b]] for h in held[b]]
+        assert lens.tolist() == stay and count.tolist() == [nb - sum(-(-n // page) for n in stay), 0]
+        assert [(row >= 0).sum().item() for row in table] == [-(-n // page) for n in stay]
+    assert flashdecode.device_status() == 0
