@@ -708,3 +708,23 @@ def test_whole_step_captured():
         assert lens.tolist() == stay and count.tolist() == [nb - sum(-(-n // page) for n in stay), 0]
         assert [(row >= 0).sum().item() for row in table] == [-(-n // page) for n in stay]
     assert flashdecode.device_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Hq,Hkv,sq", [(2, 2, 4), (3, 3, 3), (4, 2, 2), (2, 1, 2)])
+def test_few_rows_of_several_query_tokens(D, Hq, Hkv, sq):
+    """Up to four rows in all, twice in a tile's columns: causal masks inside a
+    page, a NaN of V that only the last rows see, a sequence over many CTAs."""
+    seqlens = [sq, 1, 0, 63, 130, 20000]
+    t = make(seqlens, Hq, Hkv, D=D, page=16, sq=sq, seed=D + sq, dtype=torch.float16)
+    clean = {n: x.clone() for n, x in t.items()}
+    at = 129
+    t["vb"][int(t["bt"][4, at // 16]), 0, at % 16, 1] = 0x7F
+    for out_dtype in (None, torch.float32):
+        out, lse = call(on_gpu(t), causal=True, out_dtype=out_dtype)
+        ref = reference(clean, causal=True)
+        nan = torch.isnan(out.cpu())
+        want = torch.zeros_like(nan)
+        want[4, sq - 1, :Hq // Hkv, 16:32] = True
+        assert torch.equal(nan, want)
+        check(torch.where(nan, ref[0].to(out.dtype), out.cpu()), lse, ref)
