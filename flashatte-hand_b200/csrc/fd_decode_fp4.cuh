@@ -1094,6 +1094,10 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
 #pragma unroll 1
     for (int row0 = row_tw; row0 < nrows; row0 += kAt * row_ways) {
       float mm = neg_inf, den = 0.f;  // of row lv
+      // rows past the last are read as the first, and not written
+      int row_at[kAt];
+#pragma unroll
+      for (int v = 0; v < kAt; ++v) row_at[v] = (row0 + v * row_ways < nrows ? v * row_ways : 0) * D;
       float o[kAt][kPieces][kVec];
 #pragma unroll
       for (int v = 0; v < kAt; ++v)
@@ -1112,9 +1116,9 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
         for (int u = 0; u < kAt; ++u) {
 #pragma unroll
           for (int v = 0; v < kAt; ++v) {
-            if (j0 + u < nseg && row0 + v * row_ways < nrows) {
+            if (j0 + u < nseg) {
 #pragma unroll
-              for (int q = 0; q < kPieces; ++q) load_vec(src + v * row_ways * D + q * 32 * kVec, x[v][u][q]);
+              for (int q = 0; q < kPieces; ++q) load_vec(src + row_at[v] + q * 32 * kVec, x[v][u][q]);
             }
           }
           src += lse_step * D;
@@ -1138,8 +1142,7 @@ __global__ void __launch_bounds__(kFp4Threads, Fp4Geo<D, NT>::kCtas)
 #pragma unroll
           for (int u = 0; u < kAt; ++u) {
             const float wu = __shfl_sync(0xffffffffu, w, v * kAt + u);
-            // not read above; one whose weight is 0 counts, for its NaNs
-            if (j0 + u >= nseg || row0 + v * row_ways >= nrows) continue;
+            if (j0 + u >= nseg) continue;  // (one whose weight is 0 counts, for its NaNs)
 #pragma unroll
             for (int q = 0; q < kPieces; ++q)
 #pragma unroll
