@@ -20,14 +20,14 @@ constexpr int kMaxDevices = 64;
 // Split cost model of the 4-bit cache (units and meaning as in fd_api.cu: a
 // tile, 128 tokens of one head or 64 of two, costs 8 and a bit).  A pair costs
 // its CTA about 5 us beside its tiles (query, joining, partials, arrival), five
-// tiles' time.  From 45 to 60 it makes little difference; config 3 takes 126 us
-// at 30, 115 at 52 and 119 at 90, 4 speculated tokens of 32 sequences 43.6,
-// 40.6 and 41.6 us.
+// tiles' time.  From 45 to 60 it makes little difference; config 3 takes 135 us
+// at 30, 130 at 52 and 135 at 90, 4 speculated tokens of 32 sequences 48.2,
+// 46.5 and 48.2 us.
 constexpr int kCostTile4 = 2;
 constexpr int kCostSeg4 = 52;
 // Short launches take whole pairs where no CTA gets more than 12 tiles: 64
-// sequences of up to 600 tokens 22.9 -> 22.0 us, eight 1k-token sequences alike,
-// but config 1 (16 tiles) 15.7 -> 20.5.
+// sequences of up to 600 tokens 23.4 -> 22.2 us, eight 1k-token sequences alike,
+// but config 1 (16 tiles) 16.2 -> 20.6.
 constexpr int kAlignTiles4 = 12;
 int cost_tile4() { static const int v = fd::env_int("FD_COST_TILE4", kCostTile4, 0, 64); return v; }
 int cost_seg4() { static const int v = fd::env_int("FD_COST_SEG4", kCostSeg4, 1, 256); return v; }

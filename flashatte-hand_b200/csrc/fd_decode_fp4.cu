@@ -6,9 +6,9 @@
 namespace fd {
 
 // 16 query rows a pass double the multiplications of each byte of K and V but
-// halve the passes (32 sequences of 4096 tokens, 16 rows a KV head: 56 us in
-// one pass, 78 in two; up to 8 rows the second half would be idle: 41 us
-// against 56); at head dim 256 their accumulators do not fit registers.
+// halve the passes (32 sequences of 4096 tokens, 16 rows a KV head: 63 us in
+// one pass, 77 in two; up to 8 rows the second half would be idle: 47 us
+// against 60); at head dim 256 their accumulators do not fit registers.
 int fp4_rows(int head_dim, int64_t qrows) { return head_dim == 256 || qrows <= 8 ? 8 : 16; }
 
 int fp4_max_grid(int head_dim, int rows, int sms) {

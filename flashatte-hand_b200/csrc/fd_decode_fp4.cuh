@@ -53,7 +53,7 @@
 // A CTA is four warps, and a schedule tile four 32-token stages, one a warp:
 // HW = 2 neighbouring KV heads of the same tokens (1 where their number is odd,
 // and in short launches), so that the warps together read 128-byte runs (one
-// head a CTA costs 1.27 times the DRAM traffic, 107 instead of 68 us on config
+// head a CTA costs 1.27 times the DRAM traffic, 104 instead of 69 us on config
 // 2), times 4 / HW stages along the sequence.  Each warp has a ring and a
 // softmax state of its own, and nothing in the loop waits for another warp.
 // The ring runs across segments (a segment is the CTA's part of a sequence's
@@ -62,20 +62,20 @@
 // fd_decode_sm100.cuh, a head of a segment at a time.
 //
 // What bounds it.  32 tokens of K and V of a head at D = 128 are 4.6 KB, 765
-// cycles of a quarter SM's share of the HBM, and 499 instructions of a warp:
-// 128 conversions of code pairs and 84 other ones on the half-rate ALU, 128
-// half-rate f16 multiplications, 32 mma, 38 loads and stores.  Two warps a
-// scheduler overlap these to 831 cycles (840 with the loads from HBM: 6.2
-// TB/s); three (3 CTAs an SM, 168 registers) were 10 to 17 % slower, with more
-// segments for each.  So the loop is written for few instructions (the
+// cycles of a quarter SM's share of the HBM, and with up to four rows 506
+// instructions of a warp: 128 conversions of code pairs and 87 other ones on the
+// half-rate ALU, 128 half-rate f16 multiplications, 32 mma, 38 loads and stores
+// (with 5 to 8 rows 16 mma and some 20 others more).  Two warps a scheduler
+// overlap these to 850 cycles (5.9 to 6.0 TB/s; no fewer from L2); three (3 CTAs
+// an SM, 168 registers) were 10 to 17 % slower, with more segments for each.  So the loop is written for few instructions (the
 // half-rate ones most of all): every five ALU instructions of it are a percent.
 //
-// Measured on a B200 (back-to-back launches; 6.56 TB/s is its copy rate): 64
-// sequences of 4096 tokens, 32 over 8 heads, D = 128: 68.5 us, 4.4 TB/s; two
-// of 262144: 117 us, 5.2 TB/s; the fixed part of a launch is 20 us (first data
-// after 6.5 us: schedule 1.5, first page ids 1.9, query 1.3, data 1.8; 2 to 3
-// us for a segment's end, 1.5 to 5 for a joining, the rest ramps and
-// imbalance).
+// Measured on a B200 (6.56 TB/s is its copy rate): 64 sequences of 4096 tokens,
+// 32 over 8 heads, D = 128: 69.5 us as launches replayed back to back, 4.3 TB/s,
+// and 75 as calls one after another on changing inputs; two of 262144: 119 us,
+// 5.1 TB/s, and 137.  The fixed part of a launch is 20 us (first data after 6.4
+// us: schedule 1.7, first page ids 2.0, query 1.0, data 1.6; 2 to 3 us for a
+// segment's end, 1.5 to 6 for a joining, the rest ramps and imbalance).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -109,7 +109,7 @@ template <int D, int NT> struct Fp4Geo {
   static constexpr int kTileScales = kSubTokens * kScaleBytes;
   static constexpr int kStageBytes = 2 * kTileBytes + 2 * kTileScales;
   static constexpr int kRows = 8 * NT;
-  // CTAs per SM (D = 64: 50.5 us for 64 sequences of 4096 tokens, 52.6 with 2),
+  // CTAs per SM (D = 64: 50.3 us for 64 sequences of 4096 tokens, 51.8 with 2),
   // and stages of a ring: enough for the HBM's latency; 4 at D = 128 and 5 at
   // D = 64 were within 1 % and not better
   static constexpr int kCtas = D == 64 ? 3 : 2;
@@ -245,7 +245,7 @@ template <> __device__ __forceinline__ float2 pair_to_float2<__half>(uint32_t w)
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-// N words (1, 2, 4 or 8) from shared memory in the widest loads.
+// N words (1, 2 or 4) from shared memory in one load.
 template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
   if constexpr (N == 1) {
     w[0] = *reinterpret_cast<const uint32_t*>(p);

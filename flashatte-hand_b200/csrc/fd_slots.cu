@@ -19,8 +19,10 @@
 // the half-rate ALU works in 56 %).  Back 66.5 us, 5.2 TB/s, bound by the
 // latency of slot, codes and store (two rows at a time: 80 registers, 81 us;
 // six CTAs an SM: spilled, 112 us; lanes exchanging halves for whole-sector
-// stores: 64 registers, 72 us).  16-bit rows 9.0 us for 50 MB, 5.6 TB/s; a
-// decode step's rows 3 us, a launch.
+// stores: 64 registers, 72 us).  The same rows into an e4m3 cache 75 us (its
+// divisions are whole ones) and back 64; into a 16-bit one 81, 5.9 TB/s, and
+// back 79.  12k 16-bit rows 9.0 us for 50 MB, 5.6 TB/s; a decode step's rows 3
+// us, a launch.
 #include <cuda_runtime.h>
 
 #include <cstdint>
