@@ -81,12 +81,20 @@ def _new(shape, dtype: torch.dtype, dev: torch.device, stream=None) -> torch.Ten
     there: a block of the current stream's pool may still be read by work
     queued on that stream for its last owner.  The current stream, where the
     caller may use and drop it, is recorded."""
-    if stream is None:
+    if stream is None or stream.cuda_stream == _stream_handle(None, dev):
         return torch.empty(shape, dtype=dtype, device=dev)
-    with torch.cuda.stream(stream):
+    with _on_stream(stream, dev):
         t = torch.empty(shape, dtype=dtype, device=dev)
     t.record_stream(torch.cuda.current_stream(dev))
     return t
+
+
+def _on_stream(stream, dev: torch.device):
+    """Context that makes `stream` current: torch's, or any object that names a
+    stream of `dev` by its cuda_stream."""
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(stream.cuda_stream, device=dev)
+    return torch.cuda.stream(stream)
 
 
 def _require_cuda(*tensors: torch.Tensor) -> None:
@@ -627,7 +635,7 @@ def combine_lse(part_o: torch.Tensor, part_lse: torch.Tensor, out_dtype: torch.d
         raise ValueError("partials must be fp32")
     n, rows, D = part_o.shape
     st = stream if stream is not None else torch.cuda.current_stream(part_o.device)
-    with torch.cuda.stream(st):  # copies are read by the kernel on this stream
+    with _on_stream(st, part_o.device):  # copies are read by the kernel on this stream
         if part_o.stride()[1:] != (D, 1):
             part_o = part_o.contiguous()
         if part_lse.stride(1) != 1:

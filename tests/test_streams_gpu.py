@@ -55,3 +55,19 @@ def test_outputs_of_a_call_on_another_stream(name):
     for x, y in zip(got, want):
         assert torch.equal(x, y)
         assert x.untyped_storage().data_ptr() not in blocks
+
+
+@pytest.mark.parametrize("name", ["flash_decode", "gather_kv", "combine_lse"])
+def test_a_stream_by_its_handle(name):
+    """Any object with a cuda_stream serves, the current stream among them."""
+    class Handle:
+        def __init__(self, stream):
+            self.cuda_stream = stream.cuda_stream
+
+    call = calls()[name]
+    want = call(None)
+    torch.cuda.synchronize()
+    for stream in (torch.cuda.Stream(), torch.cuda.current_stream()):
+        got = call(Handle(stream))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
